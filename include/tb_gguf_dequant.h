@@ -8,7 +8,8 @@
  * link against this library unchanged.  Part 2 adds stream-ordered
  * device-pointer entry points that have no reference counterpart.  Part 3
  * is the batch-1 decode step built on the matvec (a GPU form of
- * layer4/tb_infer.c's tb_infer_decode).
+ * layer4/tb_infer.c's tb_infer_decode).  Part 4 is the paged cache: rotary
+ * append, attention and page copies for many sequences in one pool of pages.
  *
  * Conventions (shared with the reference):
  *   - int returns are 1 = success, 0 = failure (the caller may fall back);
@@ -383,6 +384,148 @@ int    tb_cuda_dec_set_moe_layer(void *dec, int layer, const void *w_router, int
                                  const void *w_gate_up_exps, int gate_up_qtype, const void *w_down_exps,
                                  int down_qtype);
 void   tb_cuda_dec_destroy(void *dec);
+
+/* ───────────── Part 4: the paged cache (no reference counterpart) ────────────
+ *
+ * K and V of many sequences in one pool of pages, the operators on it, and the
+ * host-side bookkeeping of who holds which page.  All of it is independent of
+ * the decoder of part 3.  Element types are ggml's ids 0 (F32), 1 (F16) and
+ * 30 (BF16), for the activations and for the cache, in any combination. */
+
+/* A pool of n_pages pages of page_size positions for each of n_layers layers.
+ * Element (layer, page, head, position, d) of K is k[layer * layer_stride +
+ * page * page_stride + head * head_stride + position * pos_stride + d], V
+ * likewise; strides in elements.  head_dim is 64 or 128; page_size a multiple
+ * of 16, at most 65536; k, v and every stride a multiple of 16 bytes, at least
+ * head_dim, and no two elements at one address. */
+typedef struct {
+    void     *k, *v;
+    int       type, n_layers, n_pages, page_size, n_kv_heads, head_dim;
+    long long layer_stride, page_stride, head_stride, pos_stride;
+} tb_kv_cache;
+
+/* One step's ragged batch.  Sequence s has the new tokens [d_start[s],
+ * d_start[s+1]) (none: an empty range) of the step's rows, d_len[s] positions
+ * including them (its new token i sits at position d_len[s] - new + i), and
+ * position p in page d_pages[s * pages_stride + p / page_size].  The arrays
+ * are device memory, read by the kernels.  n_tokens: rows in the step's
+ * buffers (rows outside every sequence are left alone); max_new and max_len:
+ * the most new tokens and positions of any sequence; they only choose between
+ * kernels, and the results are right for any value.
+ * A sequence whose range leaves [0, n_tokens], whose new tokens outnumber its
+ * positions or whose positions outnumber its table's sets the error word (2)
+ * and is skipped, its rows of the output zero; so does a page outside the
+ * pool, whose positions then count as hidden and are not stored to. */
+typedef struct {
+    const int *d_start, *d_len, *d_pages;
+    int        n_seqs, n_tokens, max_new, max_len, pages_stride;
+} tb_kv_batch;
+
+/* Rows of heads: element (token t, head h, d) is p[t * row + h * head + d]
+ * (strides in elements; p and both strides multiples of 16 bytes). */
+typedef struct {
+    const void *p;
+    long long   row, head;
+} tb_kv_rows;
+
+/* What tb_cuda_kv_append_dev does to q and k before it stores them.
+ * d_table: [n_pos][rot_dim / 2][2] fp32 (cos, sin) as tb_cuda_rope_table_dev
+ * fills it (NULL: no rotation); the first rot_dim (even, <= head_dim)
+ * dimensions of a head rotate, in pairs (2 i, 2 i + 1) when interleaved, else
+ * (i, i + rot_dim / 2).  d_q_norm / d_k_norm: [head_dim] fp32 weights of a
+ * per-head RMS norm that comes before the rotation (NULL: none). */
+typedef struct {
+    const float *d_table, *d_q_norm, *d_k_norm;
+    int          n_pos, rot_dim, interleaved;
+    float        eps;
+} tb_kv_rope;
+
+/* How rotary angles are scaled for contexts past the trained one.  Pair i of
+ * rot_dim / 2 turns by f_i = base^(-2 i / rot_dim) a position, then
+ *   mode 0  unscaled;
+ *   mode 1  f_i / factor (linear position interpolation);
+ *   mode 2  base * factor^(rot_dim / (rot_dim - 2)) in the place of base;
+ *   mode 3  by parts (YaRN, Peng et al. 2023): with r_i = orig_len f_i / 2 pi
+ *           turns over the trained context and g = clamp((r_i - beta_slow) /
+ *           (beta_fast - beta_slow), 0, 1): f_i (g + (1 - g) / factor).
+ * cos and sin are multiplied by attn_factor (0: 1, or 0.1 ln(factor) + 1 in
+ * mode 3).  Modes 1-3: factor >= 1; mode 3: orig_len > 0 and beta_fast >
+ * beta_slow (both 0: 32 and 1). */
+typedef struct {
+    double base, factor, beta_fast, beta_slow, attn_factor;
+    int    mode, orig_len;
+} tb_rope_scale;
+
+/* Fills d_table[n_pos][rot_dim / 2][2] with cos and sin of position * angle,
+ * computed in 64 bits and rounded once.  Stream-ordered.  1 = issued. */
+int    tb_cuda_rope_table_dev(float *d_table, int n_pos, int rot_dim, const tb_rope_scale *s, void *stream);
+
+/* The step's new rows: q [n_tokens][n_heads] is normed and rotated into q_out
+ * (io_type both; may be the same rows), k and v [n_tokens][n_kv_heads]
+ * (io_type) go to their positions of the layer's pages, k normed and rotated,
+ * both rounded to the cache's type.  n_heads is a multiple of the cache's
+ * n_kv_heads.  All arithmetic is fp32.  rope NULL: copies.  A position past
+ * the table sets the error word (2) and its token is skipped.  Pages shared
+ * between sequences must not be appended to (tb_cuda_kv_pool_extend copies
+ * them first).  Stream-ordered.  1 = issued, 0 = refused arguments or a launch
+ * error. */
+int    tb_cuda_kv_append_dev(const tb_kv_cache *cache, int layer, const tb_kv_batch *batch, int io_type, int n_heads,
+                             const tb_kv_rows *q, const tb_kv_rows *k, const tb_kv_rows *v, const tb_kv_rows *q_out,
+                             const tb_kv_rope *rope, void *stream);
+
+/* Attention of the step's new tokens over their sequences' pages (the new ones
+ * appended before): the token at position i sees the positions j <= i, with
+ * window > 0 only those with i - j < window or j < sinks;
+ *   out[t][h] = sum_j softmax_j(scale * q[t][h] . k[j]) v[j]
+ * with kv head h / (n_heads / n_kv_heads).  A row that sees nothing is zero.
+ * Hidden positions have no influence, whatever bits they hold.  Scores,
+ * softmax and sums are fp32; fp32 activations keep fp32 accuracy over any
+ * cache type; 16-bit activations over a cache of the same type may round the
+ * softmax numerators to that type before the second product.  d_ws: workspace
+ * of tb_cuda_kv_attend_ws() bytes, 16-byte aligned, zeroed once before its
+ * first call and left zeroed where it matters by every call; calls that may
+ * overlap on the GPU need one each.  Stream-ordered.  1 = issued. */
+size_t tb_cuda_kv_attend_ws(void);
+int    tb_cuda_kv_attend_dev(const tb_kv_cache *cache, int layer, const tb_kv_batch *batch, int io_type, int n_heads,
+                             const tb_kv_rows *q, const tb_kv_rows *out, float scale, int window, int sinks,
+                             void *d_ws, size_t ws_bytes, void *stream);
+
+/* Pages dst[i] = pages src[i] for i < n, K and V of every layer.  src and dst
+ * are host memory, free to be reused on return.  Sources may repeat; a
+ * destination that is given twice or is also a source is refused, so the order
+ * of the copies cannot matter.  Stream-ordered.  1 = issued. */
+int    tb_cuda_kv_copy_dev(const tb_kv_cache *cache, const int *src, const int *dst, int n, void *stream);
+
+/* Host bookkeeping of a pool's pages (launches nothing, needs no device; a
+ * handle is not thread-safe).  Sequences are small integers, reused after
+ * tb_cuda_kv_pool_free; pages are counted by the sequences that hold them. */
+void  *tb_cuda_kv_pool_create(int n_pages, int page_size);
+void   tb_cuda_kv_pool_destroy(void *pool);
+/* A new empty sequence; -1 on failure. */
+int    tb_cuda_kv_pool_new(void *pool);
+/* A new sequence with the same positions, sharing every page; -1 on failure. */
+int    tb_cuda_kv_pool_fork(void *pool, int seq);
+/* Room for n more positions.  When the last page is part-filled and shared,
+ * the sequence gets a copy of its own first: the caller must copy *src to *dst
+ * (tb_cuda_kv_copy_dev) before anything is appended.  Returns the number of
+ * such copies (0 or 1), or -1 with nothing changed (unknown sequence, n < 0,
+ * too few free pages, or more than INT_MAX positions). */
+int    tb_cuda_kv_pool_extend(void *pool, int seq, int n, int *src, int *dst);
+/* Drops the positions from len on (0 <= len <= its length).  1 = ok. */
+int    tb_cuda_kv_pool_truncate(void *pool, int seq, int len);
+/* Ends the sequence; its unshared pages are free again.  1 = ok. */
+int    tb_cuda_kv_pool_free(void *pool, int seq);
+/* Moves the pages in use into the lowest page numbers: fills src / dst with at
+ * most cap moves (the caller copies them before the next step) and changes
+ * every sequence's table accordingly.  Returns the number of moves; the pool
+ * is compact when that is less than cap; -1 for bad arguments. */
+int    tb_cuda_kv_pool_compact(void *pool, int *src, int *dst, int cap);
+/* The sequence's length in positions, -1 if unknown. */
+int    tb_cuda_kv_pool_len(void *pool, int seq);
+/* Its pages in order, at most cap of them; returns how many it has, -1 if unknown. */
+int    tb_cuda_kv_pool_pages(void *pool, int seq, int *pages, int cap);
+/* Pages that no sequence holds. */
+int    tb_cuda_kv_pool_free_pages(void *pool);
 
 #ifdef __cplusplus
 }

@@ -32,6 +32,36 @@ class DecLayer(ctypes.Structure):
                 ("q_norm", ctypes.c_void_p), ("k_norm", ctypes.c_void_p)]
 
 
+class KvCache(ctypes.Structure):
+    """tb_kv_cache (include/tb_gguf_dequant.h, part 4)."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p)] + \
+               [(n, ctypes.c_int) for n in ("type", "n_layers", "n_pages", "page_size", "n_kv_heads", "head_dim")] + \
+               [(n, ctypes.c_longlong) for n in ("layer_stride", "page_stride", "head_stride", "pos_stride")]
+
+
+class KvBatch(ctypes.Structure):
+    """tb_kv_batch (include/tb_gguf_dequant.h, part 4)."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("d_start", "d_len", "d_pages")] + \
+               [(n, ctypes.c_int) for n in ("n_seqs", "n_tokens", "max_new", "max_len", "pages_stride")]
+
+
+class KvRows(ctypes.Structure):
+    """tb_kv_rows (include/tb_gguf_dequant.h, part 4)."""
+    _fields_ = [("p", ctypes.c_void_p), ("row", ctypes.c_longlong), ("head", ctypes.c_longlong)]
+
+
+class KvRope(ctypes.Structure):
+    """tb_kv_rope (include/tb_gguf_dequant.h, part 4)."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("d_table", "d_q_norm", "d_k_norm")] + \
+               [(n, ctypes.c_int) for n in ("n_pos", "rot_dim", "interleaved")] + [("eps", ctypes.c_float)]
+
+
+class RopeScale(ctypes.Structure):
+    """tb_rope_scale (include/tb_gguf_dequant.h, part 4)."""
+    _fields_ = [(n, ctypes.c_double) for n in ("base", "factor", "beta_fast", "beta_slow", "attn_factor")] + \
+               [("mode", ctypes.c_int), ("orig_len", ctypes.c_int)]
+
+
 def lib() -> ctypes.CDLL:
     global _lib
     if _lib is not None:
@@ -92,6 +122,25 @@ def lib() -> ctypes.CDLL:
         "tb_cuda_dec_set_sampling": (c_int, [c_void_p, ctypes.c_float, c_int, ctypes.c_float]),
         "tb_cuda_dec_generate_u": (c_int, [c_void_p, c_int, c_int, c_int, fp, ctypes.POINTER(c_int), fp, fp]),
         "tb_cuda_dec_destroy": (None, [c_void_p]),
+        "tb_cuda_rope_table_dev": (c_int, [c_void_p, c_int, c_int, ctypes.POINTER(RopeScale), c_void_p]),
+        "tb_cuda_kv_append_dev": (c_int, [ctypes.POINTER(KvCache), c_int, ctypes.POINTER(KvBatch), c_int, c_int] +
+                                  [ctypes.POINTER(KvRows)] * 4 + [ctypes.POINTER(KvRope), c_void_p]),
+        "tb_cuda_kv_attend_ws": (c_size_t, []),
+        "tb_cuda_kv_attend_dev": (c_int, [ctypes.POINTER(KvCache), c_int, ctypes.POINTER(KvBatch), c_int, c_int] +
+                                  [ctypes.POINTER(KvRows)] * 2 +
+                                  [ctypes.c_float, c_int, c_int, c_void_p, c_size_t, c_void_p]),
+        "tb_cuda_kv_copy_dev": (c_int, [ctypes.POINTER(KvCache), c_void_p, c_void_p, c_int, c_void_p]),
+        "tb_cuda_kv_pool_create": (c_void_p, [c_int, c_int]),
+        "tb_cuda_kv_pool_destroy": (None, [c_void_p]),
+        "tb_cuda_kv_pool_new": (c_int, [c_void_p]),
+        "tb_cuda_kv_pool_fork": (c_int, [c_void_p, c_int]),
+        "tb_cuda_kv_pool_extend": (c_int, [c_void_p, c_int, c_int, ctypes.POINTER(c_int), ctypes.POINTER(c_int)]),
+        "tb_cuda_kv_pool_truncate": (c_int, [c_void_p, c_int, c_int]),
+        "tb_cuda_kv_pool_free": (c_int, [c_void_p, c_int]),
+        "tb_cuda_kv_pool_compact": (c_int, [c_void_p, c_void_p, c_void_p, c_int]),
+        "tb_cuda_kv_pool_len": (c_int, [c_void_p, c_int]),
+        "tb_cuda_kv_pool_pages": (c_int, [c_void_p, c_int, c_void_p, c_int]),
+        "tb_cuda_kv_pool_free_pages": (c_int, [c_void_p]),
     }
     for name, (res, args) in sig.items():
         f = getattr(L, name)
@@ -116,4 +165,8 @@ def exported_symbols() -> list[str]:
         "tb_cuda_dec_tp_handle", "tb_cuda_dec_tp_connect", "tb_cuda_dec_create_moe", "tb_cuda_dec_create_moe_tp", "tb_cuda_dec_set_moe_layer",
         "tb_cuda_dec_step", "tb_cuda_dec_prefill", "tb_cuda_dec_generate", "tb_cuda_dec_set_sampling", "tb_cuda_dec_generate_u",
         "tb_cuda_dec_destroy",
+        "tb_cuda_rope_table_dev", "tb_cuda_kv_append_dev", "tb_cuda_kv_attend_ws", "tb_cuda_kv_attend_dev",
+        "tb_cuda_kv_copy_dev", "tb_cuda_kv_pool_create", "tb_cuda_kv_pool_destroy", "tb_cuda_kv_pool_new",
+        "tb_cuda_kv_pool_fork", "tb_cuda_kv_pool_extend", "tb_cuda_kv_pool_truncate", "tb_cuda_kv_pool_free",
+        "tb_cuda_kv_pool_compact", "tb_cuda_kv_pool_len", "tb_cuda_kv_pool_pages", "tb_cuda_kv_pool_free_pages",
     ])

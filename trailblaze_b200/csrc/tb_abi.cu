@@ -15,14 +15,17 @@
 // launch fail (return 0/NULL) without touching the GPU.  TB_WAIT_LIMIT sets
 // the poll limit of the kernels' bounded pipeline waits.
 #include <atomic>
+#include <cmath>
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
 #include <mutex>
+#include <utility>
 
 #include "../../include/tb_gguf_dequant.h"
 #include "tb_common.cuh"
 #include "tb_internal.h"
+#include "tb_paged.cuh"
 
 namespace {
 
@@ -152,6 +155,77 @@ const NaDev *na_device_locked()
     g_na[g_nna] = d;
     return &g_na[g_nna++];
 }
+
+// ---- argument checks of the paged cache's entry points (part 4) ----
+int kv_esize(int type) { return type == tb::QT_F32 ? 4 : type == tb::QT_F16 || type == tb::QT_BF16 ? 2 : 0; }
+
+// True when no two elements of a strided array share an address: each
+// dimension, in order of stride, steps over what the smaller ones span.
+bool kv_disjoint(long long extent, int n, long long (*dims)[2])
+{
+    for (int i = 0; i < n; ++i)
+        for (int j = i + 1; j < n; ++j)
+            if (dims[j][0] < dims[i][0]) std::swap(dims[i], dims[j]);
+    for (int i = 0; i < n; ++i) {
+        const long long stride = dims[i][0], count = dims[i][1];
+        if (count <= 1) continue;
+        if (stride < extent || stride > (1ll << 60) / count) return false;
+        extent += stride * (count - 1);
+    }
+    return true;
+}
+
+bool kv_cache_ok(const tb_kv_cache *c, int layer)
+{
+    if (!c || !c->k || !c->v) return false;
+    const int es = kv_esize(c->type);
+    if (!es || (c->head_dim != 64 && c->head_dim != 128) || c->page_size <= 0 || c->page_size % 16 ||
+        c->page_size > 65536 || c->n_layers <= 0 || c->n_layers > 65535 || c->n_pages <= 0 || c->n_kv_heads <= 0 ||
+        layer < 0 || layer >= c->n_layers)
+        return false;
+    if ((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) & 15u) return false;
+    long long d[4][2] = {{c->layer_stride, c->n_layers},
+                         {c->page_stride, c->n_pages},
+                         {c->head_stride, c->n_kv_heads},
+                         {c->pos_stride, c->page_size}};
+    // 2^39 bytes and up do not fit a tensor map's strides
+    for (auto &e : d)
+        if (e[0] < c->head_dim || (e[0] * es) % 16 || e[0] > (1ll << 37)) return false;
+    return kv_disjoint(c->head_dim, 4, d);
+}
+
+bool kv_batch_ok(const tb_kv_batch *b)
+{
+    return b && b->n_seqs >= 0 && b->n_tokens >= 0 && b->max_new >= 0 && b->max_len >= 0 && b->pages_stride >= 0 &&
+           (b->n_seqs == 0 || (b->d_start && b->d_len && (b->d_pages || b->pages_stride == 0)));
+}
+
+bool kv_rows_ok(const tb_kv_rows *r, int type, int n_tokens, int heads, int hd, bool written)
+{
+    const int es = kv_esize(type);
+    if (!r || !es) return false;
+    if (n_tokens == 0) return true;
+    if (!r->p || (reinterpret_cast<uintptr_t>(r->p) & 15u) || r->row < 0 || r->head < 0 || (r->row * es) % 16 ||
+        (r->head * es) % 16 || r->row > (1ll << 40) || r->head > (1ll << 40))
+        return false;
+    long long d[2][2] = {{r->row, n_tokens}, {r->head, heads}};
+    return !written || kv_disjoint(hd, 2, d);
+}
+
+tb::KvView kv_view(const tb_kv_cache *c, int layer)
+{
+    const long long off = layer * c->layer_stride * kv_esize(c->type);
+    return tb::KvView{static_cast<const char *>(c->k) + off, static_cast<const char *>(c->v) + off, c->page_stride,
+                      c->head_stride, c->pos_stride, c->n_pages, c->page_size, c->n_kv_heads,
+                      tb::make_fastdiv(static_cast<uint32_t>(c->page_size))};
+}
+
+tb::KvBatch kv_batch(const tb_kv_batch *b)
+{
+    return tb::KvBatch{b->d_start, b->d_len, b->d_pages, b->n_seqs, b->n_tokens, b->pages_stride};
+}
+
+tb::KvRows kv_rows(const tb_kv_rows *r) { return tb::KvRows{r->p, r->row, r->head}; }
 
 }  // namespace
 
@@ -499,6 +573,104 @@ int tb_cuda_matvec_device_noalloc(const void *W_device, int qtype, int M, int K,
         return 0;
     }
     return 1;
+}
+
+int tb_cuda_rope_table_dev(float *d_table, int n_pos, int rot_dim, const tb_rope_scale *s, void *stream)
+{
+    if (!d_table || (reinterpret_cast<uintptr_t>(d_table) & 7u) || n_pos < 0 || rot_dim <= 0 || rot_dim % 2 || !s ||
+        s->mode < 0 || s->mode > 3 || !(s->base > 0.0 && s->base < 1e300) || !(s->attn_factor >= 0.0))
+        return 0;
+    if (s->mode > 0 && !(s->factor >= 1.0 && s->factor < 1e300)) return 0;
+    if (s->mode == 2 && rot_dim <= 2) return 0;
+    double fast = s->beta_fast, slow = s->beta_slow;
+    if (fast == 0.0 && slow == 0.0) fast = 32.0, slow = 1.0;
+    if (s->mode == 3 && !(s->orig_len > 0 && fast > slow)) return 0;
+    const double attn = s->attn_factor > 0.0 ? s->attn_factor : s->mode == 3 ? 0.1 * log(s->factor) + 1.0 : 1.0;
+    if (n_pos == 0) return 1;
+    {
+        std::lock_guard<std::mutex> lk(g_mu);
+        if (!ensure_init_locked(false)) return 0;
+    }
+    const int r = tb::rope_table_launch(d_table, n_pos, rot_dim, s->base, s->factor, fast, slow, s->orig_len, attn,
+                                        s->mode, static_cast<cudaStream_t>(stream));
+    if (r) g_launches.fetch_add(1, std::memory_order_relaxed);
+    return r;
+}
+
+int tb_cuda_kv_append_dev(const tb_kv_cache *cache, int layer, const tb_kv_batch *batch, int io_type, int n_heads,
+                          const tb_kv_rows *q, const tb_kv_rows *k, const tb_kv_rows *v, const tb_kv_rows *q_out,
+                          const tb_kv_rope *rope, void *stream)
+{
+    if (!kv_cache_ok(cache, layer) || !kv_batch_ok(batch) || n_heads <= 0 || n_heads % cache->n_kv_heads) return 0;
+    const int t = batch->n_tokens, hd = cache->head_dim;
+    if (!kv_rows_ok(q, io_type, t, n_heads, hd, false) || !kv_rows_ok(k, io_type, t, cache->n_kv_heads, hd, false) ||
+        !kv_rows_ok(v, io_type, t, cache->n_kv_heads, hd, false) || !kv_rows_ok(q_out, io_type, t, n_heads, hd, true))
+        return 0;
+    tb_kv_rope r{};
+    if (rope) r = *rope;
+    if (r.d_table && ((reinterpret_cast<uintptr_t>(r.d_table) & 7u) || r.n_pos < 0 || r.rot_dim <= 0 || r.rot_dim % 2 ||
+                      r.rot_dim > hd))
+        return 0;
+    if (((reinterpret_cast<uintptr_t>(r.d_q_norm) | reinterpret_cast<uintptr_t>(r.d_k_norm)) & 15u) ||
+        ((r.d_q_norm || r.d_k_norm) && !(r.eps >= 0.f)))
+        return 0;
+    if (t == 0 || batch->n_seqs == 0) return 1;
+    int nsm, *derr;
+    {
+        std::lock_guard<std::mutex> lk(g_mu);
+        if (!ensure_init_locked(false)) return 0;
+        nsm = g.num_sms;
+        derr = g.d_err;
+    }
+    const int ok = tb::kv_append_launch(kv_view(cache, layer), kv_batch(batch), hd, io_type, cache->type, n_heads,
+                                        kv_rows(q), kv_rows(k), kv_rows(v), kv_rows(q_out), r.d_table, r.d_q_norm,
+                                        r.d_k_norm, r.n_pos, r.d_table ? r.rot_dim : 0, r.interleaved != 0, r.eps, derr,
+                                        nsm, static_cast<cudaStream_t>(stream));
+    if (ok) g_launches.fetch_add(1, std::memory_order_relaxed);
+    return ok;
+}
+
+size_t tb_cuda_kv_attend_ws(void) { return tb::kv_attend_ws(); }
+
+int tb_cuda_kv_attend_dev(const tb_kv_cache *cache, int layer, const tb_kv_batch *batch, int io_type, int n_heads,
+                          const tb_kv_rows *q, const tb_kv_rows *out, float scale, int window, int sinks, void *d_ws,
+                          size_t ws_bytes, void *stream)
+{
+    if (!kv_cache_ok(cache, layer) || !kv_batch_ok(batch) || n_heads <= 0 || n_heads % cache->n_kv_heads ||
+        !std::isfinite(scale) || window < 0 || sinks < 0)
+        return 0;
+    const int t = batch->n_tokens, hd = cache->head_dim;
+    if (!kv_rows_ok(q, io_type, t, n_heads, hd, false) || !kv_rows_ok(out, io_type, t, n_heads, hd, true)) return 0;
+    if (!d_ws || (reinterpret_cast<uintptr_t>(d_ws) & 15u) || ws_bytes < tb::kv_attend_ws()) return 0;
+    if (t == 0 || batch->n_seqs == 0) return 1;
+    int nsm, *derr;
+    {
+        std::lock_guard<std::mutex> lk(g_mu);
+        if (!ensure_init_locked(false)) return 0;
+        nsm = g.num_sms;
+        derr = g.d_err;
+    }
+    const int ok = tb::kv_attend_launch(kv_view(cache, layer), kv_batch(batch), hd, io_type, cache->type, n_heads,
+                                        kv_rows(q), kv_rows(out), scale, window, sinks, batch->max_new, batch->max_len,
+                                        d_ws, derr, nsm, static_cast<cudaStream_t>(stream));
+    if (ok) g_launches.fetch_add(1, std::memory_order_relaxed);
+    return ok;
+}
+
+int tb_cuda_kv_copy_dev(const tb_kv_cache *cache, const int *src, const int *dst, int n, void *stream)
+{
+    if (!kv_cache_ok(cache, 0) || n < 0 || (n > 0 && (!src || !dst))) return 0;
+    if (n == 0) return 1;
+    {
+        std::lock_guard<std::mutex> lk(g_mu);
+        if (!ensure_init_locked(false)) return 0;
+    }
+    const int ok = tb::kv_copy_launch(cache->k, cache->v, kv_esize(cache->type), cache->n_layers, cache->n_pages,
+                                      cache->page_size, cache->n_kv_heads, cache->head_dim, cache->layer_stride,
+                                      cache->page_stride, cache->head_stride, cache->pos_stride, src, dst, n,
+                                      static_cast<cudaStream_t>(stream));
+    if (ok) g_launches.fetch_add(1, std::memory_order_relaxed);
+    return ok;
 }
 
 }  // extern "C"
