@@ -644,15 +644,17 @@ int tb_cuda_kv_attend_dev(const tb_kv_cache *cache, int layer, const tb_kv_batch
     if (!d_ws || (reinterpret_cast<uintptr_t>(d_ws) & 15u) || ws_bytes < tb::kv_attend_ws()) return 0;
     if (t == 0 || batch->n_seqs == 0) return 1;
     int nsm, *derr;
+    uint32_t lim;
     {
         std::lock_guard<std::mutex> lk(g_mu);
         if (!ensure_init_locked(false)) return 0;
         nsm = g.num_sms;
         derr = g.d_err;
+        lim = g.wait_limit;
     }
     const int ok = tb::kv_attend_launch(kv_view(cache, layer), kv_batch(batch), hd, io_type, cache->type, n_heads,
                                         kv_rows(q), kv_rows(out), scale, window, sinks, batch->max_new, batch->max_len,
-                                        d_ws, derr, nsm, static_cast<cudaStream_t>(stream));
+                                        d_ws, derr, nsm, lim, static_cast<cudaStream_t>(stream));
     if (ok) g_launches.fetch_add(1, std::memory_order_relaxed);
     return ok;
 }

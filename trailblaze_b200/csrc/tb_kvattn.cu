@@ -1,5 +1,34 @@
 // tb_kvattn.cu — attention of a step's new tokens over the paged cache
 // (include/tb_gguf_dequant.h part 4, tb_cuda_kv_attend_dev).
+//
+// k_kv_few: few query rows per kv head (single tokens, short chunks), bound by
+// the cache's bytes.
+//
+// An item is (sequence, kv head, 8 query rows): row r of a sequence's n * G rows
+// (G = query heads per kv head) is new token r / G, head r % G of the group.  Its
+// positions come in slices of 16 (16 divides a page), a step is one slice for
+// each of the CTA's W warps.  All items' steps, laid end to end, are cut into
+// equal parts, one per CTA, whatever the sequences' lengths: a CTA works through
+// the end of one item, whole items, and the beginning of another.  Items that lie
+// in one CTA are written out directly, the others' parts go to the workspace and
+// the last CTA to arrive adds them in CTA order, so results repeat bit for bit.
+//
+// Each warp streams its own slices of K and V through its own ring of TMA copies
+// (128-byte swizzle, one mbarrier a stage), with no CTA barrier inside an item.
+// The products run on mma.sync with the query rows as N = 8 (a decode step has 4
+// to 8 of them; as M they would waste half or more of a 16-row tile and twice the
+// registers): S^T[16 positions][8 rows] = K Q^T, O^T[dim][8 rows] += V^T P^T.
+// tcgen05's smallest tile is 64 rows of M: at this arithmetic intensity the
+// tensor pipe idles either way.
+//
+// Precision: 16-bit activations over a cache of their type multiply as they are;
+// P goes in as a high and a low 16-bit part.  fp32 activations are split into
+// parts of the cache's type (3 bf16, or 2 fp16 of a row scaled by a power of two
+// so that its largest element is near 2^13); an fp32 cache is split into two
+// tf32 parts, of which the low-low product is dropped (2^-22).  Scores, softmax and
+// sums are fp32.
+#include <cuda.h>
+
 #include <cmath>
 #include <cstdio>
 
@@ -11,66 +40,795 @@ struct AttnArgs {
     KvView c;
     KvBatch b;
     KvRows q, o;
-    int nh, window, sinks;
+    int nh, group, window, sinks;
     float scale2;   // scale * log2(e)
     int *err;
+    uint32_t wait_limit;
+    int ax_pos, ax_head, ax_page;   // the tensor maps' axes 1..3: which of them is which
+    float *part;                    // [2 * gridDim.x] partial results
+    unsigned *arrived;              // [gridDim.x] arrival counters, zero between calls
 };
 
-// One warp per (row, head), fp32, a position at a time.
-template <int HD, int TI, int TC>
-__global__ void __launch_bounds__(256) k_kv_rows(const AttnArgs a)
+// ---- PTX ----
+__device__ __forceinline__ void ldsm4(uint32_t a, uint32_t (&r)[4])
 {
-    using I = typename KvType<TI>::E;
-    using C = typename KvType<TC>::E;
-    constexpr int D = HD / 32;
-    __shared__ int s_at;
-    const int t = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int s = kv_seq_of_row(a.b, t, &s_at, a.err);
-    if (s < 0) return;
-    KvSeq sq;
-    const bool ok = kv_seq(a.b, a.c, s, sq, a.err);
-    const int pos = sq.len - sq.n + (t - sq.row0);
-    for (int h = blockIdx.y * 8 + warp; h < a.nh; h += gridDim.y * 8) {
-        float q[D], acc[D], m, l;
-        const I *qp = static_cast<const I *>(a.q.p) + t * a.q.row + h * a.q.head + lane * D;
-#pragma unroll
-        for (int d = 0; d < D; ++d) q[d] = kv_f(qp[d]) * a.scale2;
-        kv_row_attend<HD, C>(a.b, a.c, s, h / (a.nh / a.c.n_kv_heads), pos, 0, ok ? sq.len : 0, a.window, a.sinks, q, m,
-                             l, acc, a.err);
-        I *op = static_cast<I *>(const_cast<void *>(a.o.p)) + t * a.o.row + h * a.o.head + lane * D;
-#pragma unroll
-        for (int d = 0; d < D; ++d) kv_store1(op + d, m == -INFINITY ? 0.f : acc[d] / l);
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(a)
+                 : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t a, uint32_t (&r)[4])
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(a)
+                 : "memory");
+}
+__device__ __forceinline__ uint32_t mat_t(uint32_t x)   // transpose of an 8 x 8 matrix of 16-bit elements
+{
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+template <int TC>
+__device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+    if constexpr (TC == QT_BF16)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                     "{%0, %1, %2, %3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                     "{%0, %1, %2, %3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                 "{%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float ex2(float x)   // 2^x, 2 ulp; 0 for -inf
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map, int x, int y, int z, int w, uint32_t bar)
+{
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, "
+                 "%5}], [%6];" ::"r"(dst),
+                 "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
+                 : "memory");
+}
+
+// x = hi + lo, hi rounded to tf32 (10 bits of mantissa); the tensor core reads
+// lo's upper 19 bits: what is lost lies 2^-21 below x and has no preferred sign.
+__device__ __forceinline__ void split_tf32(uint32_t x, uint32_t &hi, uint32_t &lo)
+{
+    hi = (x + 0x1000u) & 0xFFFFE000u;
+    lo = __float_as_uint(__uint_as_float(x) - __uint_as_float(hi));
+}
+// Two fp32 as a pair of 16-bit elements, and what the rounding left over.
+template <int TC>
+__device__ __forceinline__ uint32_t pack16(float &x, float &y)
+{
+    uint32_t w;
+    if constexpr (TC == QT_BF16) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+        w = *reinterpret_cast<const uint32_t *>(&h);
+        x -= __uint_as_float(w << 16);
+        y -= __uint_as_float(w & 0xFFFF0000u);
+    } else {
+        const __half2 h = __floats2half2_rn(x, y);
+        w = *reinterpret_cast<const uint32_t *>(&h);
+        const float2 f = __half22float2(h);
+        x -= f.x;
+        y -= f.y;
+    }
+    return w;
+}
+
+// ---- the layout of an item's positions ----
+static constexpr int kSlice = 16;
+
+// The slices that any row of a sequence sees: [0, ns) and [lo, lo + n - ns).
+struct KvSlices {
+    int ns, lo, n;
+};
+__device__ __forceinline__ KvSlices kv_slices(const KvSeq &q, int window, int sinks)
+{
+    const KvSpan sp = kv_span(q.len - q.n, window, sinks);   // of the first row, which sees furthest back
+    const int all = (q.len + kSlice - 1) / kSlice;
+    KvSlices s{0, 0, all};
+    if (sinks < sp.lo) {
+        s.ns = (sinks + kSlice - 1) / kSlice;
+        s.lo = sp.lo / kSlice > s.ns ? sp.lo / kSlice : s.ns;
+        s.n = s.ns + all - s.lo;
+    }
+    return s;
+}
+
+struct FewShared {
+    float m[4][8], l[4][8];   // [warp][row]
+    unsigned long long scan[4], at;
+    int seq, fail, last, bad[8];
+};
+
+template <int HD, int TI, int TC>
+struct FewCfg {
+    static constexpr int ES = TC == QT_F32 ? 4 : 2;
+    static constexpr int W = 4;                                 // warps
+    static constexpr int SB = 2 * kSlice * HD * ES;             // bytes of a slice, K and V
+    static constexpr int NST = SB >= 16384 ? 3 : SB >= 8192 ? 3 : 6;
+    static constexpr int CTAS = SB >= 16384 ? 1 : 2;            // per SM
+    static constexpr int NQ = TC == QT_F32 ? 2 : TI == TC ? 1 : TC == QT_BF16 ? 3 : 2;
+    static constexpr int NP = TC == QT_BF16 && TI == QT_F32 ? 3 : 2;
+    static constexpr int MERGE = W * 8 * HD * 4;
+    // Rings, merge buffer, barriers, FewShared.  Nothing static and no slack for
+    // alignment, so that two CTAs fit an SM: the block's window begins on a 1 KB
+    // boundary, which the kernel checks.
+    static constexpr int SMEM = W * NST * SB + MERGE + W * NST * 8 + static_cast<int>(sizeof(FewShared));
+};
+// floats of one partial result: 8 rows of O, then m and l of each
+__host__ __device__ constexpr int few_part(int hd) { return 8 * hd + 16; }
+
+// A place in the sequence of all items' steps.
+struct KvCur {
+    int s, h, rt, step;     // sequence, kv head, row tile, step
+    KvSeq q;
+    KvSlices sl;
+    int tiles, steps;       // row tiles per head, steps per item
+};
+
+template <int W>
+__device__ __forceinline__ void kv_cur_seq(const AttnArgs &a, KvCur &c)
+{
+    // sequences that cannot be are skipped here; the scan has reported them
+    while (c.s < a.b.n_seqs && (!kv_seq(a.b, a.c, c.s, c.q, nullptr) || c.q.n == 0)) ++c.s;
+    if (c.s >= a.b.n_seqs) return;
+    c.sl = kv_slices(c.q, a.window, a.sinks);
+    c.tiles = (c.q.n * a.group + 7) >> 3;
+    c.steps = (c.sl.n + W - 1) / W;
+}
+
+template <int W>
+__device__ __forceinline__ unsigned long long kv_seq_steps(const AttnArgs &a, int s, bool &bad)
+{
+    KvSeq q;
+    if (!kv_seq(a.b, a.c, s, q, nullptr)) {
+        bad = true;
+        return 0;
+    }
+    if (q.n == 0) return 0;
+    const KvSlices sl = kv_slices(q, a.window, a.sinks);
+    const unsigned long long tiles = (static_cast<unsigned long long>(q.n) * a.group + 7) >> 3;
+    return tiles * a.c.n_kv_heads * static_cast<unsigned>((sl.n + W - 1) / W);
+}
+
+// The rows of sequences whose numbers contradict each other: the error word, and
+// zeros as far as the rows exist (one CTA, all its threads).
+template <int HD, class I>
+__device__ void kv_zero_bad(const AttnArgs &a)
+{
+    for (int s = 0; s < a.b.n_seqs; ++s) {
+        KvSeq q;
+        if (kv_seq(a.b, a.c, s, q, a.err)) continue;
+        const int lo = max(0, a.b.start[s]), hi = min(a.b.n_tokens, a.b.start[s + 1]);
+        const long long n = static_cast<long long>(max(0, hi - lo)) * a.nh * HD;
+        for (long long e = threadIdx.x; e < n; e += blockDim.x) {
+            const long long th = e / HD;
+            kv_store1(static_cast<I *>(const_cast<void *>(a.o.p)) + (lo + th / a.nh) * a.o.row + (th % a.nh) * a.o.head +
+                          e % HD,
+                      0.f);
+        }
     }
 }
 
-template <int HD, int TI>
-static void *rows_kernel(int tc)
+template <int HD, int TI, int TC>
+__global__ void __launch_bounds__(FewCfg<HD, TI, TC>::W * 32, FewCfg<HD, TI, TC>::CTAS)
+    k_kv_few(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const AttnArgs a)
 {
-    return tc == QT_F32 ? reinterpret_cast<void *>(k_kv_rows<HD, TI, QT_F32>)
-         : tc == QT_F16 ? reinterpret_cast<void *>(k_kv_rows<HD, TI, QT_F16>)
-                        : reinterpret_cast<void *>(k_kv_rows<HD, TI, QT_BF16>);
+    using Cfg = FewCfg<HD, TI, TC>;
+    using I = typename KvType<TI>::E;
+    using E = typename KvType<TC>::E;
+    constexpr int W = Cfg::W, T = W * 32, NST = Cfg::NST, NQ = Cfg::NQ, NP = Cfg::NP, ES = Cfg::ES;
+    constexpr bool X32 = TC == QT_F32;
+    constexpr int KS = X32 ? HD / 8 : HD / 16;   // steps of the product over the head's dimensions
+    constexpr int CB = HD * ES / 128;            // 128-byte columns of a row
+    constexpr uint32_t kCol = kSlice * 128, kTile = CB * kCol;
+    extern __shared__ __align__(1024) uint8_t sm[];
+    float *merge = reinterpret_cast<float *>(sm + W * NST * Cfg::SB);   // [W][8][HD]
+    uint64_t *full = reinterpret_cast<uint64_t *>(merge + Cfg::MERGE / 4);
+    FewShared &sh = *reinterpret_cast<FewShared *>(full + W * NST);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+
+    if (smem_u32(sm) & 1023u) {   // the swizzle of the copies goes by address bits
+        if (tid == 0) atomicExch(a.err, ERR_RUNTIME);
+        return;
+    }
+    if (tid == 0) {
+        for (int i = 0; i < W * NST; ++i) mbar_init(smem_u32(full + i), 1);
+        fence_mbar_init();
+        sh.fail = 0;
+        sh.seq = a.b.n_seqs;
+    }
+    // ---- this CTA's share of all steps: a scan over the sequences ----
+    const int per = (a.b.n_seqs + T - 1) / T, sq0 = tid * per, sq1 = min(a.b.n_seqs, sq0 + per);
+    unsigned long long mine = 0;
+    bool bad_seq = false;
+    for (int s = sq0; s < sq1; ++s) mine += kv_seq_steps<W>(a, s, bad_seq);
+    if (__syncthreads_or(bad_seq) && blockIdx.x == 0) kv_zero_bad<HD, I>(a);
+    unsigned long long incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const unsigned long long x = __shfl_up_sync(0xFFFFFFFFu, incl, o);
+        if (lane >= o) incl += x;
+    }
+    if (lane == 31) sh.scan[warp] = incl;
+    __syncthreads();
+    unsigned long long before = incl - mine, total = 0;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+        before += w < warp ? sh.scan[w] : 0;
+        total += sh.scan[w];
+    }
+    const unsigned G = total < gridDim.x ? static_cast<unsigned>(total) : gridDim.x, cta = blockIdx.x;
+    if (cta >= G) return;
+    const unsigned long long u0 = total * cta / G, u1 = total * (cta + 1) / G;
+    if (before <= u0 && u0 < before + mine) {
+        unsigned long long at = before;
+        for (int s = sq0; s < sq1; ++s) {
+            const unsigned long long n = kv_seq_steps<W>(a, s, bad_seq);
+            if (u0 < at + n) {
+                sh.seq = s;
+                sh.at = u0 - at;
+                break;
+            }
+            at += n;
+        }
+    }
+    __syncthreads();
+
+    KvCur cu{};
+    cu.s = sh.seq;
+    kv_cur_seq<W>(a, cu);
+    {
+        const unsigned long long r = sh.at, item = r / cu.steps;
+        cu.step = static_cast<int>(r % cu.steps);
+        cu.rt = static_cast<int>(item % cu.tiles);
+        cu.h = static_cast<int>(item / cu.tiles);
+    }
+    auto advance_item = [&](KvCur &c) {
+        c.step = 0;
+        if (++c.rt < c.tiles) return;
+        c.rt = 0;
+        if (++c.h < a.c.n_kv_heads) return;
+        c.h = 0;
+        ++c.s;
+        kv_cur_seq<W>(a, c);
+    };
+
+    // ---- the warp's ring ----
+    const uint32_t ring = smem_u32(sm) + warp * NST * Cfg::SB;
+    const uint32_t bars = smem_u32(full) + warp * NST * 8;
+    KvCur ic = cu;                              // the next step to be requested
+    unsigned long long iu = u0;
+    uint32_t issued = 0, taken = 0, hidden = 0; // slices requested / consumed; hidden: stages whose page is outside the pool
+    int pg = -1, pg_s = -1, pg_base = 0;   // lane l: the page of the warp's slice in step pg_base + l
+    bool ok = true;
+    auto issue_one = [&]() {   // requests the warp's slice of step iu, if it has one
+        const int sl = ic.step * W + warp;
+        if (sl < ic.sl.n) {
+            if (ic.s != pg_s || ic.step >= pg_base + 32 || ic.step < pg_base) {
+                pg_s = ic.s, pg_base = ic.step;
+                const int my = (ic.step + lane) * W + warp;
+                pg = -1;
+                if (my < ic.sl.n) {
+                    const int j = (my < ic.sl.ns ? my : my - ic.sl.ns + ic.sl.lo) * kSlice;
+                    pg = __ldg(a.b.pages + static_cast<long long>(ic.s) * a.b.pages_stride +
+                               fdiv(static_cast<uint32_t>(j), a.c.page_div));
+                }
+            }
+            const int page = __shfl_sync(0xFFFFFFFFu, pg, ic.step - pg_base);
+            const int j = (sl < ic.sl.ns ? sl : sl - ic.sl.ns + ic.sl.lo) * kSlice;
+            const int pos = j - static_cast<int>(fdiv(static_cast<uint32_t>(j), a.c.page_div)) * a.c.page_size;
+            const uint32_t st = issued % NST, bar = bars + st * 8, dst = ring + st * Cfg::SB;
+            const bool bad = page < 0 || page >= a.c.n_pages;
+            hidden = bad ? hidden | (1u << st) : hidden & ~(1u << st);
+            if (lane == 0) {
+                const int y = a.ax_pos == 0 ? pos : a.ax_head == 0 ? ic.h : page;
+                const int z = a.ax_pos == 1 ? pos : a.ax_head == 1 ? ic.h : page;
+                const int w = a.ax_pos == 2 ? pos : a.ax_head == 2 ? ic.h : page;
+                if (bad) {
+                    atomicExch(a.err, ERR_RUNTIME);
+                    mbar_arrive(bar);
+                } else {
+                    mbar_expect_tx(bar, Cfg::SB);
+#pragma unroll
+                    for (int cb = 0; cb < CB; ++cb) {
+                        tma_load_4d(dst + cb * kCol, &kmap, cb * (128 / ES), y, z, w, bar);
+                        tma_load_4d(dst + kTile + cb * kCol, &vmap, cb * (128 / ES), y, z, w, bar);
+                    }
+                }
+            }
+            ++issued;
+        }
+        ++iu;
+        if (++ic.step == ic.steps && iu < u1) advance_item(ic);
+    };
+    auto refill = [&]() {
+        while (ok && iu < u1 && issued - taken < NST) issue_one();
+    };
+    refill();
+
+    const uint32_t krow = (lane & 7) + ((lane >> 3) & 1) * 8, kchunk = lane >> 4;   // ldmatrix rows of K
+    const uint32_t vrow = (lane & 7) + (lane >> 4) * 8, vchunk = (lane >> 3) & 1;   // and of V, transposed
+    for (unsigned long long u = u0; u < u1;) {
+        // ---- one item, or this CTA's part of it ----
+        const bool from_start = cu.step == 0;
+        const int step0 = cu.step;
+        const unsigned long long left = u1 - u;
+        const int nstep = left < static_cast<unsigned>(cu.steps - cu.step) ? static_cast<int>(left) : cu.steps - cu.step;
+        const bool to_end = cu.step + nstep == cu.steps;
+        const int R = cu.q.n * a.group, p0 = cu.q.len - cu.q.n, r0 = cu.rt * 8;
+        // row g of Q as the B operand; rows past the last are zero
+        uint32_t qf[NQ][KS][2];
+        float rscale = a.scale2;
+        {
+            const int r = r0 + g, tok = r / a.group;
+            const bool on = r < R;
+            const I *qp = static_cast<const I *>(a.q.p) + (cu.q.row0 + (on ? tok : 0)) * a.q.row +
+                          (cu.h * a.group + (on ? r - tok * a.group : 0)) * a.q.head;
+            if constexpr (X32) {
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const float x = on ? kv_f(qp[ks * 8 + t + 4 * e]) : 0.f;
+                        split_tf32(__float_as_uint(x), qf[0][ks][e], qf[1][ks][e]);
+                    }
+            } else if constexpr (NQ == 1) {
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                        qf[0][ks][e] = on ? *reinterpret_cast<const uint32_t *>(qp + ks * 16 + 2 * t + 8 * e) : 0u;
+            } else {
+                float x[KS][4], big = 0.f;
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        x[ks][e] = on ? kv_f(qp[ks * 16 + 2 * t + 8 * (e >> 1) + (e & 1)]) : 0.f;
+                        big = fmaxf(big, fabsf(x[ks][e]));
+                    }
+                if constexpr (TC == QT_F16) {   // the row times 2^k, its largest element near 2^13
+                    big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 1));
+                    big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 2));
+                    int k = 0;
+                    if (big > 0.f && big < INFINITY) k = 13 - ilogbf(big);
+                    k = max(-100, min(100, k));
+                    const float up = ldexpf(1.f, k);
+                    rscale = ldexpf(a.scale2, -k);
+#pragma unroll
+                    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) x[ks][e] *= up;
+                }
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+#pragma unroll
+                        for (int n = 0; n < NQ; ++n) qf[n][ks][e] = pack16<TC>(x[ks][2 * e], x[ks][2 * e + 1]);
+            }
+        }
+        // columns 2 t and 2 t + 1 of S^T and O^T: their positions (-1: no row) and scales
+        int pos[2];
+        float rs[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int r = r0 + 2 * t + e;
+            pos[e] = r < R ? p0 + r / a.group : -1;
+            rs[e] = __shfl_sync(0xFFFFFFFFu, rscale, (2 * t + e) * 4);
+        }
+        const int pmin = p0 + r0 / a.group, pmax = p0 + (min(r0 + 8, R) - 1) / a.group;
+        float O[HD / 16][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < HD / 16; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) O[i][e] = 0.f;
+
+        for (int k = 0; k < nstep; ++k) {
+            const int sl = (step0 + k) * W + warp;
+            if (sl < cu.sl.n && ok) {
+                const uint32_t st = taken % NST, kb = ring + st * Cfg::SB, vb = kb + kTile;
+                const int j0 = (sl < cu.sl.ns ? sl : sl - cu.sl.ns + cu.sl.lo) * kSlice;
+                ok = mbar_wait_bounded(bars + st * 8, (taken / NST) & 1u, a.err, a.wait_limit);
+                ok = __all_sync(0xFFFFFFFFu, ok);
+                if (!ok) {
+                    sh.fail = 1;
+                    break;
+                }
+                const bool bad = (hidden >> st) & 1u;
+                if (j0 + kSlice > cu.q.len && !bad) {
+                    // positions that no one wrote: whatever V holds there, 0 * it has to be 0
+                    const int r1 = cu.q.len - j0;
+                    for (int i = lane; i < (kSlice - r1) * (HD * ES / 16); i += 32) {
+                        const int r = r1 + i / (HD * ES / 16), c = i % (HD * ES / 16);
+                        const uint32_t at = vb + (c >> 3) * kCol + r * 128 + ((c & 7) << 4);
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory");
+                    }
+                    fence_proxy_async_smem();   // before the stage's next copy
+                    __syncwarp();
+                }
+                // ---- S^T = K Q^T ----
+                float c[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    const uint32_t ch = 2 * ks + kchunk;
+                    uint32_t x[4];
+                    ldsm4(kb + (ch >> 3) * kCol + krow * 128 + (((ch & 7) ^ (krow & 7)) << 4), x);
+                    if constexpr (X32) {
+                        uint32_t hi[4], lo[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) split_tf32(x[e], hi[e], lo[e]);
+                        mma_tf32(c[ks & 1], lo, qf[0][ks][0], qf[0][ks][1]);
+                        mma_tf32(c[ks & 1], hi, qf[1][ks][0], qf[1][ks][1]);
+                        mma_tf32(c[ks & 1], hi, qf[0][ks][0], qf[0][ks][1]);
+                    } else {
+#pragma unroll
+                        for (int n = NQ - 1; n >= 0; --n) mma16<TC>(c[ks & 1], x, qf[n][ks][0], qf[n][ks][1]);
+                    }
+                }
+                float x[4];   // (position g, row 2 t), (g, 2 t + 1), (g + 8, 2 t), (g + 8, 2 t + 1)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = (c[0][e] + c[1][e]) * rs[e & 1];
+                if (bad || j0 + kSlice - 1 > pmin ||
+                    (a.window > 0 && j0 <= pmax - a.window && j0 + kSlice > a.sinks)) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int j = j0 + g + 8 * (e >> 1), p = pos[e & 1];
+                        const bool see = !bad && j <= p && (a.window == 0 || p - j < a.window || j < a.sinks);
+                        x[e] = see ? x[e] : -INFINITY;
+                    }
+                }
+                // ---- the running maximum: moved only when a score passes it by 2^8 ----
+                if (__any_sync(0xFFFFFFFFu, fmaxf(x[0], x[2]) > m[0] + 8.f || fmaxf(x[1], x[3]) > m[1] + 8.f)) {
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float mx = fmaxf(x[e], x[e + 2]);
+#pragma unroll
+                        for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, o));
+                        mx = fmaxf(mx, m[e]);
+                        const float corr = m[e] == -INFINITY ? 0.f : ex2(m[e] - mx);
+                        m[e] = mx;
+                        l[e] *= corr;
+#pragma unroll
+                        for (int i = 0; i < HD / 16; ++i) O[i][e] *= corr, O[i][e + 2] *= corr;
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = ex2(x[e] - (m[e & 1] == -INFINITY ? 0.f : m[e & 1]));
+                l[0] += x[0] + x[2];
+                l[1] += x[1] + x[3];
+                // ---- O^T += V^T P^T ----
+                if constexpr (X32) {
+                    uint32_t ph[2][2], pl[2][2];   // [8 positions][2 t and 2 t + 1 of them, row g]
+#pragma unroll
+                    for (int kb8 = 0; kb8 < 2; ++kb8)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const int from = (2 * t + e) * 4 + (g >> 1);
+                            const float y0 = __shfl_sync(0xFFFFFFFFu, x[2 * kb8], from);
+                            const float y1 = __shfl_sync(0xFFFFFFFFu, x[2 * kb8 + 1], from);
+                            split_tf32(__float_as_uint((g & 1) ? y1 : y0), ph[kb8][e], pl[kb8][e]);
+                        }
+#pragma unroll
+                    for (int kb8 = 0; kb8 < 2; ++kb8)
+#pragma unroll
+                        for (int jb = 0; jb < HD / 64; ++jb) {
+                            uint4 v[2][2];   // [column 2 jb, 2 jb + 1][position 2 t, 2 t + 1]: 4 dimensions each
+#pragma unroll
+                            for (int cc = 0; cc < 2; ++cc)
+#pragma unroll
+                                for (int e = 0; e < 2; ++e) {
+                                    const uint32_t r = kb8 * 8 + 2 * t + e;
+                                    v[cc][e] = lds_u128(shared_after(vb + (2 * jb + cc) * kCol + r * 128 + ((g ^ (r & 7)) << 4)));
+                                }
+#pragma unroll
+                            for (int d = 0; d < 4; ++d) {
+                                uint32_t hi[4], lo[4];
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    const uint4 &w = v[e & 1][e >> 1];
+                                    split_tf32(d == 0 ? w.x : d == 1 ? w.y : d == 2 ? w.z : w.w, hi[e], lo[e]);
+                                }
+                                float(&o)[4] = O[jb * 4 + d];
+                                mma_tf32(o, lo, ph[kb8][0], ph[kb8][1]);
+                                mma_tf32(o, hi, pl[kb8][0], pl[kb8][1]);
+                                mma_tf32(o, hi, ph[kb8][0], ph[kb8][1]);
+                            }
+                        }
+                } else {
+                    uint32_t pb[NP][2];
+#pragma unroll
+                    for (int n = 0; n < NP; ++n)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) pb[n][e] = mat_t(pack16<TC>(x[2 * e], x[2 * e + 1]));
+#pragma unroll
+                    for (int i = 0; i < HD / 16; ++i) {
+                        const uint32_t ch = 2 * i + vchunk;
+                        uint32_t v[4];
+                        ldsm4t(vb + (ch >> 3) * kCol + vrow * 128 + (((ch & 7) ^ (vrow & 7)) << 4), v);
+#pragma unroll
+                        for (int n = NP - 1; n >= 0; --n) mma16<TC>(O[i], v, pb[n][0], pb[n][1]);
+                    }
+                }
+                __syncwarp();   // every lane has read the stage
+                ++taken;
+                refill();
+            }
+        }
+        // ---- the warps' parts of the item, added in warp order ----
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) l[e] += __shfl_xor_sync(0xFFFFFFFFu, l[e], o);
+            if (g == 0) sh.m[warp][2 * t + e] = m[e], sh.l[warp][2 * t + e] = l[e];
+#pragma unroll
+            for (int i = 0; i < HD / 16; ++i)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const int d = X32 ? (i >> 2) * 64 + k * 32 + 4 * g + (i & 3) : i * 16 + k * 8 + g;
+                    merge[(warp * 8 + 2 * t + e) * HD + d] = O[i][e + 2 * k];
+                }
+        }
+        if (tid < 8) sh.bad[tid] = 0;
+        __syncthreads();
+        const int rows = min(8, R - r0);
+        constexpr int PER = 8 * HD / T;                  // consecutive dimensions of one row a thread
+        constexpr int RT = HD / PER;                     // threads a row
+        const int mr = tid / RT, md = (tid % RT) * PER;  // the thread's row and first dimension
+        float M = -INFINITY, L = 0.f, acc[PER];
+#pragma unroll
+        for (int d = 0; d < PER; ++d) acc[d] = 0.f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) M = fmaxf(M, sh.m[w][mr]);
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            const float f = sh.m[w][mr] == -INFINITY ? 0.f : ex2(sh.m[w][mr] - M);
+            // a warp that saw nothing of the row has l = 0, unless what it saw was NaN
+            L += sh.m[w][mr] == -INFINITY ? sh.l[w][mr] : f * sh.l[w][mr];
+#pragma unroll
+            for (int d = 0; d < PER; ++d) acc[d] = fmaf(f, merge[(w * 8 + mr) * HD + md + d], acc[d]);
+        }
+        bool odd = !isfinite(L) || M == INFINITY;
+#pragma unroll
+        for (int d = 0; d < PER; ++d) odd = odd || !isfinite(acc[d]);
+        if (__syncthreads_or(odd && mr < rows && !sh.fail)) {
+            // a row that is not finite: V of a position that this row does not see may have
+            // been (0 * NaN).  Such rows once more, over their own positions only.
+            if (odd) sh.bad[mr] = 1;
+            __syncthreads();
+            const int ja = step0 * W, jb = min(cu.sl.n, (step0 + nstep) * W);   // the part's slices
+            for (int r = warp; r < rows; r += W) {
+                if (!sh.bad[r]) continue;
+                constexpr int D = HD / 32;
+                const int tok = (r0 + r) / a.group, hh = (r0 + r) - tok * a.group;
+                const I *qp = static_cast<const I *>(a.q.p) + (cu.q.row0 + tok) * a.q.row +
+                              (cu.h * a.group + hh) * a.q.head + lane * D;
+                float q[D], am[2], al[2], ac[2][D];
+#pragma unroll
+                for (int d = 0; d < D; ++d) q[d] = kv_f(qp[d]) * a.scale2;
+                // its slices before and after the gap between the first tokens and the window
+                const int b0 = min(ja, cu.sl.ns), b1 = min(jb, cu.sl.ns);
+                const int c0 = max(ja, cu.sl.ns) - cu.sl.ns + cu.sl.lo, c1 = max(jb, cu.sl.ns) - cu.sl.ns + cu.sl.lo;
+                kv_row_attend<HD, E>(a.b, a.c, cu.s, cu.h, p0 + tok, b0 * kSlice, b1 * kSlice, a.window, a.sinks, q,
+                                     am[0], al[0], ac[0], a.err);
+                kv_row_attend<HD, E>(a.b, a.c, cu.s, cu.h, p0 + tok, c0 * kSlice, min(c1 * kSlice, cu.q.len), a.window,
+                                     a.sinks, q, am[1], al[1], ac[1], a.err);
+                const float mm = fmaxf(am[0], am[1]);
+                const float f0 = am[0] == -INFINITY ? 0.f : ex2(am[0] - mm), f1 = am[1] == -INFINITY ? 0.f : ex2(am[1] - mm);
+#pragma unroll
+                for (int d = 0; d < D; ++d) merge[r * HD + lane * D + d] = ac[0][d] * f0 + ac[1][d] * f1;
+                if (lane == 0) {
+                    sh.m[0][r] = mm;
+                    sh.l[0][r] = (am[0] == -INFINITY ? al[0] : al[0] * f0) + (am[1] == -INFINITY ? al[1] : al[1] * f1);
+                }
+            }
+            __syncthreads();
+            if (mr < rows && sh.bad[mr]) {
+                M = sh.m[0][mr];
+                L = sh.l[0][mr];
+#pragma unroll
+                for (int d = 0; d < PER; ++d) acc[d] = merge[mr * HD + md + d];
+            }
+        }
+        auto write_out = [&]() {
+            if (mr >= rows) return;
+            const int tok = (r0 + mr) / a.group, hh = (r0 + mr) - tok * a.group;
+            I *op = static_cast<I *>(const_cast<void *>(a.o.p)) + (cu.q.row0 + tok) * a.o.row +
+                    (cu.h * a.group + hh) * a.o.head + md;
+            const float inv = 1.0f / L;
+#pragma unroll
+            for (int d = 0; d < PER; ++d) kv_store1(op + d, L == 0.f ? 0.f : acc[d] * inv);
+        };
+        if (from_start && to_end) {
+            write_out();
+        } else {
+            // ---- the CTAs' parts: the last to arrive adds them, in CTA order ----
+            constexpr int P = few_part(HD);
+            const unsigned long long i0 = u - step0, i1 = i0 + cu.steps;   // the item's steps
+            const unsigned c0 = static_cast<unsigned>(((i0 + 1) * G - 1) / total);
+            const unsigned c1 = static_cast<unsigned>((i1 * G - 1) / total);
+            float *mp = a.part + static_cast<size_t>(2 * cta + (from_start ? 1 : 0)) * P;
+            if (mr < rows) {
+#pragma unroll
+                for (int d = 0; d < PER; ++d) mp[mr * HD + md + d] = acc[d];
+                if (md == 0) mp[8 * HD + mr] = M, mp[8 * HD + 8 + mr] = L;
+            }
+            __threadfence();
+            __syncthreads();
+            if (tid == 0) sh.last = atomicInc(a.arrived + c0, c1 - c0) == c1 - c0;   // wraps back to zero
+            __syncthreads();
+            if (sh.last) {
+                __threadfence();
+                if (mr < rows) {
+                    M = -INFINITY;
+                    for (unsigned c = c0; c <= c1; ++c)
+                        M = fmaxf(M, __ldcg(a.part + static_cast<size_t>(2 * c + (c == c0 ? 1 : 0)) * P + 8 * HD + mr));
+                    L = 0.f;
+#pragma unroll
+                    for (int d = 0; d < PER; ++d) acc[d] = 0.f;
+                    for (unsigned c = c0; c <= c1; ++c) {
+                        const float *pp = a.part + static_cast<size_t>(2 * c + (c == c0 ? 1 : 0)) * P;
+                        const float pm = __ldcg(pp + 8 * HD + mr), pl = __ldcg(pp + 8 * HD + 8 + mr);
+                        const float f = pm == -INFINITY ? 0.f : ex2(pm - M);
+                        L += pm == -INFINITY ? pl : f * pl;
+#pragma unroll
+                        for (int d = 0; d < PER; ++d) acc[d] = fmaf(f, __ldcg(pp + mr * HD + md + d), acc[d]);
+                    }
+                }
+                write_out();
+            }
+        }
+        u += nstep;
+        cu.step += nstep;
+        if (u < u1) advance_item(cu);
+        __syncthreads();   // merge and sh are free again
+    }
+    // after a wait that ran out: the copies still in flight, as far as they come
+    while (!ok && taken < issued) {
+        mbar_wait_bounded(bars + (taken % NST) * 8, (taken / NST) & 1u, a.err, a.wait_limit);
+        ++taken;
+    }
 }
 
-size_t kv_attend_ws() { return 16; }
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+using EncodeTiled = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                                 const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
-int kv_attend_launch(const KvView &c, const KvBatch &b, int hd, int ti, int tc, int nh, const KvRows &q,
-                     const KvRows &o, float scale, int window, int sinks, int max_new, int max_len, void *ws, int *err,
-                     int sms, cudaStream_t st)
+static EncodeTiled encode_tiled()
 {
-    const NvtxRange nvtx("tb.kv_attend");
-    (void)max_new, (void)max_len, (void)ws, (void)sms;
-    if (b.n_tokens == 0) return 1;
-    AttnArgs a{c, b, q, o, nh, window, sinks, scale * 1.4426950408889634f, err};
-    void *fn = hd == 128 ? (ti == QT_F32 ? rows_kernel<128, QT_F32>(tc) : ti == QT_F16 ? rows_kernel<128, QT_F16>(tc)
-                                                                                : rows_kernel<128, QT_BF16>(tc))
-                         : (ti == QT_F32 ? rows_kernel<64, QT_F32>(tc) : ti == QT_F16 ? rows_kernel<64, QT_F16>(tc)
-                                                                               : rows_kernel<64, QT_BF16>(tc));
-    void *args[] = {&a};
-    if (cudaLaunchKernel(fn, dim3(b.n_tokens, (nh + 7) / 8), dim3(256), args, 0, st) != cudaSuccess) {
+    static const EncodeTiled fn = [] {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult q{};
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess) {
+            cudaGetLastError();
+            return static_cast<EncodeTiled>(nullptr);
+        }
+        return reinterpret_cast<EncodeTiled>(p);
+    }();
+    return fn;
+}
+
+// The layer's K and V as 4-D tensors: dimension, then position in the page, head
+// and page in order of their strides (ax: which axis each became).  Boxes of
+// 128 bytes by box_rows positions, 128-byte swizzle; pages outside the pool read
+// as zeros.
+static bool kv_maps(const KvView &c, int hd, int tc, int box_rows, CUtensorMap *k, CUtensorMap *v, int (&ax)[3])
+{
+    EncodeTiled enc = encode_tiled();
+    if (!enc) {
+        fprintf(stderr, "[tb_cuda] kv_attend: cuTensorMapEncodeTiled not available\n");
+        return false;
+    }
+    const cuuint64_t es = tc == QT_F32 ? 4 : 2;
+    cuuint64_t size[3] = {static_cast<cuuint64_t>(c.page_size), static_cast<cuuint64_t>(c.n_kv_heads),
+                          static_cast<cuuint64_t>(c.n_pages)};
+    cuuint64_t stride[3] = {static_cast<cuuint64_t>(c.pos_stride) * es, static_cast<cuuint64_t>(c.head_stride) * es,
+                            static_cast<cuuint64_t>(c.page_stride) * es};
+    int order[3] = {0, 1, 2};
+    for (int i = 0; i < 3; ++i)
+        for (int j = i + 1; j < 3; ++j)
+            if (stride[order[j]] < stride[order[i]]) {
+                const int x = order[i];
+                order[i] = order[j];
+                order[j] = x;
+            }
+    cuuint64_t dims[4] = {static_cast<cuuint64_t>(hd)}, strides[3];
+    cuuint32_t box[4] = {static_cast<cuuint32_t>(128 / es), 1, 1, 1};
+    const cuuint32_t estr[4] = {1, 1, 1, 1};
+    for (int i = 0; i < 3; ++i) {
+        ax[order[i]] = i;
+        dims[i + 1] = size[order[i]];
+        strides[i] = stride[order[i]];
+        if (order[i] == 0) box[i + 1] = static_cast<cuuint32_t>(box_rows);
+    }
+    const CUtensorMapDataType type = tc == QT_F32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                     : tc == QT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                    : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    for (int i = 0; i < 2; ++i) {
+        const CUresult r = enc(i ? v : k, type, 4, const_cast<void *>(i ? c.v : c.k), dims, strides, box, estr,
+                               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+        if (r != CUDA_SUCCESS) {
+            fprintf(stderr, "[tb_cuda] kv_attend: tensor map encode failed (%d)\n", static_cast<int>(r));
+            return false;
+        }
+    }
+    return true;
+}
+
+// Workspace: the arrival counters (the part that stays zero between calls), then
+// the partial results, two a CTA.
+static constexpr int kMaxCtas = 512;
+static constexpr size_t kCounterBytes = kMaxCtas * sizeof(unsigned);
+size_t kv_attend_ws() { return kCounterBytes + sizeof(float) * 2 * kMaxCtas * few_part(128); }
+
+template <int HD, int TI, int TC>
+static int few_launch(AttnArgs &a, int sms, cudaStream_t st)
+{
+    using Cfg = FewCfg<HD, TI, TC>;
+    CUtensorMap km, vm;
+    int ax[3];
+    if (!kv_maps(a.c, HD, TC, kSlice, &km, &vm, ax)) return 0;
+    a.ax_pos = ax[0], a.ax_head = ax[1], a.ax_page = ax[2];
+    auto fn = k_kv_few<HD, TI, TC>;
+    if (!smem_attr_once(reinterpret_cast<const void *>(fn), Cfg::SMEM)) {
         cudaGetLastError();
         return 0;
     }
-    return 1;
+    const int grid = sms * Cfg::CTAS < kMaxCtas ? sms * Cfg::CTAS : kMaxCtas;
+    fn<<<grid, Cfg::W * 32, Cfg::SMEM, st>>>(km, vm, a);
+    return cudaGetLastError() == cudaSuccess ? 1 : 0;
+}
+
+template <int HD, int TI>
+static int few_types(AttnArgs &a, int tc, int sms, cudaStream_t st)
+{
+    return tc == QT_F32   ? few_launch<HD, TI, QT_F32>(a, sms, st)
+           : tc == QT_F16 ? few_launch<HD, TI, QT_F16>(a, sms, st)
+                          : few_launch<HD, TI, QT_BF16>(a, sms, st);
+}
+
+template <int HD>
+static int few(AttnArgs &a, int ti, int tc, int sms, cudaStream_t st)
+{
+    return ti == QT_F32   ? few_types<HD, QT_F32>(a, tc, sms, st)
+           : ti == QT_F16 ? few_types<HD, QT_F16>(a, tc, sms, st)
+                          : few_types<HD, QT_BF16>(a, tc, sms, st);
+}
+
+int kv_attend_launch(const KvView &c, const KvBatch &b, int hd, int ti, int tc, int nh, const KvRows &q,
+                     const KvRows &o, float scale, int window, int sinks, int max_new, int max_len, void *ws, int *err,
+                     int sms, uint32_t wait_limit, cudaStream_t st)
+{
+    const NvtxRange nvtx("tb.kv_attend");
+    (void)max_new, (void)max_len;
+    AttnArgs a{c, b, q, o, nh, nh / c.n_kv_heads, window, sinks, scale * 1.4426950408889634f, err, wait_limit};
+    a.arrived = static_cast<unsigned *>(ws);
+    a.part = reinterpret_cast<float *>(static_cast<char *>(ws) + kCounterBytes);
+    return hd == 128 ? few<128>(a, ti, tc, sms, st) : few<64>(a, ti, tc, sms, st);
 }
 
 }  // namespace tb

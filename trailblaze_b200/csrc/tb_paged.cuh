@@ -42,7 +42,7 @@ int kv_copy_launch(void *k, void *v, int esize, int n_layers, int n_pages, int p
 size_t kv_attend_ws();
 int kv_attend_launch(const KvView &c, const KvBatch &b, int hd, int ti, int tc, int nh, const KvRows &q,
                      const KvRows &o, float scale, int window, int sinks, int max_new, int max_len, void *ws, int *err,
-                     int sms, cudaStream_t st);
+                     int sms, uint32_t wait_limit, cudaStream_t st);
 
 // Element types as template arguments.
 template <int T> struct KvType;
