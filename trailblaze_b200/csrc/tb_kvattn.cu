@@ -27,27 +27,9 @@
 // so that its largest element is near 2^13); an fp32 cache is split into two
 // tf32 parts, of which the low-low product is dropped (2^-22).  Scores, softmax and
 // sums are fp32.
-#include <cuda.h>
-
-#include <cmath>
-#include <cstdio>
-
-#include "tb_paged.cuh"
+#include "tb_kvattn.cuh"
 
 namespace tb {
-
-struct AttnArgs {
-    KvView c;
-    KvBatch b;
-    KvRows q, o;
-    int nh, group, window, sinks;
-    float scale2;   // scale * log2(e)
-    int *err;
-    uint32_t wait_limit;
-    int ax_pos, ax_head, ax_page;   // the tensor maps' axes 1..3: which of them is which
-    float *part;                    // [2 * gridDim.x] partial results
-    unsigned *arrived;              // [gridDim.x] arrival counters, zero between calls
-};
 
 // ---- PTX ----
 __device__ __forceinline__ void ldsm4(uint32_t a, uint32_t (&r)[4])
@@ -91,20 +73,6 @@ __device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], 
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ float ex2(float x)   // 2^x, 2 ulp; 0 for -inf
-{
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map, int x, int y, int z, int w, uint32_t bar)
-{
-    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, "
-                 "%5}], [%6];" ::"r"(dst),
-                 "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
-                 : "memory");
-}
-
 // x = hi + lo, hi rounded to tf32 (10 bits of mantissa); the tensor core reads
 // lo's upper 19 bits: what is lost lies 2^-21 below x and has no preferred sign.
 __device__ __forceinline__ void split_tf32(uint32_t x, uint32_t &hi, uint32_t &lo)
@@ -176,6 +144,12 @@ struct FewCfg {
 // floats of one partial result: 8 rows of O, then m and l of each
 __host__ __device__ constexpr int few_part(int hd) { return 8 * hd + 16; }
 
+// True for a sequence of this launch.
+__device__ __forceinline__ bool few_seq(const AttnArgs &a, const KvSeq &q)
+{
+    return q.n > 0 && static_cast<long long>(q.n) * a.group <= a.many_rows;
+}
+
 // A place in the sequence of all items' steps.
 struct KvCur {
     int s, h, rt, step;     // sequence, kv head, row tile, step
@@ -188,7 +162,7 @@ template <int W>
 __device__ __forceinline__ void kv_cur_seq(const AttnArgs &a, KvCur &c)
 {
     // sequences that cannot be are skipped here; the scan has reported them
-    while (c.s < a.b.n_seqs && (!kv_seq(a.b, a.c, c.s, c.q, nullptr) || c.q.n == 0)) ++c.s;
+    while (c.s < a.b.n_seqs && (!kv_seq(a.b, a.c, c.s, c.q, nullptr) || !few_seq(a, c.q))) ++c.s;
     if (c.s >= a.b.n_seqs) return;
     c.sl = kv_slices(c.q, a.window, a.sinks);
     c.tiles = (c.q.n * a.group + 7) >> 3;
@@ -203,29 +177,10 @@ __device__ __forceinline__ unsigned long long kv_seq_steps(const AttnArgs &a, in
         bad = true;
         return 0;
     }
-    if (q.n == 0) return 0;
+    if (!few_seq(a, q)) return 0;
     const KvSlices sl = kv_slices(q, a.window, a.sinks);
     const unsigned long long tiles = (static_cast<unsigned long long>(q.n) * a.group + 7) >> 3;
     return tiles * a.c.n_kv_heads * static_cast<unsigned>((sl.n + W - 1) / W);
-}
-
-// The rows of sequences whose numbers contradict each other: the error word, and
-// zeros as far as the rows exist (one CTA, all its threads).
-template <int HD, class I>
-__device__ void kv_zero_bad(const AttnArgs &a)
-{
-    for (int s = 0; s < a.b.n_seqs; ++s) {
-        KvSeq q;
-        if (kv_seq(a.b, a.c, s, q, a.err)) continue;
-        const int lo = max(0, a.b.start[s]), hi = min(a.b.n_tokens, a.b.start[s + 1]);
-        const long long n = static_cast<long long>(max(0, hi - lo)) * a.nh * HD;
-        for (long long e = threadIdx.x; e < n; e += blockDim.x) {
-            const long long th = e / HD;
-            kv_store1(static_cast<I *>(const_cast<void *>(a.o.p)) + (lo + th / a.nh) * a.o.row + (th % a.nh) * a.o.head +
-                          e % HD,
-                      0.f);
-        }
-    }
 }
 
 template <int HD, int TI, int TC>
@@ -712,78 +667,19 @@ __global__ void __launch_bounds__(FewCfg<HD, TI, TC>::W * 32, FewCfg<HD, TI, TC>
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
-using EncodeTiled = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
-                                 const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
-                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-static EncodeTiled encode_tiled()
-{
-    static const EncodeTiled fn = [] {
-        void *p = nullptr;
-        cudaDriverEntryPointQueryResult q{};
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
-            q != cudaDriverEntryPointSuccess) {
-            cudaGetLastError();
-            return static_cast<EncodeTiled>(nullptr);
-        }
-        return reinterpret_cast<EncodeTiled>(p);
-    }();
-    return fn;
-}
-
-// The layer's K and V as 4-D tensors: dimension, then position in the page, head
-// and page in order of their strides (ax: which axis each became).  Boxes of
-// 128 bytes by box_rows positions, 128-byte swizzle; pages outside the pool read
-// as zeros.
-static bool kv_maps(const KvView &c, int hd, int tc, int box_rows, CUtensorMap *k, CUtensorMap *v, int (&ax)[3])
-{
-    EncodeTiled enc = encode_tiled();
-    if (!enc) {
-        fprintf(stderr, "[tb_cuda] kv_attend: cuTensorMapEncodeTiled not available\n");
-        return false;
-    }
-    const cuuint64_t es = tc == QT_F32 ? 4 : 2;
-    cuuint64_t size[3] = {static_cast<cuuint64_t>(c.page_size), static_cast<cuuint64_t>(c.n_kv_heads),
-                          static_cast<cuuint64_t>(c.n_pages)};
-    cuuint64_t stride[3] = {static_cast<cuuint64_t>(c.pos_stride) * es, static_cast<cuuint64_t>(c.head_stride) * es,
-                            static_cast<cuuint64_t>(c.page_stride) * es};
-    int order[3] = {0, 1, 2};
-    for (int i = 0; i < 3; ++i)
-        for (int j = i + 1; j < 3; ++j)
-            if (stride[order[j]] < stride[order[i]]) {
-                const int x = order[i];
-                order[i] = order[j];
-                order[j] = x;
-            }
-    cuuint64_t dims[4] = {static_cast<cuuint64_t>(hd)}, strides[3];
-    cuuint32_t box[4] = {static_cast<cuuint32_t>(128 / es), 1, 1, 1};
-    const cuuint32_t estr[4] = {1, 1, 1, 1};
-    for (int i = 0; i < 3; ++i) {
-        ax[order[i]] = i;
-        dims[i + 1] = size[order[i]];
-        strides[i] = stride[order[i]];
-        if (order[i] == 0) box[i + 1] = static_cast<cuuint32_t>(box_rows);
-    }
-    const CUtensorMapDataType type = tc == QT_F32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
-                                     : tc == QT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
-                                                    : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-    for (int i = 0; i < 2; ++i) {
-        const CUresult r = enc(i ? v : k, type, 4, const_cast<void *>(i ? c.v : c.k), dims, strides, box, estr,
-                               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-        if (r != CUDA_SUCCESS) {
-            fprintf(stderr, "[tb_cuda] kv_attend: tensor map encode failed (%d)\n", static_cast<int>(r));
-            return false;
-        }
-    }
-    return true;
-}
-
 // Workspace: the arrival counters (the part that stays zero between calls), then
 // the partial results, two a CTA.
 static constexpr int kMaxCtas = 512;
 static constexpr size_t kCounterBytes = kMaxCtas * sizeof(unsigned);
-size_t kv_attend_ws() { return kCounterBytes + sizeof(float) * 2 * kMaxCtas * few_part(128); }
+size_t kv_attend_ws()
+{
+    const size_t few = sizeof(float) * 2 * kMaxCtas * few_part(128), many = 2 * kManyCtas * kv_many_part_bytes();
+    return kCounterBytes + (few > many ? few : many);
+}
+
+// Query rows per kv head up to which a sequence's attention is bound by the
+// cache's bytes in k_kv_few.
+static constexpr int kFewRows = 16;
 
 template <int HD, int TI, int TC>
 static int few_launch(AttnArgs &a, int sms, cudaStream_t st)
@@ -824,10 +720,22 @@ int kv_attend_launch(const KvView &c, const KvBatch &b, int hd, int ti, int tc, 
                      int sms, uint32_t wait_limit, cudaStream_t st)
 {
     const NvtxRange nvtx("tb.kv_attend");
-    (void)max_new, (void)max_len;
+    (void)max_len;
     AttnArgs a{c, b, q, o, nh, nh / c.n_kv_heads, window, sinks, scale * 1.4426950408889634f, err, wait_limit};
     a.arrived = static_cast<unsigned *>(ws);
     a.part = reinterpret_cast<float *>(static_cast<char *>(ws) + kCounterBytes);
+    a.many_rows = 0x7FFFFFFF;
+    // Chunks go to the tensor-core kernel: 16-bit activations over a cache of their
+    // type, whole groups of heads in 128 rows, and a scale that keeps the order of
+    // scores.  Where the batch holds short sequences besides, both kernels run and
+    // each takes its own; which sequences those are is decided on the device.
+    if (ti == tc && tc != QT_F32 && a.group <= 128 && scale > 0.f &&
+        static_cast<long long>(max_new) * a.group > kFewRows) {
+        const bool mixed = b.n_tokens < static_cast<long long>(b.n_seqs) * max_new;
+        const int r = kv_many_launch(a, hd, tc, mixed ? kFewRows : 0, sms, st);
+        if (r == 0 || (r == 1 && !mixed)) return r;
+        if (r == 1) a.many_rows = kFewRows;
+    }
     return hd == 128 ? few<128>(a, ti, tc, sms, st) : few<64>(a, ti, tc, sms, st);
 }
 

@@ -1,0 +1,729 @@
+// tb_kvmany.cu — attention of chunks of new tokens over the paged cache on the
+// 5th-generation tensor cores (include/tb_gguf_dequant.h part 4): k_kv_many, for
+// 16-bit activations over a cache of the same type and enough query rows per kv
+// head to fill tiles of 128.
+//
+// An item is (sequence, kv head, 2 x 128 query rows): with G query heads per kv
+// head a group of 128 rows holds 128 / G whole tokens, row = token * G + head.  A
+// unit is an item's product with a tile of 128 positions.  All items' units, laid
+// end to end, are cut into equal parts, one per CTA (one CTA per SM): causal
+// triangles, windows and ragged lengths balance by themselves, and a short chunk
+// late in a long context still fills the GPU.  An item cut between CTAs is joined
+// by the last of them to arrive, in CTA order.
+//
+// Inside a CTA (384 threads):
+//   warps 0-3, 4-7  softmax of row group 0 / 1, one row a thread;
+//   warp 8          the MMAs, one elected thread: S_g = Q_g K^T (128 x 128, both
+//                   operands in shared memory), O_g += P_g V (P_g read from TMEM);
+//   warp 9          K and V tiles by TMA into a ring, page by page;
+//   warp 10         Q tiles by TMA (the next item's while the last one's softmax
+//                   and epilogue still run).
+// TMEM: S_0, S_1 (128 fp32 columns each, P_g overwrites the first half of S_g as
+// 16-bit pairs), O_0, O_1.  The two groups take turns on the tensor core: while
+// one's softmax runs, the other's products do.  The MMA order PV_g(j), S_g(j + 1)
+// makes the overwriting of P_g safe without a barrier, since MMAs of one thread
+// execute in order; when S_g(j) is complete so is PV_g(j - 1), which is why the
+// softmax threads may rescale O_g between seeing S_g and handing over P_g.
+//
+// The running maximum moves only when a score passes it by 2^8 (exponents stay
+// far inside fp32 and fp16), so rescaling O is rare.  P is rounded to the cache's
+// type for the second product, whose unit takes nothing wider: 2^-9 (bf16) of
+// each term, unbiased, about what the output's own rounding is; sums are fp32 of
+// the unrounded P.
+#include "tb_kvattn.cuh"
+
+namespace tb {
+
+static constexpr int kTileN = 128;      // positions of a tile
+static constexpr int kManyThreads = 384;
+
+struct ManyArgs {
+    AttnArgs a;
+    int tpt;         // tokens of a row group: 128 / G
+    int few_rows;    // sequences of at most this many rows are another launch's
+    int box;         // positions of one K or V box
+    int bf16;
+};
+
+template <int HD>
+struct ManyCfg {
+    static constexpr int SLOT = kTileN * HD * 2;         // one K or V tile
+    static constexpr int QG = 128 * HD * 2;              // one row group's Q
+    static constexpr int NS = HD == 128 ? 5 : 10;        // ring slots
+    static constexpr int SMEM = 1024 + 2 * QG + NS * SLOT + 1024;
+    static constexpr int PART = 256 * HD + 512;          // floats of a partial result: O, m, l
+};
+
+struct ManyShared {
+    uint64_t sfull[2], pready[2], ofull[2], qfull, qempty, done, join, kvfull[10], kvempty[10];
+    unsigned long long scan[12], u0;
+    uint32_t tmem;
+    int seq, head, rt, off, fail, bad, last;
+};
+static_assert(sizeof(ManyShared) <= 1024, "ManyShared");
+
+// ---- the items ----
+struct ManyItem {
+    int s, h, rt;           // sequence, kv head, row tile
+    KvSeq q;
+    int n_rt;               // row tiles a head
+    int t0, t1;             // new tokens [t0, t1) of the sequence
+    int ns, lo, n;          // its position tiles: [0, ns) and [lo, lo + n - ns)
+};
+
+__device__ __forceinline__ int many_tiles(const ManyArgs &a, const KvSeq &q, int rt, ManyItem *it)
+{
+    const int t0 = rt * 2 * a.tpt, t1 = min(q.n, t0 + 2 * a.tpt), p0 = q.len - q.n;
+    const KvSpan sp = kv_span(p0 + t0, a.a.window, a.a.sinks);
+    const int hi = (p0 + t1 - 1) / kTileN + 1;
+    int ns = 0, lo = 0, n = hi;
+    if (a.a.sinks < sp.lo) {
+        ns = (a.a.sinks + kTileN - 1) / kTileN;
+        lo = max(sp.lo / kTileN, ns);
+        n = ns + hi - lo;
+    }
+    if (it) it->t0 = t0, it->t1 = t1, it->ns = ns, it->lo = lo, it->n = n;
+    return n;
+}
+// True for a sequence of this launch.
+__device__ __forceinline__ bool many_seq(const ManyArgs &a, int s, KvSeq &q)
+{
+    return kv_seq(a.a.b, a.a.c, s, q, nullptr) && static_cast<long long>(q.n) * a.a.group > a.few_rows && q.n > 0;
+}
+__device__ __forceinline__ void many_enter(const ManyArgs &a, ManyItem &it)   // at sequence it.s, or a later one
+{
+    while (it.s < a.a.b.n_seqs && !many_seq(a, it.s, it.q)) ++it.s;
+    it.n_rt = (it.q.n + 2 * a.tpt - 1) / (2 * a.tpt);
+}
+__device__ __forceinline__ void many_next(const ManyArgs &a, ManyItem &it)
+{
+    if (++it.rt == it.n_rt) {
+        it.rt = 0;
+        if (++it.h == a.a.c.n_kv_heads) {
+            it.h = 0;
+            ++it.s;
+            many_enter(a, it);
+        }
+    }
+    many_tiles(a, it.q, it.rt, &it);
+}
+__device__ __forceinline__ int many_tile_pos(const ManyItem &it, int j) { return (j < it.ns ? j : j - it.ns + it.lo) * kTileN; }
+
+// ---- TMEM ----
+#define TB_R32(r)                                                                                                       \
+    "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),       \
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),     \
+        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),     \
+        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+#define TB_W32(c, r)                                                                                                    \
+    c(r[0]), c(r[1]), c(r[2]), c(r[3]), c(r[4]), c(r[5]), c(r[6]), c(r[7]), c(r[8]), c(r[9]), c(r[10]), c(r[11]),       \
+        c(r[12]), c(r[13]), c(r[14]), c(r[15]), c(r[16]), c(r[17]), c(r[18]), c(r[19]), c(r[20]), c(r[21]), c(r[22]),   \
+        c(r[23]), c(r[24]), c(r[25]), c(r[26]), c(r[27]), c(r[28]), c(r[29]), c(r[30]), c(r[31])
+#define TB_LIST32                                                                                                       \
+    "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, "   \
+    "%24, %25, %26, %27, %28, %29, %30, %31}"
+__device__ __forceinline__ void tmem_ld32(uint32_t at, uint32_t *r)
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 " TB_LIST32 ", [%32];" : TB_W32("=r", r) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t at, const uint32_t *r)
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], " TB_LIST32 ";" ::TB_R32(r), "r"(at) : "memory");
+}
+// The loads before it are complete; the registers pass through, so that nothing
+// that uses them moves ahead.
+__device__ __forceinline__ void tmem_wait_ld(uint32_t *r)
+{
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : TB_W32("+r", r)::"memory");
+}
+__device__ __forceinline__ void after_wait(uint32_t *r) { asm volatile("" : TB_W32("+r", r)::"memory"); }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// D[tmem] (+)= A[tmem] * B[smem desc], one thread
+__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                            uint32_t accumulate)
+{
+    asm volatile("{\n\t.reg .pred p;\n\t"
+                 "setp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+                 "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+                 : "memory");
+}
+// Shared-memory descriptor of V as the B operand: rows are positions (the
+// product's K), 128-byte columns of 64 dimensions (its N, "MN-major") with the
+// 128-byte swizzle.  Leading byte offset: from one 64-dimension column to the
+// next; stride byte offset: from 8 positions to the next 8.
+__device__ __forceinline__ uint64_t v_desc(uint32_t saddr)
+{
+    uint64_t d = 0;
+    d |= static_cast<uint64_t>((saddr >> 4) & 0x3FFFu);
+    d |= static_cast<uint64_t>((kTileN * 128u) >> 4) << 16;
+    d |= static_cast<uint64_t>(1024u >> 4) << 32;
+    d |= static_cast<uint64_t>(1u) << 46;
+    d |= static_cast<uint64_t>(2u) << 61;
+    return d;
+}
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *map, int x, int y, int z, uint32_t bar)
+{
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
+                 "[%5];" ::"r"(dst),
+                 "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
+                 : "memory");
+}
+
+// One row again, over the visible positions of the part's tiles [j0, j1) only, by
+// the whole warp: acc[d] of dimensions lane * HD / 32 + d, m and l.
+template <int HD, class I>
+__device__ __noinline__ void many_row_again(const ManyArgs &a, const ManyItem &it, int tok, int hh, int j0, int j1,
+                                            float &m, float &l, float (&acc)[HD / 32])
+{
+    constexpr int D = HD / 32;
+    const int lane = threadIdx.x & 31;
+    const I *qp = static_cast<const I *>(a.a.q.p) + (it.q.row0 + tok) * a.a.q.row + (it.h * a.a.group + hh) * a.a.q.head +
+                  lane * D;
+    float q[D], am[2], al[2], ac[2][D];
+#pragma unroll
+    for (int d = 0; d < D; ++d) q[d] = kv_f(qp[d]) * a.a.scale2;
+    const int pos = it.q.len - it.q.n + tok;
+    const int b0 = min(j0, it.ns) * kTileN, b1 = min(j1, it.ns) * kTileN;
+    const int c0 = (max(j0, it.ns) - it.ns + it.lo) * kTileN, c1 = (max(j1, it.ns) - it.ns + it.lo) * kTileN;
+    kv_row_attend<HD, I>(a.a.b, a.a.c, it.s, it.h, pos, b0, min(b1, it.q.len), a.a.window, a.a.sinks, q, am[0], al[0],
+                         ac[0], a.a.err);
+    kv_row_attend<HD, I>(a.a.b, a.a.c, it.s, it.h, pos, c0, min(c1, it.q.len), a.a.window, a.a.sinks, q, am[1], al[1],
+                         ac[1], a.a.err);
+    m = fmaxf(am[0], am[1]);
+    const float f0 = am[0] == -INFINITY ? 0.f : ex2(am[0] - m), f1 = am[1] == -INFINITY ? 0.f : ex2(am[1] - m);
+    l = (am[0] == -INFINITY ? al[0] : al[0] * f0) + (am[1] == -INFINITY ? al[1] : al[1] * f1);
+#pragma unroll
+    for (int d = 0; d < D; ++d) acc[d] = ac[0][d] * f0 + ac[1][d] * f1;
+}
+
+template <int HD, class I>
+__global__ void __launch_bounds__(kManyThreads, 1)
+    k_kv_many(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
+              const __grid_constant__ CUtensorMap vmap, const __grid_constant__ ManyArgs a)
+{
+    using Cfg = ManyCfg<HD>;
+    constexpr int CB = HD / 64;   // 128-byte columns
+    constexpr int NS = Cfg::NS;
+    extern __shared__ __align__(1024) uint8_t smraw[];
+    uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smraw) + 1023) & ~uintptr_t(1023));
+    ManyShared &sh = *reinterpret_cast<ManyShared *>(sm + 2 * Cfg::QG + NS * Cfg::SLOT);
+    const uint32_t qbase = smem_u32(sm), ring = qbase + 2 * Cfg::QG;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const uint32_t lim = a.a.wait_limit;
+    int *err = a.a.err;
+
+    if (tid == 0) {
+        for (int g = 0; g < 2; ++g) {
+            mbar_init(smem_u32(&sh.sfull[g]), 1);
+            mbar_init(smem_u32(&sh.pready[g]), 128);
+            mbar_init(smem_u32(&sh.ofull[g]), 1);
+        }
+        mbar_init(smem_u32(&sh.qfull), 1);
+        mbar_init(smem_u32(&sh.qempty), 1);
+        mbar_init(smem_u32(&sh.done), 1);
+        mbar_init(smem_u32(&sh.join), 256);
+        for (int i = 0; i < NS; ++i) {
+            mbar_init(smem_u32(&sh.kvfull[i]), 1);
+            mbar_init(smem_u32(&sh.kvempty[i]), 1);
+        }
+        fence_mbar_init();
+        sh.fail = 0;
+        sh.bad = 0;
+    }
+    // ---- this CTA's share of all units: a scan over the sequences ----
+    const int per = (a.a.b.n_seqs + kManyThreads - 1) / kManyThreads;
+    const int sq0 = min(a.a.b.n_seqs, tid * per), sq1 = min(a.a.b.n_seqs, sq0 + per);
+    auto head_units = [&](const KvSeq &q) {
+        unsigned long long f = 0;
+        const int n_rt = (q.n + 2 * a.tpt - 1) / (2 * a.tpt);
+        for (int rt = 0; rt < n_rt; ++rt) f += many_tiles(a, q, rt, nullptr);
+        return f;
+    };
+    unsigned long long mine = 0;
+    bool bad_seq = false;
+    for (int s = sq0; s < sq1; ++s) {
+        KvSeq q;
+        bad_seq = bad_seq || !kv_seq(a.a.b, a.a.c, s, q, nullptr);
+        if (many_seq(a, s, q)) mine += head_units(q) * a.a.c.n_kv_heads;
+    }
+    unsigned long long incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const unsigned long long x = __shfl_up_sync(0xFFFFFFFFu, incl, o);
+        if (lane >= o) incl += x;
+    }
+    if (lane == 31) sh.scan[warp] = incl;
+    if (__syncthreads_or(bad_seq) && blockIdx.x == 0) kv_zero_bad<HD, I>(a.a);
+    unsigned long long before = incl - mine, total = 0;
+    for (int w = 0; w < kManyThreads / 32; ++w) {
+        before += w < warp ? sh.scan[w] : 0;
+        total += sh.scan[w];
+    }
+    const unsigned G = total < gridDim.x ? static_cast<unsigned>(total) : gridDim.x, cta = blockIdx.x;
+    if (cta >= G) return;
+    const unsigned long long u0 = total * cta / G, u1 = total * (cta + 1) / G;
+    if (before <= u0 && u0 < before + mine) {
+        unsigned long long at = before;
+        for (int s = sq0; s < sq1; ++s) {
+            KvSeq q;
+            if (!many_seq(a, s, q)) continue;
+            const unsigned long long f = head_units(q), n = f * a.a.c.n_kv_heads;
+            if (u0 < at + n) {
+                unsigned long long r = (u0 - at) % f;
+                int rt = 0;
+                for (;; ++rt) {
+                    const unsigned k = many_tiles(a, q, rt, nullptr);
+                    if (r < k) break;
+                    r -= k;
+                }
+                sh.seq = s;
+                sh.head = static_cast<int>((u0 - at) / f);
+                sh.rt = rt;
+                sh.off = static_cast<int>(r);
+                break;
+            }
+            at += n;
+        }
+    }
+    if (warp == 8) {
+        tmem_alloc(smem_u32(&sh.tmem), 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tm = sh.tmem;
+
+    ManyItem it{};
+    it.s = sh.seq, it.h = sh.head, it.rt = sh.rt;
+    many_enter(a, it);
+    many_tiles(a, it.q, it.rt, &it);
+    int j0 = sh.off;             // the first of the item's tiles that is this CTA's
+    unsigned long long u = u0;
+    // the item's tiles [j0, j1) are this CTA's
+    auto part_end = [&]() {
+        const unsigned long long left = u1 - u;
+        return left < static_cast<unsigned>(it.n - j0) ? j0 + static_cast<int>(left) : it.n;
+    };
+    auto next_item = [&](int j1) {
+        u += j1 - j0;
+        j0 = 0;
+        if (u < u1) many_next(a, it);
+    };
+    auto failed = [&]() { return *reinterpret_cast<volatile int *>(&sh.fail) != 0; };
+    auto wait = [&](uint64_t *bar, uint32_t parity) {   // by a whole warp
+        const bool ok = mbar_wait_bounded(smem_u32(bar), parity & 1u, err, lim);
+        if (__all_sync(0xFFFFFFFFu, ok) && !failed()) return true;
+        *reinterpret_cast<volatile int *>(&sh.fail) = 1;
+        return false;
+    };
+
+    uint32_t kv_issued = 0, q_issued = 0;   // in the warps that issue them
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        if (warp == 9) {
+            // ---- K and V ----
+            bool ok = true;
+            while (ok && u < u1) {
+                const int j1 = part_end();
+                for (int j = j0; ok && j < j1; ++j) {
+                    const int p0 = many_tile_pos(it, j), boxes = kTileN / a.box;
+                    // lane l: box l of the tile, its page (past the end: a page that reads as zeros)
+                    int page = a.a.c.n_pages, pos = 0;
+                    const int p = p0 + lane * a.box;
+                    if (lane < boxes && p < it.q.len) {
+                        const uint32_t pi = fdiv(static_cast<uint32_t>(p), a.a.c.page_div);
+                        page = __ldg(a.a.b.pages + static_cast<long long>(it.s) * a.a.b.pages_stride + pi);
+                        pos = p - static_cast<int>(pi) * a.a.c.page_size;
+                        if (page < 0 || page >= a.a.c.n_pages) {
+                            atomicExch(err, ERR_RUNTIME);
+                            *reinterpret_cast<volatile int *>(&sh.bad) = 1;
+                            page = a.a.c.n_pages;
+                        }
+                    }
+                    const int y = a.a.ax_pos == 0 ? pos : a.a.ax_head == 0 ? it.h : page;
+                    const int z = a.a.ax_pos == 1 ? pos : a.a.ax_head == 1 ? it.h : page;
+                    const int w = a.a.ax_pos == 2 ? pos : a.a.ax_head == 2 ? it.h : page;
+                    for (int kv = 0; kv < 2; ++kv) {
+                        const uint32_t n = kv_issued, slot = n % NS, bar = smem_u32(&sh.kvfull[slot]);
+                        if (n >= NS) ok = wait(&sh.kvempty[slot], (n / NS) - 1u);
+                        if (!ok) break;
+                        if (lane == 0) mbar_expect_tx(bar, Cfg::SLOT);
+                        __syncwarp();
+                        if (lane < boxes) {
+                            const uint32_t dst = ring + slot * Cfg::SLOT + lane * a.box * 128;
+#pragma unroll
+                            for (int cb = 0; cb < CB; ++cb)
+                                tma_load_4d(dst + cb * kTileN * 128, kv ? &vmap : &kmap, cb * 64, y, z, w, bar);
+                        }
+                        __syncwarp();
+                        ++kv_issued;
+                    }
+                }
+                next_item(j1);
+            }
+        } else if (warp == 10) {
+            // ---- Q ----
+            bool ok = true;
+            while (ok && u < u1) {
+                const int j1 = part_end();
+                if (q_issued > 0) ok = wait(&sh.qempty, q_issued - 1u);
+                if (!ok) break;
+                if (elect_one()) {
+                    const uint32_t bar = smem_u32(&sh.qfull);
+                    mbar_expect_tx(bar, 2u * CB * 128u * a.tpt * a.a.group);
+                    for (int g = 0; g < 2; ++g)
+                        for (int cb = 0; cb < CB; ++cb)
+                            tma_load_3d(qbase + g * Cfg::QG + cb * 128 * 128, &qmap, cb * 64, it.h * a.a.group,
+                                        it.q.row0 + it.t0 + g * a.tpt, bar);
+                }
+                __syncwarp();
+                ++q_issued;
+                next_item(j1);
+            }
+        } else if (warp == 8) {
+            // ---- the MMAs ----
+            const uint32_t fmt = a.bf16 ? 1u : 0u;
+            const uint32_t id_s = (1u << 4) | (fmt << 7) | (fmt << 10) | ((kTileN >> 3) << 17) | (8u << 24);
+            const uint32_t id_o = (1u << 4) | (fmt << 7) | (fmt << 10) | (1u << 16) | ((HD >> 3) << 17) | (8u << 24);
+            uint32_t n = 0, q = 0, np = 0;   // ring slots, items and P tiles taken
+            bool ok = true;
+            auto issue_s = [&](int g, uint32_t slot) {
+                const uint32_t kb = ring + slot * Cfg::SLOT, qb = qbase + g * Cfg::QG;
+#pragma unroll
+                for (int ks = 0; ks < HD / 16; ++ks) {
+                    const uint32_t off = (ks >> 2) * (128 * 128) + (ks & 3) * 32;
+                    umma_f16(tm + g * 128, sw128_desc(qb + off), sw128_desc(kb + off), id_s, ks > 0);
+                }
+                umma_commit(smem_u32(&sh.sfull[g]));
+            };
+            while (ok && u < u1) {
+                const int j1 = part_end();
+                ok = wait(&sh.qfull, q) && wait(&sh.kvfull[n % NS], n / NS);
+                if (!ok) break;
+                tc_fence_after();
+                if (elect_one()) {
+                    issue_s(0, n % NS);
+                    issue_s(1, n % NS);
+                    umma_commit(smem_u32(&sh.kvempty[n % NS]));
+                    if (j1 - j0 == 1) umma_commit(smem_u32(&sh.qempty));
+                }
+                __syncwarp();
+                ++n;
+                for (int j = j0; ok && j < j1; ++j) {
+                    const uint32_t vs = n % NS, vpar = n / NS, kn = (n + 1) % NS, kpar = (n + 1) / NS;
+                    const bool more = j + 1 < j1;
+                    ok = wait(&sh.kvfull[vs], vpar);
+                    if (!ok) break;
+                    // positions that no one wrote in the sequence's last box: 0 * whatever V holds has to be 0
+                    const int r1 = it.q.len - many_tile_pos(it, j);
+                    if (r1 < kTileN && r1 % a.box) {
+                        const int rows = a.box - r1 % a.box;
+                        for (int i = lane; i < rows * (HD / 8); i += 32) {
+                            const int r = r1 + i / (HD / 8), c = i % (HD / 8);
+                            const uint32_t at = ring + vs * Cfg::SLOT + (c >> 3) * (kTileN * 128) + r * 128 + ((c & 7) << 4);
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory");
+                        }
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                    }
+                    for (int g = 0; ok && g < 2; ++g) {
+                        ok = wait(&sh.pready[g], np);
+                        if (ok && g == 0 && more) ok = wait(&sh.kvfull[kn], kpar);
+                        if (!ok) break;
+                        tc_fence_after();
+                        if (elect_one()) {
+                            const uint32_t vb = ring + vs * Cfg::SLOT;
+#pragma unroll
+                            for (int ks = 0; ks < kTileN / 16; ++ks)
+                                umma_f16_ts(tm + 256 + g * HD, tm + g * 128 + ks * 8, v_desc(vb + ks * 2048), id_o,
+                                            (j > j0 || ks > 0) ? 1u : 0u);
+                            if (g == 1) umma_commit(smem_u32(&sh.kvempty[vs]));
+                            if (more) {
+                                issue_s(g, kn);
+                                if (g == 1) {
+                                    umma_commit(smem_u32(&sh.kvempty[kn]));
+                                    if (j + 2 == j1) umma_commit(smem_u32(&sh.qempty));
+                                }
+                            } else {
+                                umma_commit(smem_u32(&sh.ofull[g]));
+                            }
+                        }
+                        __syncwarp();
+                    }
+                    ++np;
+                    n += more ? 2 : 1;
+                }
+                ++q;
+                next_item(j1);
+            }
+            // every MMA issued is complete before TMEM is given back
+            if (elect_one()) umma_commit(smem_u32(&sh.done));
+            __syncwarp();
+            mbar_wait_bounded(smem_u32(&sh.done), 0, err, lim);
+        }
+    } else {
+        // ---- softmax: thread = row ----
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        const int g = warp >> 2, lr = (warp & 3) * 32 + lane;
+        const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+        const uint32_t ts = tm + g * 128 + lanes, to = tm + 256 + g * HD + lanes;
+        const int tok_in = lr / a.a.group, hh = lr - tok_in * a.a.group;
+        const float sc = a.a.scale2;
+        uint32_t cnt = 0, items = 0, joins = 0;
+        bool ok = true;
+        auto join = [&]() {   // of the 256 softmax threads; bounded like every wait
+            mbar_arrive(smem_u32(&sh.join));
+            ok = wait(&sh.join, joins++);
+            return ok;
+        };
+        while (ok && u < u1) {
+            const int j1 = part_end();
+            const int tok = it.t0 + g * a.tpt + tok_in;
+            const bool on = tok_in < a.tpt && tok < it.t1;
+            const int p0 = it.q.len - it.q.n, pos = on ? p0 + tok : -1;
+            // the group's first and last position
+            const int pmin = p0 + it.t0 + g * a.tpt, pmax = p0 + min(it.t1, it.t0 + (g + 1) * a.tpt) - 1;
+            float m = -INFINITY, l = 0.f;
+            for (int j = j0; j < j1; ++j) {
+                ok = wait(&sh.sfull[g], cnt);
+                if (!ok) break;
+                ++cnt;
+                tc_fence_after();
+                uint32_t s[128];
+                tmem_ld32(ts, s);
+                tmem_ld32(ts + 32, s + 32);
+                tmem_ld32(ts + 64, s + 64);
+                tmem_ld32(ts + 96, s + 96);
+                tmem_wait_ld(s);
+                after_wait(s + 32);
+                after_wait(s + 64);
+                after_wait(s + 96);
+                const int k0 = many_tile_pos(it, j);
+                if (k0 + kTileN - 1 > pmin) {
+                    const int last = pos - k0;   // the last column that the row sees
+#pragma unroll
+                    for (int c = 0; c < 128; ++c)
+                        if (c > last) s[c] = 0xFF800000u;
+                }
+                if (a.a.window > 0 && k0 <= pmax - a.a.window && k0 + kTileN > a.a.sinks) {
+                    const int first = pos - a.a.window + 1 - k0, sinks = a.a.sinks - k0;   // columns below first, past the sinks
+#pragma unroll
+                    for (int c = 0; c < 128; ++c)
+                        if (c < first && c >= sinks) s[c] = 0xFF800000u;
+                }
+                float mx = -INFINITY;
+#pragma unroll
+                for (int c = 0; c < 128; c += 2)
+                    mx = fmaxf(fmaxf(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), mx);
+                mx *= sc;
+                if (__any_sync(0xFFFFFFFFu, mx > m + 8.f)) {
+                    const float mn = fmaxf(m, mx);
+                    const float corr = m == -INFINITY ? 0.f : ex2(m - mn);
+                    l *= corr;
+                    m = mn;
+                    if (j > j0) {
+#pragma unroll 1
+                        for (int c = 0; c < HD; c += 32) {
+                            uint32_t o[32];
+                            tmem_ld32(to + c, o);
+                            tmem_wait_ld(o);
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
+                            tmem_st32(to + c, o);
+                        }
+                    }
+                }
+                const float nm = m == -INFINITY ? 0.f : -m;
+                const float2 sc2 = make_float2(sc, sc), nm2 = make_float2(nm, nm);
+                float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+                for (int c = 0; c < 64; ++c) {   // the pairs take the places of scores that are done with
+                    float2 x = __ffma2_rn(make_float2(__uint_as_float(s[2 * c]), __uint_as_float(s[2 * c + 1])), sc2, nm2);
+                    x.x = ex2(x.x);
+                    x.y = ex2(x.y);
+                    sum[c & 1] = __fadd2_rn(sum[c & 1], x);
+                    if constexpr (std::is_same<I, __nv_bfloat16>::value) {
+                        const __nv_bfloat162 h = __floats2bfloat162_rn(x.x, x.y);
+                        s[c] = *reinterpret_cast<const uint32_t *>(&h);
+                    } else {
+                        const __half2 h = __floats2half2_rn(x.x, x.y);
+                        s[c] = *reinterpret_cast<const uint32_t *>(&h);
+                    }
+                    if (c == 31) tmem_st32(ts, s);
+                }
+                tmem_st32(ts + 32, s + 32);
+                tmem_wait_st();
+                tc_fence_before();
+                mbar_arrive(smem_u32(&sh.pready[g]));
+                l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+            }
+            if (!ok || !wait(&sh.ofull[g], items)) break;
+            ++items;
+            tc_fence_after();
+            // ---- the part's result: out, or the workspace ----
+            const bool whole = j0 == 0 && j1 == it.n;
+            float *part = a.a.part + static_cast<size_t>(2 * cta + (j0 == 0 ? 1 : 0)) * Cfg::PART;
+            const int row = g * 128 + lr;
+            I *out = static_cast<I *>(const_cast<void *>(a.a.o.p)) + (it.q.row0 + (on ? tok : 0)) * a.a.o.row +
+                     (it.h * a.a.group + hh) * a.a.o.head;
+            bool odd = !isfinite(l) || m == INFINITY || *reinterpret_cast<volatile int *>(&sh.bad);
+            const float inv = l == 0.f ? 0.f : 1.0f / l;
+#pragma unroll 1
+            for (int c = 0; c < HD; c += 32) {
+                uint32_t o[32];
+                tmem_ld32(to + c, o);
+                tmem_wait_ld(o);
+#pragma unroll
+                for (int i = 0; i < 32; ++i) odd = odd || !isfinite(__uint_as_float(o[i]));
+                if (whole) {
+                    if (on) {
+#pragma unroll
+                        for (int i = 0; i < 32; i += 8) {
+                            float x[8];
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) x[e] = l == 0.f ? 0.f : __uint_as_float(o[i + e]) * inv;
+                            kv_store8(out + c + i, x);
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4)
+                        reinterpret_cast<uint4 *>(part)[((c + i) / 4) * 256 + row] = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                }
+            }
+            if (!whole) part[256 * HD + row] = m, part[256 * HD + 256 + row] = l;
+            // rows that are not finite: V of a position that this row does not see may have been
+            // (0 * NaN), or a page lies outside the pool.  Once more, over their own positions only.
+            for (unsigned todo = __ballot_sync(0xFFFFFFFFu, odd && on); todo; todo &= todo - 1) {
+                const int src = __ffs(todo) - 1;
+                const int rtok = __shfl_sync(0xFFFFFFFFu, tok, src), rhh = __shfl_sync(0xFFFFFFFFu, hh, src);
+                float rm, rl, acc[HD / 32];
+                many_row_again<HD, I>(a, it, rtok, rhh, j0, j1, rm, rl, acc);
+                const int rrow = g * 128 + (warp & 3) * 32 + src;
+                I *ro = static_cast<I *>(const_cast<void *>(a.a.o.p)) + (it.q.row0 + rtok) * a.a.o.row +
+                        (it.h * a.a.group + rhh) * a.a.o.head;
+                for (int d = 0; d < HD / 32; ++d) {
+                    const int dim = lane * (HD / 32) + d;
+                    if (whole) kv_store1(ro + dim, rl == 0.f ? 0.f : acc[d] / rl);
+                    else part[((dim / 4) * 256 + rrow) * 4 + (dim & 3)] = acc[d];
+                }
+                if (!whole && lane == 0) part[256 * HD + rrow] = rm, part[256 * HD + 256 + rrow] = rl;
+                __syncwarp();
+            }
+            if (!whole) {
+                // ---- the last CTA of the item to arrive adds the parts, in CTA order ----
+                const unsigned long long i0 = u - j0, i1 = i0 + it.n;
+                const unsigned c0 = static_cast<unsigned>(((i0 + 1) * G - 1) / total);
+                const unsigned c1 = static_cast<unsigned>((i1 * G - 1) / total);
+                __threadfence();
+                if (!join()) break;
+                if (tid == 0) sh.last = atomicInc(a.a.arrived + c0, c1 - c0) == c1 - c0;   // wraps back to zero
+                if (!join()) break;
+                if (sh.last) {
+                    __threadfence();
+                    float M = -INFINITY, L = 0.f;
+                    for (unsigned c = c0; c <= c1; ++c)
+                        M = fmaxf(M, __ldcg(a.a.part + static_cast<size_t>(2 * c + (c == c0 ? 1 : 0)) * Cfg::PART + 256 * HD + row));
+                    for (unsigned c = c0; c <= c1; ++c) {
+                        const float *pp = a.a.part + static_cast<size_t>(2 * c + (c == c0 ? 1 : 0)) * Cfg::PART + 256 * HD + row;
+                        const float pm = __ldcg(pp), pl = __ldcg(pp + 256);
+                        L += pm == -INFINITY ? pl : ex2(pm - M) * pl;
+                    }
+#pragma unroll 1
+                    for (int d = 0; d < HD; d += 32) {
+                        float x[32];
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) x[i] = 0.f;
+                        for (unsigned c = c0; c <= c1; ++c) {
+                            const float *pp = a.a.part + static_cast<size_t>(2 * c + (c == c0 ? 1 : 0)) * Cfg::PART;
+                            const float pm = __ldcg(pp + 256 * HD + row), f = pm == -INFINITY ? 0.f : ex2(pm - M);
+#pragma unroll
+                            for (int i = 0; i < 32; i += 4) {
+                                const float4 v = __ldcg(reinterpret_cast<const float4 *>(pp) + ((d + i) / 4) * 256 + row);
+                                x[i] = fmaf(f, v.x, x[i]);
+                                x[i + 1] = fmaf(f, v.y, x[i + 1]);
+                                x[i + 2] = fmaf(f, v.z, x[i + 2]);
+                                x[i + 3] = fmaf(f, v.w, x[i + 3]);
+                            }
+                        }
+                        if (on) {
+#pragma unroll
+                            for (int i = 0; i < 32; i += 8) {
+                                float y[8];
+#pragma unroll
+                                for (int e = 0; e < 8; ++e) y[e] = L == 0.f ? 0.f : x[i + e] / L;
+                                kv_store8(out + d + i, y);
+                            }
+                        }
+                    }
+                }
+                if (!join()) break;   // sh.last is free again
+            }
+            next_item(j1);
+        }
+    }
+    // ---- the end: nothing in flight, TMEM given back ----
+    tc_fence_before();
+    __syncthreads();
+    if (sh.fail) {   // a wait ran out: the copies still in flight, as far as they come
+        if (warp == 9)
+            for (uint32_t n = kv_issued > NS ? kv_issued - NS : 0; n < kv_issued; ++n)
+                mbar_wait_bounded(smem_u32(&sh.kvfull[n % NS]), (n / NS) & 1u, err, lim);
+        if (warp == 10 && q_issued > 0) mbar_wait_bounded(smem_u32(&sh.qfull), (q_issued - 1) & 1u, err, lim);
+    }
+    __syncthreads();
+    if (warp == 8) {
+        tc_fence_after();
+        tmem_dealloc(tm, 512);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+size_t kv_many_part_bytes() { return sizeof(float) * ManyCfg<128>::PART; }
+
+template <int HD, class I>
+static int many_launch(ManyArgs &m, int tc, int sms, cudaStream_t st)
+{
+    AttnArgs &a = m.a;
+    CUtensorMap qm, km, vm;
+    int ax[3];
+    m.box = kTileN;
+    while (a.c.page_size % m.box) m.box >>= 1;   // at least 16: it divides every page
+    if (!kv_maps(a.c, HD, tc, m.box, &km, &vm, ax)) return 0;
+    a.ax_pos = ax[0], a.ax_head = ax[1], a.ax_page = ax[2];
+    // Q: dimension, head, token; boxes of 64 dimensions x G heads x the group's tokens
+    const cuuint64_t dims[3] = {static_cast<cuuint64_t>(HD), static_cast<cuuint64_t>(a.nh),
+                                static_cast<cuuint64_t>(a.b.n_tokens)};
+    const cuuint64_t strides[2] = {static_cast<cuuint64_t>(a.nh > 1 ? a.q.head : HD) * 2,
+                                   static_cast<cuuint64_t>(a.b.n_tokens > 1 ? a.q.row : static_cast<long long>(a.nh) * HD) * 2};
+    const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(a.group), static_cast<cuuint32_t>(m.tpt)}, estr[3] = {1, 1, 1};
+    EncodeTiled enc = encode_tiled();
+    if (!enc || enc(&qm, tc == QT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+                    const_cast<void *>(a.q.p), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS) {
+        return -1;   // strides that a tensor map cannot have
+    }
+    auto fn = k_kv_many<HD, I>;
+    if (!smem_attr_once(reinterpret_cast<const void *>(fn), ManyCfg<HD>::SMEM)) {
+        cudaGetLastError();
+        return 0;
+    }
+    fn<<<sms < kManyCtas ? sms : kManyCtas, kManyThreads, ManyCfg<HD>::SMEM, st>>>(qm, km, vm, m);
+    return cudaGetLastError() == cudaSuccess ? 1 : 0;
+}
+
+int kv_many_launch(AttnArgs a, int hd, int tc, int few_rows, int sms, cudaStream_t st)
+{
+    ManyArgs m{a, 128 / a.group, few_rows, 0, tc == QT_BF16};
+    if (hd == 128)
+        return tc == QT_BF16 ? many_launch<128, __nv_bfloat16>(m, tc, sms, st) : many_launch<128, __half>(m, tc, sms, st);
+    return tc == QT_BF16 ? many_launch<64, __nv_bfloat16>(m, tc, sms, st) : many_launch<64, __half>(m, tc, sms, st);
+}
+
+}  // namespace tb
