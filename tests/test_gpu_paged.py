@@ -154,6 +154,19 @@ def test_hidden_values_have_no_influence(paged, kq, io, bad):
         assert bool(got[where - 20:40].isnan().all())   # rows that see it
 
 
+@pytest.mark.parametrize("io", [F32, F16, BF16])
+@pytest.mark.parametrize("which", ["k", "v"])
+def test_nan_in_k_or_v_alone(paged, kq, io, which):
+    """A NaN that a row sees makes its output NaN, wherever in a tile it lies; rows before it stay finite."""
+    for where in (0, 1, 37, 100, 255):
+        c = Case(paged, [300, 1], [300, 270], 4, 2, 64, io, io, 16, seed=18)
+        for s in range(2):
+            page = int(c.table[s, where // 16])
+            (c.k if which == "k" else c.v)[1, page, :, where % 16] = math.nan
+        got = c.cache.attend(1, c.batch, c.q).isnan()
+        assert bool(got[where:].all()) and not bool(got[:where].any()), where
+
+
 def test_large_scores(paged, kq):
     """Scores up to some thousands: the running maximum keeps every exponent at or below zero."""
     c = Case(paged, [1, 33], [500, 100], 4, 2, 128, F32, F32, 16, seed=7)

@@ -13,11 +13,12 @@
 //
 // Inside a CTA (384 threads):
 //   warps 0-3, 4-7  softmax of row group 0 / 1, one row a thread;
-//   warp 8          the MMAs, one elected thread: S_g = Q_g K^T (128 x 128, both
+//   warp 8          the MMAs, one thread: S_g = Q_g K^T (128 x 128, both
 //                   operands in shared memory), O_g += P_g V (P_g read from TMEM);
 //   warp 9          K and V tiles by TMA into a ring, page by page;
 //   warp 10         Q tiles by TMA (the next item's while the last one's softmax
-//                   and epilogue still run).
+//                   and epilogue still run);
+//   warp 11         zeros into V past a sequence's end.
 // TMEM: S_0, S_1 (128 fp32 columns each, P_g overwrites the first half of S_g as
 // 16-bit pairs), O_0, O_1.  The two groups take turns on the tensor core: while
 // one's softmax runs, the other's products do.  The MMA order PV_g(j), S_g(j + 1)
@@ -36,6 +37,7 @@ namespace tb {
 
 static constexpr int kTileN = 128;      // positions of a tile
 static constexpr int kManyThreads = 384;
+static constexpr int kPolyOf8 = 3;      // of 8 pairs of scores, how many go through exp2_poly
 
 struct ManyArgs {
     AttnArgs a;
@@ -49,13 +51,14 @@ template <int HD>
 struct ManyCfg {
     static constexpr int SLOT = kTileN * HD * 2;         // one K or V tile
     static constexpr int QG = 128 * HD * 2;              // one row group's Q
-    static constexpr int NS = HD == 128 ? 5 : 10;        // ring slots
-    static constexpr int SMEM = 1024 + 2 * QG + NS * SLOT + 1024;
+    static constexpr int NS = HD == 128 ? 4 : 8;         // ring slots
+    static constexpr int STAGE = 4096;                   // a softmax warp's staging for its output rows
+    static constexpr int SMEM = 1024 + 2 * QG + NS * SLOT + 8 * STAGE + 1024;
     static constexpr int PART = 256 * HD + 512;          // floats of a partial result: O, m, l
 };
 
 struct ManyShared {
-    uint64_t sfull[2], pready[2], ofull[2], qfull, qempty, done, join, kvfull[10], kvempty[10];
+    uint64_t sfull[2], pready[2][2], ofull[2], qfull, qempty, done, join, kvfull[8], kvempty[8], vready[8];
     unsigned long long scan[12], u0;
     uint32_t tmem;
     int seq, head, rt, off, fail, bad, last;
@@ -106,6 +109,28 @@ __device__ __forceinline__ void many_next(const ManyArgs &a, ManyItem &it)
         }
     }
     many_tiles(a, it.q, it.rt, &it);
+}
+// Units of one head of the lane's sequence q (n = 0: none); the whole warp calls it.
+// Long chunks' row tiles are counted by all lanes together.
+__device__ __forceinline__ unsigned long long many_head_units(const ManyArgs &a, const KvSeq &q)
+{
+    const int lane = threadIdx.x & 31, n_rt = (q.n + 2 * a.tpt - 1) / (2 * a.tpt);
+    unsigned long long f = 0;
+    if (n_rt <= 4)
+        for (int rt = 0; rt < n_rt; ++rt) f += many_tiles(a, q, rt, nullptr);
+    for (unsigned todo = __ballot_sync(0xFFFFFFFFu, n_rt > 4); todo; todo &= todo - 1) {
+        const int src = __ffs(todo) - 1;
+        KvSeq x = q;
+        x.n = __shfl_sync(0xFFFFFFFFu, q.n, src);
+        x.len = __shfl_sync(0xFFFFFFFFu, q.len, src);
+        const int m = __shfl_sync(0xFFFFFFFFu, n_rt, src);
+        unsigned long long c = 0;
+        for (int rt = lane; rt < m; rt += 32) c += many_tiles(a, x, rt, nullptr);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) c += __shfl_xor_sync(0xFFFFFFFFu, c, o);
+        if (lane == src) f = c;
+    }
+    return f;
 }
 __device__ __forceinline__ int many_tile_pos(const ManyItem &it, int j) { return (j < it.ns ? j : j - it.ns + it.lo) * kTileN; }
 
@@ -171,11 +196,43 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *map
                  : "memory");
 }
 
+__device__ __forceinline__ void prefetch_map(const CUtensorMap *m)
+{
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(m)) : "memory");
+}
+
+// 2^x for two x, on the FMA pipe: the multi-function unit gives 4 results a clock
+// and sub-core, and 128 x 128 scores would hold it as long as the tensor core
+// needs for both products.  x = n + f with n the nearest integer (by adding 1.5 *
+// 2^23), 2^f on [-0.5, 0.5] by a polynomial of least relative error (Remez
+// exchange; degree 3: 7.5e-5, 4: 2.6e-6, to be rounded to bf16 or fp16), n into
+// the exponent.  x below -126 gives about 2^-126.
+template <int DEG>
+__device__ __forceinline__ float2 exp2_poly(float2 x)
+{
+    constexpr float C3[4] = {0.9999280735f, 0.6932609855f, 0.2426111222f, 0.05517166906f};
+    constexpr float C4[5] = {0.9999992614f, 0.6931218147f, 0.2402474482f, 0.05591786032f, 0.009570101912f};
+    auto c = [&](int i) { return DEG == 3 ? make_float2(C3[i > 3 ? 0 : i], C3[i > 3 ? 0 : i]) : make_float2(C4[i], C4[i]); };
+    // a NaN stays one here and leaves as 2^127 or more, which P's rounding makes
+    // infinite: the row is then done again
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-126.f));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-126.f));
+    const float2 big = make_float2(12582912.f, 12582912.f), nbig = make_float2(-12582912.f, -12582912.f);
+    const float2 t = __fadd2_rn(x, big);
+    const float2 n = __fadd2_rn(t, nbig);
+    const float2 f = __ffma2_rn(n, make_float2(-1.f, -1.f), x);
+    float2 p = c(DEG);
+#pragma unroll
+    for (int i = DEG - 1; i >= 0; --i) p = __ffma2_rn(p, f, c(i));
+    return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)),
+                       __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
+}
+
 // One row again, over the visible positions of the part's tiles [j0, j1) only, by
-// the whole warp: acc[d] of dimensions lane * HD / 32 + d, m and l.
+// the whole warp: res = m, l and the sums of dimensions lane * HD / 32 ....
 template <int HD, class I>
-__device__ __noinline__ void many_row_again(const ManyArgs &a, const ManyItem &it, int tok, int hh, int j0, int j1,
-                                            float &m, float &l, float (&acc)[HD / 32])
+__device__ __noinline__ void many_row_again(const ManyArgs &a, const ManyItem it, int tok, int hh, int j0, int j1,
+                                            float *res)
 {
     constexpr int D = HD / 32;
     const int lane = threadIdx.x & 31;
@@ -191,11 +248,12 @@ __device__ __noinline__ void many_row_again(const ManyArgs &a, const ManyItem &i
                          ac[0], a.a.err);
     kv_row_attend<HD, I>(a.a.b, a.a.c, it.s, it.h, pos, c0, min(c1, it.q.len), a.a.window, a.a.sinks, q, am[1], al[1],
                          ac[1], a.a.err);
-    m = fmaxf(am[0], am[1]);
+    const float m = fmaxf(am[0], am[1]);
     const float f0 = am[0] == -INFINITY ? 0.f : ex2(am[0] - m), f1 = am[1] == -INFINITY ? 0.f : ex2(am[1] - m);
-    l = (am[0] == -INFINITY ? al[0] : al[0] * f0) + (am[1] == -INFINITY ? al[1] : al[1] * f1);
+    res[0] = m;
+    res[1] = (am[0] == -INFINITY ? al[0] : al[0] * f0) + (am[1] == -INFINITY ? al[1] : al[1] * f1);
 #pragma unroll
-    for (int d = 0; d < D; ++d) acc[d] = ac[0][d] * f0 + ac[1][d] * f1;
+    for (int d = 0; d < D; ++d) res[2 + d] = ac[0][d] * f0 + ac[1][d] * f1;
 }
 
 template <int HD, class I>
@@ -206,9 +264,11 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     using Cfg = ManyCfg<HD>;
     constexpr int CB = HD / 64;   // 128-byte columns
     constexpr int NS = Cfg::NS;
+    constexpr bool BF = std::is_same<I, __nv_bfloat16>::value;
     extern __shared__ __align__(1024) uint8_t smraw[];
     uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smraw) + 1023) & ~uintptr_t(1023));
-    ManyShared &sh = *reinterpret_cast<ManyShared *>(sm + 2 * Cfg::QG + NS * Cfg::SLOT);
+    uint8_t *stage = sm + 2 * Cfg::QG + NS * Cfg::SLOT;
+    ManyShared &sh = *reinterpret_cast<ManyShared *>(stage + 8 * Cfg::STAGE);
     const uint32_t qbase = smem_u32(sm), ring = qbase + 2 * Cfg::QG;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t lim = a.a.wait_limit;
@@ -217,7 +277,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     if (tid == 0) {
         for (int g = 0; g < 2; ++g) {
             mbar_init(smem_u32(&sh.sfull[g]), 1);
-            mbar_init(smem_u32(&sh.pready[g]), 128);
+            mbar_init(smem_u32(&sh.pready[g][0]), 128);
+            mbar_init(smem_u32(&sh.pready[g][1]), 128);
             mbar_init(smem_u32(&sh.ofull[g]), 1);
         }
         mbar_init(smem_u32(&sh.qfull), 1);
@@ -227,26 +288,26 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         for (int i = 0; i < NS; ++i) {
             mbar_init(smem_u32(&sh.kvfull[i]), 1);
             mbar_init(smem_u32(&sh.kvempty[i]), 1);
+            mbar_init(smem_u32(&sh.vready[i]), 1);
         }
         fence_mbar_init();
         sh.fail = 0;
         sh.bad = 0;
     }
+    if (warp == 9 && lane < 2) prefetch_map(lane ? &vmap : &kmap);
+    if (warp == 10 && lane == 0) prefetch_map(&qmap);
     // ---- this CTA's share of all units: a scan over the sequences ----
     const int per = (a.a.b.n_seqs + kManyThreads - 1) / kManyThreads;
     const int sq0 = min(a.a.b.n_seqs, tid * per), sq1 = min(a.a.b.n_seqs, sq0 + per);
-    auto head_units = [&](const KvSeq &q) {
-        unsigned long long f = 0;
-        const int n_rt = (q.n + 2 * a.tpt - 1) / (2 * a.tpt);
-        for (int rt = 0; rt < n_rt; ++rt) f += many_tiles(a, q, rt, nullptr);
-        return f;
-    };
     unsigned long long mine = 0;
     bool bad_seq = false;
-    for (int s = sq0; s < sq1; ++s) {
-        KvSeq q;
-        bad_seq = bad_seq || !kv_seq(a.a.b, a.a.c, s, q, nullptr);
-        if (many_seq(a, s, q)) mine += head_units(q) * a.a.c.n_kv_heads;
+    for (int k = 0; k < per; ++k) {
+        KvSeq q{};
+        if (sq0 + k < sq1) {
+            bad_seq = bad_seq || !kv_seq(a.a.b, a.a.c, sq0 + k, q, nullptr);
+            if (!many_seq(a, sq0 + k, q)) q.n = 0;
+        }
+        mine += many_head_units(a, q) * a.a.c.n_kv_heads;
     }
     unsigned long long incl = mine;
 #pragma unroll
@@ -264,28 +325,46 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     const unsigned G = total < gridDim.x ? static_cast<unsigned>(total) : gridDim.x, cta = blockIdx.x;
     if (cta >= G) return;
     const unsigned long long u0 = total * cta / G, u1 = total * (cta + 1) / G;
-    if (before <= u0 && u0 < before + mine) {
+    const bool mine_u0 = before <= u0 && u0 < before + mine;
+    if (__any_sync(0xFFFFFFFFu, mine_u0)) {   // the warp whose sequences hold u0
         unsigned long long at = before;
-        for (int s = sq0; s < sq1; ++s) {
-            KvSeq q;
-            if (!many_seq(a, s, q)) continue;
-            const unsigned long long f = head_units(q), n = f * a.a.c.n_kv_heads;
-            if (u0 < at + n) {
-                unsigned long long r = (u0 - at) % f;
-                int rt = 0;
-                for (;; ++rt) {
-                    const unsigned k = many_tiles(a, q, rt, nullptr);
-                    if (r < k) break;
-                    r -= k;
-                }
-                sh.seq = s;
-                sh.head = static_cast<int>((u0 - at) / f);
-                sh.rt = rt;
-                sh.off = static_cast<int>(r);
-                break;
-            }
+        bool found = false;
+        KvSeq fq{};
+        int fs = 0;
+        unsigned long long fr = 0, ff = 1;
+        for (int k = 0; k < per; ++k) {
+            KvSeq q{};
+            if (sq0 + k < sq1 && !many_seq(a, sq0 + k, q)) q.n = 0;
+            const unsigned long long f = many_head_units(a, q), n = f * a.a.c.n_kv_heads;
+            if (mine_u0 && !found && u0 < at + n) found = true, fq = q, fs = sq0 + k, fr = u0 - at, ff = f;
             at += n;
         }
+        const int src = __ffs(__ballot_sync(0xFFFFFFFFu, found)) - 1;
+        fq.n = __shfl_sync(0xFFFFFFFFu, fq.n, src);
+        fq.len = __shfl_sync(0xFFFFFFFFu, fq.len, src);
+        const unsigned long long r = __shfl_sync(0xFFFFFFFFu, fr, src), f = __shfl_sync(0xFFFFFFFFu, ff, src);
+        unsigned long long rem = r % f;   // units of the head before u0: the row tile, 32 at a time
+        const int n_rt = (fq.n + 2 * a.tpt - 1) / (2 * a.tpt);
+        for (int base = 0; base < n_rt; base += 32) {
+            const unsigned long long k = base + lane < n_rt ? many_tiles(a, fq, base + lane, nullptr) : 0;
+            unsigned long long c = k;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const unsigned long long x = __shfl_up_sync(0xFFFFFFFFu, c, o);
+                if (lane >= o) c += x;
+            }
+            const unsigned hit = __ballot_sync(0xFFFFFFFFu, rem < c);
+            if (hit) {
+                if (lane == __ffs(hit) - 1) {
+                    sh.head = static_cast<int>(r / f);
+                    sh.rt = base + lane;
+                    sh.off = static_cast<int>(rem - (c - k));
+                }
+                break;
+            }
+            rem -= __shfl_sync(0xFFFFFFFFu, c, 31);
+        }
+        if (lane == src) sh.seq = fs;
     }
     if (warp == 8) {
         tmem_alloc(smem_u32(&sh.tmem), 512);
@@ -313,11 +392,18 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         if (u < u1) many_next(a, it);
     };
     auto failed = [&]() { return *reinterpret_cast<volatile int *>(&sh.fail) != 0; };
-    auto wait = [&](uint64_t *bar, uint32_t parity) {   // by a whole warp
-        const bool ok = mbar_wait_bounded(smem_u32(bar), parity & 1u, err, lim);
-        if (__all_sync(0xFFFFFFFFu, ok) && !failed()) return true;
+    auto wait1 = [&](uint64_t *bar, uint32_t parity) {   // by one thread; ends early when another role has given up
+        const uint32_t at = smem_u32(bar);
+        if (mbar_try_wait(at, parity & 1u)) return true;
+        for (uint32_t i = 0; i < lim && !failed(); ++i)
+            if (mbar_try_wait(at, parity & 1u)) return true;
+        if (!failed()) atomicExch(err, ERR_WAIT_TIMEOUT);
         *reinterpret_cast<volatile int *>(&sh.fail) = 1;
         return false;
+    };
+    auto wait = [&](uint64_t *bar, uint32_t parity) {   // by a whole warp
+        const bool ok = wait1(bar, parity);
+        return __all_sync(0xFFFFFFFFu, ok) != 0;
     };
 
     uint32_t kv_issued = 0, q_issued = 0;   // in the warps that issue them
@@ -383,76 +469,90 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                 ++q_issued;
                 next_item(j1);
             }
-        } else if (warp == 8) {
-            // ---- the MMAs ----
-            const uint32_t fmt = a.bf16 ? 1u : 0u;
-            const uint32_t id_s = (1u << 4) | (fmt << 7) | (fmt << 10) | ((kTileN >> 3) << 17) | (8u << 24);
-            const uint32_t id_o = (1u << 4) | (fmt << 7) | (fmt << 10) | (1u << 16) | ((HD >> 3) << 17) | (8u << 24);
-            uint32_t n = 0, q = 0, np = 0;   // ring slots, items and P tiles taken
+        } else if (warp == 11) {
+            // ---- every V tile passes by here.  Positions that no one wrote, in the box that
+            // holds the sequence's end: whatever V has there, 0 * it has to be 0 ----
             bool ok = true;
-            auto issue_s = [&](int g, uint32_t slot) {
-                const uint32_t kb = ring + slot * Cfg::SLOT, qb = qbase + g * Cfg::QG;
-#pragma unroll
-                for (int ks = 0; ks < HD / 16; ++ks) {
-                    const uint32_t off = (ks >> 2) * (128 * 128) + (ks & 3) * 32;
-                    umma_f16(tm + g * 128, sw128_desc(qb + off), sw128_desc(kb + off), id_s, ks > 0);
-                }
-                umma_commit(smem_u32(&sh.sfull[g]));
-            };
+            uint32_t n = 1;
             while (ok && u < u1) {
                 const int j1 = part_end();
-                ok = wait(&sh.qfull, q) && wait(&sh.kvfull[n % NS], n / NS);
-                if (!ok) break;
-                tc_fence_after();
-                if (elect_one()) {
-                    issue_s(0, n % NS);
-                    issue_s(1, n % NS);
-                    umma_commit(smem_u32(&sh.kvempty[n % NS]));
-                    if (j1 - j0 == 1) umma_commit(smem_u32(&sh.qempty));
-                }
-                __syncwarp();
-                ++n;
-                for (int j = j0; ok && j < j1; ++j) {
-                    const uint32_t vs = n % NS, vpar = n / NS, kn = (n + 1) % NS, kpar = (n + 1) / NS;
-                    const bool more = j + 1 < j1;
-                    ok = wait(&sh.kvfull[vs], vpar);
+                for (int j = j0; j < j1; ++j, n += 2) {
+                    const uint32_t slot = n % NS;
+                    ok = wait(&sh.kvfull[slot], n / NS);
                     if (!ok) break;
-                    // positions that no one wrote in the sequence's last box: 0 * whatever V holds has to be 0
                     const int r1 = it.q.len - many_tile_pos(it, j);
                     if (r1 < kTileN && r1 % a.box) {
                         const int rows = a.box - r1 % a.box;
                         for (int i = lane; i < rows * (HD / 8); i += 32) {
                             const int r = r1 + i / (HD / 8), c = i % (HD / 8);
-                            const uint32_t at = ring + vs * Cfg::SLOT + (c >> 3) * (kTileN * 128) + r * 128 + ((c & 7) << 4);
+                            const uint32_t at = ring + slot * Cfg::SLOT + (c >> 3) * (kTileN * 128) + r * 128 + ((c & 7) << 4);
                             asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory");
                         }
                         fence_proxy_async_smem();
-                        __syncwarp();
                     }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(smem_u32(&sh.vready[slot]));
+                }
+                next_item(j1);
+            }
+        } else if (lane == 0) {
+            // ---- the MMAs, one thread ----
+            const uint32_t fmt = a.bf16 ? 1u : 0u;
+            const uint32_t id_s = (1u << 4) | (fmt << 7) | (fmt << 10) | ((kTileN >> 3) << 17) | (8u << 24);
+            const uint32_t id_o = (1u << 4) | (fmt << 7) | (fmt << 10) | (1u << 16) | ((HD >> 3) << 17) | (8u << 24);
+            const uint64_t qd = sw128_desc(qbase), kd = sw128_desc(ring), vd = v_desc(ring);
+            uint32_t n = 0, q = 0, np = 0;   // ring slots, items and P tiles taken
+            bool ok = true;
+            auto issue_s = [&](int g, uint32_t slot) {
+                const uint64_t qg = qd + ((g * Cfg::QG) >> 4), kg = kd + ((slot * Cfg::SLOT) >> 4);
+#pragma unroll
+                for (int ks = 0; ks < HD / 16; ++ks) {
+                    const uint32_t off = ((ks >> 2) * (128 * 128) + (ks & 3) * 32) >> 4;
+                    umma_f16(tm + g * 128, qg + off, kg + off, id_s, ks > 0);
+                }
+                umma_commit(smem_u32(&sh.sfull[g]));
+            };
+            while (ok && u < u1) {
+                const int j1 = part_end();
+                ok = wait1(&sh.qfull, q) && wait1(&sh.kvfull[n % NS], n / NS);
+                if (!ok) break;
+                tc_fence_after();
+                issue_s(0, n % NS);
+                issue_s(1, n % NS);
+                umma_commit(smem_u32(&sh.kvempty[n % NS]));
+                if (j1 - j0 == 1) umma_commit(smem_u32(&sh.qempty));
+                ++n;
+                for (int j = j0; j < j1; ++j) {
+                    const uint32_t vs = n % NS, vpar = n / NS, kn = (n + 1) % NS, kpar = (n + 1) / NS;
+                    const bool more = j + 1 < j1;
+                    const uint64_t vg = vd + ((vs * Cfg::SLOT) >> 4);
+                    ok = wait1(&sh.vready[vs], vpar);
                     for (int g = 0; ok && g < 2; ++g) {
-                        ok = wait(&sh.pready[g], np);
-                        if (ok && g == 0 && more) ok = wait(&sh.kvfull[kn], kpar);
+                        ok = wait1(&sh.pready[g][0], np);
                         if (!ok) break;
                         tc_fence_after();
-                        if (elect_one()) {
-                            const uint32_t vb = ring + vs * Cfg::SLOT;
 #pragma unroll
-                            for (int ks = 0; ks < kTileN / 16; ++ks)
-                                umma_f16_ts(tm + 256 + g * HD, tm + g * 128 + ks * 8, v_desc(vb + ks * 2048), id_o,
-                                            (j > j0 || ks > 0) ? 1u : 0u);
-                            if (g == 1) umma_commit(smem_u32(&sh.kvempty[vs]));
-                            if (more) {
-                                issue_s(g, kn);
-                                if (g == 1) {
-                                    umma_commit(smem_u32(&sh.kvempty[kn]));
-                                    if (j + 2 == j1) umma_commit(smem_u32(&sh.qempty));
-                                }
-                            } else {
-                                umma_commit(smem_u32(&sh.ofull[g]));
+                        for (int ks = 0; ks < kTileN / 32; ++ks)
+                            umma_f16_ts(tm + 256 + g * HD, tm + g * 128 + ks * 8, vg + ks * (2048 >> 4), id_o,
+                                        (j > j0 || ks > 0) ? 1u : 0u);
+                        ok = (g == 1 || !more || wait1(&sh.kvfull[kn], kpar)) && wait1(&sh.pready[g][1], np);
+                        if (!ok) break;
+                        tc_fence_after();
+#pragma unroll
+                        for (int ks = kTileN / 32; ks < kTileN / 16; ++ks)
+                            umma_f16_ts(tm + 256 + g * HD, tm + g * 128 + ks * 8, vg + ks * (2048 >> 4), id_o, 1u);
+                        if (g == 1) umma_commit(smem_u32(&sh.kvempty[vs]));
+                        if (more) {
+                            issue_s(g, kn);
+                            if (g == 1) {
+                                umma_commit(smem_u32(&sh.kvempty[kn]));
+                                if (j + 2 == j1) umma_commit(smem_u32(&sh.qempty));
                             }
+                        } else {
+                            umma_commit(smem_u32(&sh.ofull[g]));
                         }
-                        __syncwarp();
                     }
+                    if (!ok) break;
                     ++np;
                     n += more ? 2 : 1;
                 }
@@ -460,8 +560,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                 next_item(j1);
             }
             // every MMA issued is complete before TMEM is given back
-            if (elect_one()) umma_commit(smem_u32(&sh.done));
-            __syncwarp();
+            umma_commit(smem_u32(&sh.done));
             mbar_wait_bounded(smem_u32(&sh.done), 0, err, lim);
         }
     } else {
@@ -514,10 +613,11 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                     for (int c = 0; c < 128; ++c)
                         if (c < first && c >= sinks) s[c] = 0xFF800000u;
                 }
-                float mx = -INFINITY;
+                float mxs[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                 for (int c = 0; c < 128; c += 2)
-                    mx = fmaxf(fmaxf(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), mx);
+                    mxs[(c >> 1) & 3] = fmaxf(fmaxf(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), mxs[(c >> 1) & 3]);
+                float mx = fmaxf(fmaxf(mxs[0], mxs[1]), fmaxf(mxs[2], mxs[3]));
                 mx *= sc;
                 if (__any_sync(0xFFFFFFFFu, mx > m + 8.f)) {
                     const float mn = fmaxf(m, mx);
@@ -539,25 +639,32 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                 const float nm = m == -INFINITY ? 0.f : -m;
                 const float2 sc2 = make_float2(sc, sc), nm2 = make_float2(nm, nm);
                 float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+                // P in two halves: the product of the first starts while the second is computed
 #pragma unroll
-                for (int c = 0; c < 64; ++c) {   // the pairs take the places of scores that are done with
-                    float2 x = __ffma2_rn(make_float2(__uint_as_float(s[2 * c]), __uint_as_float(s[2 * c + 1])), sc2, nm2);
-                    x.x = ex2(x.x);
-                    x.y = ex2(x.y);
-                    sum[c & 1] = __fadd2_rn(sum[c & 1], x);
-                    if constexpr (std::is_same<I, __nv_bfloat16>::value) {
-                        const __nv_bfloat162 h = __floats2bfloat162_rn(x.x, x.y);
-                        s[c] = *reinterpret_cast<const uint32_t *>(&h);
-                    } else {
-                        const __half2 h = __floats2half2_rn(x.x, x.y);
-                        s[c] = *reinterpret_cast<const uint32_t *>(&h);
+                for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                    for (int c = h * 32; c < h * 32 + 32; ++c) {   // the pairs take the places of scores that are done with
+                        float2 x = __ffma2_rn(make_float2(__uint_as_float(s[2 * c]), __uint_as_float(s[2 * c + 1])), sc2, nm2);
+                        if ((c & 7) < kPolyOf8) {
+                            x = exp2_poly<BF ? 3 : 4>(x);
+                        } else {
+                            x.x = ex2(x.x);
+                            x.y = ex2(x.y);
+                        }
+                        sum[c & 1] = __fadd2_rn(sum[c & 1], x);
+                        if constexpr (BF) {
+                            const __nv_bfloat162 w = __floats2bfloat162_rn(x.x, x.y);
+                            s[c] = *reinterpret_cast<const uint32_t *>(&w);
+                        } else {
+                            const __half2 w = __floats2half2_rn(x.x, x.y);
+                            s[c] = *reinterpret_cast<const uint32_t *>(&w);
+                        }
                     }
-                    if (c == 31) tmem_st32(ts, s);
+                    tmem_st32(ts + h * 32, s + h * 32);
+                    tmem_wait_st();
+                    tc_fence_before();
+                    mbar_arrive(smem_u32(&sh.pready[g][h]));
                 }
-                tmem_st32(ts + 32, s + 32);
-                tmem_wait_st();
-                tc_fence_before();
-                mbar_arrive(smem_u32(&sh.pready[g]));
                 l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
             }
             if (!ok || !wait(&sh.ofull[g], items)) break;
@@ -569,6 +676,17 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             const int row = g * 128 + lr;
             I *out = static_cast<I *>(const_cast<void *>(a.a.o.p)) + (it.q.row0 + (on ? tok : 0)) * a.a.o.row +
                      (it.h * a.a.group + hh) * a.a.o.head;
+            I *mine = reinterpret_cast<I *>(stage + warp * Cfg::STAGE);   // [32 rows][64], 16-byte pieces swizzled
+            const long long off = on ? out - static_cast<I *>(const_cast<void *>(a.a.o.p)) : -1;
+            auto put_rows = [&](int d) {   // dimensions [d, d + 64) of the warp's rows
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int r = i * 4 + (lane >> 3), k = lane & 7;
+                    const long long ro = __shfl_sync(0xFFFFFFFFu, off, r);
+                    const uint4 v = *reinterpret_cast<const uint4 *>(mine + r * 64 + ((k ^ r) & 7) * 8);
+                    if (ro >= 0) *reinterpret_cast<uint4 *>(static_cast<I *>(const_cast<void *>(a.a.o.p)) + ro + d + k * 8) = v;
+                }
+            };
             bool odd = !isfinite(l) || m == INFINITY || *reinterpret_cast<volatile int *>(&sh.bad);
             const float inv = l == 0.f ? 0.f : 1.0f / l;
 #pragma unroll 1
@@ -579,14 +697,18 @@ __global__ void __launch_bounds__(kManyThreads, 1)
 #pragma unroll
                 for (int i = 0; i < 32; ++i) odd = odd || !isfinite(__uint_as_float(o[i]));
                 if (whole) {
-                    if (on) {
+                    // 64 dimensions of the warp's rows through shared memory, so that 8 lanes write 128 bytes
 #pragma unroll
-                        for (int i = 0; i < 32; i += 8) {
-                            float x[8];
+                    for (int i = 0; i < 32; i += 8) {
+                        float x[8];
 #pragma unroll
-                            for (int e = 0; e < 8; ++e) x[e] = l == 0.f ? 0.f : __uint_as_float(o[i + e]) * inv;
-                            kv_store8(out + c + i, x);
-                        }
+                        for (int e = 0; e < 8; ++e) x[e] = l == 0.f ? 0.f : __uint_as_float(o[i + e]) * inv;
+                        kv_store8(mine + lane * 64 + ((((c + i) >> 3) ^ lane) & 7) * 8, x);
+                    }
+                    if (c & 32) {
+                        __syncwarp();
+                        put_rows(c & ~63);
+                        __syncwarp();
                     }
                 } else {
 #pragma unroll
@@ -600,8 +722,9 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             for (unsigned todo = __ballot_sync(0xFFFFFFFFu, odd && on); todo; todo &= todo - 1) {
                 const int src = __ffs(todo) - 1;
                 const int rtok = __shfl_sync(0xFFFFFFFFu, tok, src), rhh = __shfl_sync(0xFFFFFFFFu, hh, src);
-                float rm, rl, acc[HD / 32];
-                many_row_again<HD, I>(a, it, rtok, rhh, j0, j1, rm, rl, acc);
+                float res[2 + HD / 32];
+                many_row_again<HD, I>(a, it, rtok, rhh, j0, j1, res);
+                const float rm = res[0], rl = res[1], *acc = res + 2;
                 const int rrow = g * 128 + (warp & 3) * 32 + src;
                 I *ro = static_cast<I *>(const_cast<void *>(a.a.o.p)) + (it.q.row0 + rtok) * a.a.o.row +
                         (it.h * a.a.group + rhh) * a.a.o.head;
@@ -649,14 +772,17 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                                 x[i + 3] = fmaf(f, v.w, x[i + 3]);
                             }
                         }
-                        if (on) {
 #pragma unroll
-                            for (int i = 0; i < 32; i += 8) {
-                                float y[8];
+                        for (int i = 0; i < 32; i += 8) {
+                            float y[8];
 #pragma unroll
-                                for (int e = 0; e < 8; ++e) y[e] = L == 0.f ? 0.f : x[i + e] / L;
-                                kv_store8(out + d + i, y);
-                            }
+                            for (int e = 0; e < 8; ++e) y[e] = L == 0.f ? 0.f : x[i + e] / L;
+                            kv_store8(mine + lane * 64 + ((((d + i) >> 3) ^ lane) & 7) * 8, y);
+                        }
+                        if (d & 32) {
+                            __syncwarp();
+                            put_rows(d & ~63);
+                            __syncwarp();
                         }
                     }
                 }
