@@ -673,7 +673,7 @@ static constexpr int kMaxCtas = 512;
 static constexpr size_t kCounterBytes = kMaxCtas * sizeof(unsigned);
 size_t kv_attend_ws()
 {
-    const size_t few = sizeof(float) * 2 * kMaxCtas * few_part(128), many = 2 * kManyCtas * kv_many_part_bytes();
+    const size_t few = sizeof(float) * 2 * kMaxCtas * few_part(128), many = kManyCtas * kv_many_part_bytes();
     return kCounterBytes + (few > many ? few : many);
 }
 

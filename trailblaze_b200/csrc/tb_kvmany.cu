@@ -9,11 +9,11 @@
 // end to end, are cut into equal parts, one per CTA (one CTA per SM): causal
 // triangles, windows and ragged lengths balance by themselves, and a short chunk
 // late in a long context still fills the GPU.  An item cut between CTAs is joined
-// by the last of them to arrive, in CTA order.
+// by the CTA that has its beginning, in CTA order, so results repeat bit for bit.
 //
 // Inside a CTA (384 threads):
 //   warps 0-3, 4-7  softmax of row group 0 / 1, one row a thread;
-//   warp 8          the MMAs, one thread: S_g = Q_g K^T (128 x 128, both
+//   warp 8          the MMAs, one elected thread: S_g = Q_g K^T (128 x 128, both
 //                   operands in shared memory), O_g += P_g V (P_g read from TMEM);
 //   warp 9          K and V tiles by TMA into a ring, page by page;
 //   warp 10         Q tiles by TMA (the next item's while the last one's softmax
@@ -58,7 +58,7 @@ struct ManyCfg {
 };
 
 struct ManyShared {
-    uint64_t sfull[2], pready[2][2], ofull[2], qfull, qempty, done, join, kvfull[8], kvempty[8], vready[8];
+    uint64_t sfull[2], pready[2][2], ofull[2], qfull, qempty, done, join, kvfull[8], kvempty[4], vready[8];
     unsigned long long scan[12], u0;
     uint32_t tmem;
     int seq, head, rt, off, fail, bad, last;
@@ -228,32 +228,23 @@ __device__ __forceinline__ float2 exp2_poly(float2 x)
                        __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
 }
 
-// One row again, over the visible positions of the part's tiles [j0, j1) only, by
-// the whole warp: res = m, l and the sums of dimensions lane * HD / 32 ....
+// One row again, over its visible positions only, by the whole warp: res = the sum
+// of the numerators and the weighted sums of dimensions lane * HD / 32 ....
 template <int HD, class I>
-__device__ __noinline__ void many_row_again(const ManyArgs &a, const ManyItem it, int tok, int hh, int j0, int j1,
-                                            float *res)
+__device__ __noinline__ void many_row_again(const ManyArgs &a, const ManyItem it, int tok, int hh, float *res)
 {
     constexpr int D = HD / 32;
     const int lane = threadIdx.x & 31;
     const I *qp = static_cast<const I *>(a.a.q.p) + (it.q.row0 + tok) * a.a.q.row + (it.h * a.a.group + hh) * a.a.q.head +
                   lane * D;
-    float q[D], am[2], al[2], ac[2][D];
+    float q[D], m, l, acc[D];
 #pragma unroll
     for (int d = 0; d < D; ++d) q[d] = kv_f(qp[d]) * a.a.scale2;
-    const int pos = it.q.len - it.q.n + tok;
-    const int b0 = min(j0, it.ns) * kTileN, b1 = min(j1, it.ns) * kTileN;
-    const int c0 = (max(j0, it.ns) - it.ns + it.lo) * kTileN, c1 = (max(j1, it.ns) - it.ns + it.lo) * kTileN;
-    kv_row_attend<HD, I>(a.a.b, a.a.c, it.s, it.h, pos, b0, min(b1, it.q.len), a.a.window, a.a.sinks, q, am[0], al[0],
-                         ac[0], a.a.err);
-    kv_row_attend<HD, I>(a.a.b, a.a.c, it.s, it.h, pos, c0, min(c1, it.q.len), a.a.window, a.a.sinks, q, am[1], al[1],
-                         ac[1], a.a.err);
-    const float m = fmaxf(am[0], am[1]);
-    const float f0 = am[0] == -INFINITY ? 0.f : ex2(am[0] - m), f1 = am[1] == -INFINITY ? 0.f : ex2(am[1] - m);
-    res[0] = m;
-    res[1] = (am[0] == -INFINITY ? al[0] : al[0] * f0) + (am[1] == -INFINITY ? al[1] : al[1] * f1);
+    kv_row_attend<HD, I>(a.a.b, a.a.c, it.s, it.h, it.q.len - it.q.n + tok, 0, it.q.len, a.a.window, a.a.sinks, q, m, l,
+                         acc, a.a.err);
+    res[0] = l;
 #pragma unroll
-    for (int d = 0; d < D; ++d) res[2 + d] = ac[0][d] * f0 + ac[1][d] * f1;
+    for (int d = 0; d < D; ++d) res[1 + d] = acc[d];
 }
 
 template <int HD, class I>
@@ -270,7 +261,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     uint8_t *stage = sm + 2 * Cfg::QG + NS * Cfg::SLOT;
     ManyShared &sh = *reinterpret_cast<ManyShared *>(stage + 8 * Cfg::STAGE);
     const uint32_t qbase = smem_u32(sm), ring = qbase + 2 * Cfg::QG;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0);
     const uint32_t lim = a.a.wait_limit;
     int *err = a.a.err;
 
@@ -287,7 +278,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         mbar_init(smem_u32(&sh.join), 256);
         for (int i = 0; i < NS; ++i) {
             mbar_init(smem_u32(&sh.kvfull[i]), 1);
-            mbar_init(smem_u32(&sh.kvempty[i]), 1);
+            if (i % 2 == 0) mbar_init(smem_u32(&sh.kvempty[i / 2]), 1);
             mbar_init(smem_u32(&sh.vready[i]), 1);
         }
         fence_mbar_init();
@@ -322,9 +313,12 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         before += w < warp ? sh.scan[w] : 0;
         total += sh.scan[w];
     }
-    const unsigned G = total < gridDim.x ? static_cast<unsigned>(total) : gridDim.x, cta = blockIdx.x;
-    if (cta >= G) return;
-    const unsigned long long u0 = total * cta / G, u1 = total * (cta + 1) / G;
+    const unsigned G = total < gridDim.x ? static_cast<unsigned>(total) : gridDim.x;
+    if (blockIdx.x >= G) return;
+    const unsigned cta = G - 1 - blockIdx.x;   // of the units, against blockIdx: see the joining of parts
+    const unsigned long long per_cta = total / G;
+    const unsigned extra = static_cast<unsigned>(total % G);
+    const unsigned long long u0 = per_cta * cta + extra * cta / G, u1 = per_cta * (cta + 1) + extra * (cta + 1) / G;
     const bool mine_u0 = before <= u0 && u0 < before + mine;
     if (__any_sync(0xFFFFFFFFu, mine_u0)) {   // the warp whose sequences hold u0
         unsigned long long at = before;
@@ -392,18 +386,30 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         if (u < u1) many_next(a, it);
     };
     auto failed = [&]() { return *reinterpret_cast<volatile int *>(&sh.fail) != 0; };
-    auto wait1 = [&](uint64_t *bar, uint32_t parity) {   // by one thread; ends early when another role has given up
-        const uint32_t at = smem_u32(bar);
-        if (mbar_try_wait(at, parity & 1u)) return true;
-        for (uint32_t i = 0; i < lim && !failed(); ++i)
-            if (mbar_try_wait(at, parity & 1u)) return true;
+    // Waits, by a whole warp in step, for one or two barriers; false when the limit runs
+    // out or another role has given up.
+    auto wait2 = [&](uint64_t *b0, uint32_t p0, uint64_t *b1, uint32_t p1) {
+        const uint32_t at0 = smem_u32(b0), at1 = smem_u32(b1);
+        for (uint32_t i = 0; i < lim; ++i) {
+            const bool r0 = mbar_try_wait(at0, p0 & 1u), r1 = mbar_try_wait(at1, p1 & 1u);
+            if (__all_sync(0xFFFFFFFFu, r0 && r1)) return true;
+            if ((i & 15u) == 15u && __any_sync(0xFFFFFFFFu, failed())) break;
+        }
         if (!failed()) atomicExch(err, ERR_WAIT_TIMEOUT);
         *reinterpret_cast<volatile int *>(&sh.fail) = 1;
+        __syncwarp();
         return false;
     };
-    auto wait = [&](uint64_t *bar, uint32_t parity) {   // by a whole warp
-        const bool ok = wait1(bar, parity);
-        return __all_sync(0xFFFFFFFFu, ok) != 0;
+    auto wait = [&](uint64_t *bar, uint32_t parity) {
+        const uint32_t at = smem_u32(bar);
+        for (uint32_t i = 0; i < lim; ++i) {
+            if (__all_sync(0xFFFFFFFFu, mbar_try_wait(at, parity & 1u))) return true;
+            if ((i & 15u) == 15u && __any_sync(0xFFFFFFFFu, failed())) break;
+        }
+        if (!failed()) atomicExch(err, ERR_WAIT_TIMEOUT);
+        *reinterpret_cast<volatile int *>(&sh.fail) = 1;
+        __syncwarp();
+        return false;
     };
 
     uint32_t kv_issued = 0, q_issued = 0;   // in the warps that issue them
@@ -434,7 +440,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                     const int w = a.a.ax_pos == 2 ? pos : a.a.ax_head == 2 ? it.h : page;
                     for (int kv = 0; kv < 2; ++kv) {
                         const uint32_t n = kv_issued, slot = n % NS, bar = smem_u32(&sh.kvfull[slot]);
-                        if (n >= NS) ok = wait(&sh.kvempty[slot], (n / NS) - 1u);
+                        if (n >= NS) ok = wait(&sh.kvempty[((n - NS + 1) / 2) % (NS / 2)], (n - NS + 1) / NS);
                         if (!ok) break;
                         if (lane == 0) mbar_expect_tx(bar, Cfg::SLOT);
                         __syncwarp();
@@ -495,11 +501,13 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                 }
                 next_item(j1);
             }
-        } else if (lane == 0) {
-            // ---- the MMAs, one thread ----
+        } else {
+            // ---- the MMAs: the whole warp in step (its values stay uniform, which the
+            // instruction's operands have to be), one lane issues ----
             const uint32_t fmt = a.bf16 ? 1u : 0u;
             const uint32_t id_s = (1u << 4) | (fmt << 7) | (fmt << 10) | ((kTileN >> 3) << 17) | (8u << 24);
             const uint32_t id_o = (1u << 4) | (fmt << 7) | (fmt << 10) | (1u << 16) | ((HD >> 3) << 17) | (8u << 24);
+            const uint32_t tu = __shfl_sync(0xFFFFFFFFu, tm, 0);
             const uint64_t qd = sw128_desc(qbase), kd = sw128_desc(ring), vd = v_desc(ring);
             uint32_t n = 0, q = 0, np = 0;   // ring slots, items and P tiles taken
             bool ok = true;
@@ -508,51 +516,61 @@ __global__ void __launch_bounds__(kManyThreads, 1)
 #pragma unroll
                 for (int ks = 0; ks < HD / 16; ++ks) {
                     const uint32_t off = ((ks >> 2) * (128 * 128) + (ks & 3) * 32) >> 4;
-                    umma_f16(tm + g * 128, qg + off, kg + off, id_s, ks > 0);
+                    umma_f16(tu + g * 128, qg + off, kg + off, id_s, ks > 0);
                 }
                 umma_commit(smem_u32(&sh.sfull[g]));
             };
+            // K in ring place n and the V before it are done with once the products issued
+            // so far are: one commit for both, after what the softmax waits for
+            auto free_pair = [&](uint32_t n) { umma_commit(smem_u32(&sh.kvempty[((n + 1) / 2) % (NS / 2)])); };
             while (ok && u < u1) {
                 const int j1 = part_end();
-                ok = wait1(&sh.qfull, q) && wait1(&sh.kvfull[n % NS], n / NS);
+                ok = wait(&sh.qfull, q) && wait(&sh.kvfull[n % NS], n / NS);
                 if (!ok) break;
                 tc_fence_after();
-                issue_s(0, n % NS);
-                issue_s(1, n % NS);
-                umma_commit(smem_u32(&sh.kvempty[n % NS]));
-                if (j1 - j0 == 1) umma_commit(smem_u32(&sh.qempty));
+                if (elect_one()) {
+                    issue_s(0, n % NS);
+                    issue_s(1, n % NS);
+                    free_pair(n);
+                    if (j1 - j0 == 1) umma_commit(smem_u32(&sh.qempty));
+                }
+                __syncwarp();
                 ++n;
-                for (int j = j0; j < j1; ++j) {
+                for (int j = j0; ok && j < j1; ++j) {
                     const uint32_t vs = n % NS, vpar = n / NS, kn = (n + 1) % NS, kpar = (n + 1) / NS;
                     const bool more = j + 1 < j1;
                     const uint64_t vg = vd + ((vs * Cfg::SLOT) >> 4);
-                    ok = wait1(&sh.vready[vs], vpar);
-                    for (int g = 0; ok && g < 2; ++g) {
-                        ok = wait1(&sh.pready[g][0], np);
+#pragma unroll
+                    for (int g = 0; g < 2; ++g) {
+                        const uint32_t od = tu + 256 + g * HD, pa = tu + g * 128;
+                        ok = g == 0 ? wait2(&sh.vready[vs], vpar, &sh.pready[0][0], np) : wait(&sh.pready[1][0], np);
                         if (!ok) break;
                         tc_fence_after();
+                        if (elect_one()) {
 #pragma unroll
-                        for (int ks = 0; ks < kTileN / 32; ++ks)
-                            umma_f16_ts(tm + 256 + g * HD, tm + g * 128 + ks * 8, vg + ks * (2048 >> 4), id_o,
-                                        (j > j0 || ks > 0) ? 1u : 0u);
-                        ok = (g == 1 || !more || wait1(&sh.kvfull[kn], kpar)) && wait1(&sh.pready[g][1], np);
-                        if (!ok) break;
-                        tc_fence_after();
-#pragma unroll
-                        for (int ks = kTileN / 32; ks < kTileN / 16; ++ks)
-                            umma_f16_ts(tm + 256 + g * HD, tm + g * 128 + ks * 8, vg + ks * (2048 >> 4), id_o, 1u);
-                        if (g == 1) umma_commit(smem_u32(&sh.kvempty[vs]));
-                        if (more) {
-                            issue_s(g, kn);
-                            if (g == 1) {
-                                umma_commit(smem_u32(&sh.kvempty[kn]));
-                                if (j + 2 == j1) umma_commit(smem_u32(&sh.qempty));
-                            }
-                        } else {
-                            umma_commit(smem_u32(&sh.ofull[g]));
+                            for (int ks = 0; ks < kTileN / 32; ++ks)
+                                umma_f16_ts(od, pa + ks * 8, vg + ks * (2048 >> 4), id_o, (j > j0 || ks > 0) ? 1u : 0u);
                         }
+                        __syncwarp();
+                        ok = g == 0 && more ? wait2(&sh.kvfull[kn], kpar, &sh.pready[0][1], np) : wait(&sh.pready[g][1], np);
+                        if (!ok) break;
+                        tc_fence_after();
+                        if (elect_one()) {
+#pragma unroll
+                            for (int ks = kTileN / 32; ks < kTileN / 16; ++ks)
+                                umma_f16_ts(od, pa + ks * 8, vg + ks * (2048 >> 4), id_o, 1u);
+                            if (more) {
+                                issue_s(g, kn);
+                                if (g == 1) {
+                                    free_pair(n + 1);
+                                    if (j + 2 == j1) umma_commit(smem_u32(&sh.qempty));
+                                }
+                            } else {
+                                umma_commit(smem_u32(&sh.ofull[g]));
+                            }
+                        }
+                        __syncwarp();
                     }
-                    if (!ok) break;
                     ++np;
                     n += more ? 2 : 1;
                 }
@@ -560,7 +578,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                 next_item(j1);
             }
             // every MMA issued is complete before TMEM is given back
-            umma_commit(smem_u32(&sh.done));
+            if (elect_one()) umma_commit(smem_u32(&sh.done));
+            __syncwarp();
             mbar_wait_bounded(smem_u32(&sh.done), 0, err, lim);
         }
     } else {
@@ -670,123 +689,120 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             if (!ok || !wait(&sh.ofull[g], items)) break;
             ++items;
             tc_fence_after();
-            // ---- the part's result: out, or the workspace ----
-            const bool whole = j0 == 0 && j1 == it.n;
-            float *part = a.a.part + static_cast<size_t>(2 * cta + (j0 == 0 ? 1 : 0)) * Cfg::PART;
             const int row = g * 128 + lr;
-            I *out = static_cast<I *>(const_cast<void *>(a.a.o.p)) + (it.q.row0 + (on ? tok : 0)) * a.a.o.row +
-                     (it.h * a.a.group + hh) * a.a.o.head;
-            I *mine = reinterpret_cast<I *>(stage + warp * Cfg::STAGE);   // [32 rows][64], 16-byte pieces swizzled
-            const long long off = on ? out - static_cast<I *>(const_cast<void *>(a.a.o.p)) : -1;
-            auto put_rows = [&](int d) {   // dimensions [d, d + 64) of the warp's rows
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int r = i * 4 + (lane >> 3), k = lane & 7;
-                    const long long ro = __shfl_sync(0xFFFFFFFFu, off, r);
-                    const uint4 v = *reinterpret_cast<const uint4 *>(mine + r * 64 + ((k ^ r) & 7) * 8);
-                    if (ro >= 0) *reinterpret_cast<uint4 *>(static_cast<I *>(const_cast<void *>(a.a.o.p)) + ro + d + k * 8) = v;
-                }
-            };
-            bool odd = !isfinite(l) || m == INFINITY || *reinterpret_cast<volatile int *>(&sh.bad);
-            const float inv = l == 0.f ? 0.f : 1.0f / l;
+            if (j0 > 0) {
+                // ---- not the item's beginning: the part goes to the CTA that has it ----
+                float *part = a.a.part + static_cast<size_t>(cta) * Cfg::PART + row * 4;
 #pragma unroll 1
-            for (int c = 0; c < HD; c += 32) {
-                uint32_t o[32];
-                tmem_ld32(to + c, o);
-                tmem_wait_ld(o);
-#pragma unroll
-                for (int i = 0; i < 32; ++i) odd = odd || !isfinite(__uint_as_float(o[i]));
-                if (whole) {
-                    // 64 dimensions of the warp's rows through shared memory, so that 8 lanes write 128 bytes
-#pragma unroll
-                    for (int i = 0; i < 32; i += 8) {
-                        float x[8];
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) x[e] = l == 0.f ? 0.f : __uint_as_float(o[i + e]) * inv;
-                        kv_store8(mine + lane * 64 + ((((c + i) >> 3) ^ lane) & 7) * 8, x);
-                    }
-                    if (c & 32) {
-                        __syncwarp();
-                        put_rows(c & ~63);
-                        __syncwarp();
-                    }
-                } else {
+                for (int c = 0; c < HD; c += 32) {
+                    uint32_t o[32];
+                    tmem_ld32(to + c, o);
+                    tmem_wait_ld(o);
 #pragma unroll
                     for (int i = 0; i < 32; i += 4)
-                        reinterpret_cast<uint4 *>(part)[((c + i) / 4) * 256 + row] = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                        __stcg(reinterpret_cast<uint4 *>(part) + ((c + i) / 4) * 256, make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]));
                 }
-            }
-            if (!whole) part[256 * HD + row] = m, part[256 * HD + 256 + row] = l;
-            // rows that are not finite: V of a position that this row does not see may have been
-            // (0 * NaN), or a page lies outside the pool.  Once more, over their own positions only.
-            for (unsigned todo = __ballot_sync(0xFFFFFFFFu, odd && on); todo; todo &= todo - 1) {
-                const int src = __ffs(todo) - 1;
-                const int rtok = __shfl_sync(0xFFFFFFFFu, tok, src), rhh = __shfl_sync(0xFFFFFFFFu, hh, src);
-                float res[2 + HD / 32];
-                many_row_again<HD, I>(a, it, rtok, rhh, j0, j1, res);
-                const float rm = res[0], rl = res[1], *acc = res + 2;
-                const int rrow = g * 128 + (warp & 3) * 32 + src;
-                I *ro = static_cast<I *>(const_cast<void *>(a.a.o.p)) + (it.q.row0 + rtok) * a.a.o.row +
-                        (it.h * a.a.group + rhh) * a.a.o.head;
-                for (int d = 0; d < HD / 32; ++d) {
-                    const int dim = lane * (HD / 32) + d;
-                    if (whole) kv_store1(ro + dim, rl == 0.f ? 0.f : acc[d] / rl);
-                    else part[((dim / 4) * 256 + rrow) * 4 + (dim & 3)] = acc[d];
-                }
-                if (!whole && lane == 0) part[256 * HD + rrow] = rm, part[256 * HD + 256 + rrow] = rl;
-                __syncwarp();
-            }
-            if (!whole) {
-                // ---- the last CTA of the item to arrive adds the parts, in CTA order ----
-                const unsigned long long i0 = u - j0, i1 = i0 + it.n;
-                const unsigned c0 = static_cast<unsigned>(((i0 + 1) * G - 1) / total);
-                const unsigned c1 = static_cast<unsigned>((i1 * G - 1) / total);
+                part += 256 * HD - row * 3;
+                __stcg(part, m);
+                __stcg(part + 256, *reinterpret_cast<volatile int *>(&sh.bad) ? NAN : l);
                 __threadfence();
                 if (!join()) break;
-                if (tid == 0) sh.last = atomicInc(a.a.arrived + c0, c1 - c0) == c1 - c0;   // wraps back to zero
-                if (!join()) break;
-                if (sh.last) {
-                    __threadfence();
-                    float M = -INFINITY, L = 0.f;
-                    for (unsigned c = c0; c <= c1; ++c)
-                        M = fmaxf(M, __ldcg(a.a.part + static_cast<size_t>(2 * c + (c == c0 ? 1 : 0)) * Cfg::PART + 256 * HD + row));
-                    for (unsigned c = c0; c <= c1; ++c) {
-                        const float *pp = a.a.part + static_cast<size_t>(2 * c + (c == c0 ? 1 : 0)) * Cfg::PART + 256 * HD + row;
+                if (tid == 0) atomicAdd(a.a.arrived + static_cast<unsigned>(((u - j0 + 1) * G - 1) / total), 1u);
+            } else {
+                // ---- the beginning: the other parts, of the CTAs after this one, are added in
+                // order.  They are waited for (as every wait, within a limit): the ranges run
+                // against blockIdx, so those CTAs were started before this one. ----
+                const unsigned others = static_cast<unsigned>(((u + it.n) * G - 1) / total) - cta;
+                const float *part = a.a.part + static_cast<size_t>(cta + 1) * Cfg::PART;
+                float M = m, L = l;
+                if (others > 0) {
+                    if (tid == 0) {
+                        uint32_t i = 0;
+                        unsigned n = 0;
+                        do {
+                            asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(n) : "l"(a.a.arrived + cta) : "memory");
+                        } while (n < others && ++i < lim && !failed());
+                        if (n < others) {
+                            if (!failed()) atomicExch(err, ERR_WAIT_TIMEOUT);
+                            *reinterpret_cast<volatile int *>(&sh.fail) = 1;
+                        }
+                        a.a.arrived[cta] = 0;   // zero between calls
+                        __threadfence();
+                    }
+                    if (!join()) break;
+                    for (unsigned c = 0; c < others; ++c) M = fmaxf(M, __ldcg(part + c * Cfg::PART + 256 * HD + row));
+                    const float f = m == -INFINITY ? 0.f : ex2(m - M);
+                    L = m == -INFINITY ? l : f * l;
+                    for (unsigned c = 0; c < others; ++c) {
+                        const float *pp = part + c * Cfg::PART + 256 * HD + row;
                         const float pm = __ldcg(pp), pl = __ldcg(pp + 256);
                         L += pm == -INFINITY ? pl : ex2(pm - M) * pl;
                     }
+                }
+                I *out = static_cast<I *>(const_cast<void *>(a.a.o.p));
+                const long long off = on ? (it.q.row0 + tok) * a.a.o.row + (it.h * a.a.group + hh) * a.a.o.head : -1;
+                I *mine = reinterpret_cast<I *>(stage + warp * Cfg::STAGE);   // [32 rows][64], 16-byte pieces swizzled
+                bool odd = !isfinite(L) || M == INFINITY || *reinterpret_cast<volatile int *>(&sh.bad);
+                const float inv = L == 0.f ? 0.f : 1.0f / L, f = m == -INFINITY ? 0.f : ex2(m - M) * inv;
 #pragma unroll 1
-                    for (int d = 0; d < HD; d += 32) {
-                        float x[32];
+                for (int c = 0; c < HD; c += 64) {
+                    uint32_t o[64];
+                    tmem_ld32(to + c, o);
+                    tmem_ld32(to + c + 32, o + 32);
+                    tmem_wait_ld(o);
+                    after_wait(o + 32);
+                    float *x = reinterpret_cast<float *>(o);
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) x[i] = 0.f;
-                        for (unsigned c = c0; c <= c1; ++c) {
-                            const float *pp = a.a.part + static_cast<size_t>(2 * c + (c == c0 ? 1 : 0)) * Cfg::PART;
-                            const float pm = __ldcg(pp + 256 * HD + row), f = pm == -INFINITY ? 0.f : ex2(pm - M);
+                    for (int i = 0; i < 64; ++i) x[i] *= f;
+                    for (unsigned k = 0; k < others; ++k) {
+                        const float *pp = part + k * Cfg::PART + row * 4;
+                        const float pm = __ldcg(part + k * Cfg::PART + 256 * HD + row);
+                        const float pf = pm == -INFINITY ? 0.f : ex2(pm - M) * inv;
+                        float4 v[16];
 #pragma unroll
-                            for (int i = 0; i < 32; i += 4) {
-                                const float4 v = __ldcg(reinterpret_cast<const float4 *>(pp) + ((d + i) / 4) * 256 + row);
-                                x[i] = fmaf(f, v.x, x[i]);
-                                x[i + 1] = fmaf(f, v.y, x[i + 1]);
-                                x[i + 2] = fmaf(f, v.z, x[i + 2]);
-                                x[i + 3] = fmaf(f, v.w, x[i + 3]);
-                            }
-                        }
+                        for (int i = 0; i < 16; ++i) v[i] = __ldcg(reinterpret_cast<const float4 *>(pp) + (c / 4 + i) * 256);
 #pragma unroll
-                        for (int i = 0; i < 32; i += 8) {
-                            float y[8];
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) y[e] = L == 0.f ? 0.f : x[i + e] / L;
-                            kv_store8(mine + lane * 64 + ((((d + i) >> 3) ^ lane) & 7) * 8, y);
-                        }
-                        if (d & 32) {
-                            __syncwarp();
-                            put_rows(d & ~63);
-                            __syncwarp();
+                        for (int i = 0; i < 16; ++i) {
+                            x[4 * i] = fmaf(pf, v[i].x, x[4 * i]);
+                            x[4 * i + 1] = fmaf(pf, v[i].y, x[4 * i + 1]);
+                            x[4 * i + 2] = fmaf(pf, v[i].z, x[4 * i + 2]);
+                            x[4 * i + 3] = fmaf(pf, v[i].w, x[4 * i + 3]);
                         }
                     }
+                    float2 nil = make_float2(0.f, 0.f);   // stays zero where everything is finite
+#pragma unroll
+                    for (int i = 0; i < 64; i += 2) nil = __ffma2_rn(make_float2(x[i], x[i + 1]), make_float2(0.f, 0.f), nil);
+                    odd = odd | !(nil.x + nil.y == 0.f);
+                    // through shared memory, so that 8 lanes write 128 bytes of a row
+#pragma unroll
+                    for (int i = 0; i < 64; i += 8) {
+                        float y[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) y[e] = x[i + e];
+                        kv_store8(mine + lane * 64 + (((i >> 3) ^ lane) & 7) * 8, y);
+                    }
+                    __syncwarp();
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int r = i * 4 + (lane >> 3), k = lane & 7;
+                        const long long ro = __shfl_sync(0xFFFFFFFFu, off, r);
+                        const uint4 v = *reinterpret_cast<const uint4 *>(mine + r * 64 + ((k ^ r) & 7) * 8);
+                        if (ro >= 0) *reinterpret_cast<uint4 *>(out + ro + c + k * 8) = v;
+                    }
+                    __syncwarp();
                 }
-                if (!join()) break;   // sh.last is free again
+                // rows that are not finite: V of a position that a row does not see may have been
+                // (0 * NaN), or a page lies outside the pool.  Once more, over their own positions only.
+                for (unsigned todo = __ballot_sync(0xFFFFFFFFu, odd && on); todo; todo &= todo - 1) {
+                    const int src = __ffs(todo) - 1;
+                    const int rtok = __shfl_sync(0xFFFFFFFFu, tok, src), rhh = __shfl_sync(0xFFFFFFFFu, hh, src);
+                    const long long ro = __shfl_sync(0xFFFFFFFFu, off, src);
+                    float res[1 + HD / 32];
+                    many_row_again<HD, I>(a, it, rtok, rhh, res);
+                    for (int d = 0; d < HD / 32; ++d)
+                        kv_store1(out + ro + lane * (HD / 32) + d, res[0] == 0.f ? 0.f : res[1 + d] / res[0]);
+                    __syncwarp();
+                }
             }
             next_item(j1);
         }
