@@ -57,7 +57,17 @@ struct ManyCfg {
     static constexpr int PART = 256 * HD + 512;          // floats of a partial result: O, m, l
 };
 
+// What the MMA and softmax warps need of an item (this CTA's part of it), written
+// by the Q warp with the item's Q.
+struct alignas(16) ManyPart {
+    int row0, len, n, t0;   // the sequence's first row, length and new tokens; the item's first token,
+    int t1, s, h, tiles;    // its end; sequence, kv head; the item's position tiles,
+    int ns, lo, j0, j1;     // where they lie, and this CTA's [j0, j1) of them
+    unsigned peer, pad[3];  // j0 > 0: the CTA that joins the parts; else how many others there are
+};
+
 struct ManyShared {
+    ManyPart part[4];
     uint64_t sfull[2], pready[2][2], ofull[2], qfull, qempty, done, join, kvfull[8], kvempty[4], vready[8];
     unsigned long long scan[12], u0;
     uint32_t tmem;
@@ -231,16 +241,16 @@ __device__ __forceinline__ float2 exp2_poly(float2 x)
 // One row again, over its visible positions only, by the whole warp: res = the sum
 // of the numerators and the weighted sums of dimensions lane * HD / 32 ....
 template <int HD, class I>
-__device__ __noinline__ void many_row_again(const ManyArgs &a, const ManyItem it, int tok, int hh, float *res)
+__device__ __noinline__ void many_row_again(const ManyArgs &a, const ManyPart it, int tok, int hh, float *res)
 {
     constexpr int D = HD / 32;
     const int lane = threadIdx.x & 31;
-    const I *qp = static_cast<const I *>(a.a.q.p) + (it.q.row0 + tok) * a.a.q.row + (it.h * a.a.group + hh) * a.a.q.head +
+    const I *qp = static_cast<const I *>(a.a.q.p) + (it.row0 + tok) * a.a.q.row + (it.h * a.a.group + hh) * a.a.q.head +
                   lane * D;
     float q[D], m, l, acc[D];
 #pragma unroll
     for (int d = 0; d < D; ++d) q[d] = kv_f(qp[d]) * a.a.scale2;
-    kv_row_attend<HD, I>(a.a.b, a.a.c, it.s, it.h, it.q.len - it.q.n + tok, 0, it.q.len, a.a.window, a.a.sinks, q, m, l,
+    kv_row_attend<HD, I>(a.a.b, a.a.c, it.s, it.h, it.len - it.n + tok, 0, it.len, a.a.window, a.a.sinks, q, m, l,
                          acc, a.a.err);
     res[0] = l;
 #pragma unroll
@@ -463,6 +473,17 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                 const int j1 = part_end();
                 if (q_issued > 0) ok = wait(&sh.qempty, q_issued - 1u);
                 if (!ok) break;
+                // place q_issued % 4 is free: that item's softmax was over before the product
+                // that qempty has just reported could be issued
+                if (elect_one()) {
+                    ManyPart &pt = sh.part[q_issued % 4];
+                    pt.row0 = it.q.row0, pt.len = it.q.len, pt.n = it.q.n, pt.t0 = it.t0;
+                    pt.t1 = it.t1, pt.s = it.s, pt.h = it.h, pt.tiles = it.n;
+                    pt.ns = it.ns, pt.lo = it.lo, pt.j0 = j0, pt.j1 = j1;
+                    pt.peer = j0 > 0 ? static_cast<unsigned>(((u - j0 + 1) * G - 1) / total)
+                                     : static_cast<unsigned>(((u + it.n) * G - 1) / total) - cta;
+                }
+                __syncwarp();
                 if (elect_one()) {
                     const uint32_t bar = smem_u32(&sh.qfull);
                     mbar_expect_tx(bar, 2u * CB * 128u * a.tpt * a.a.group);
@@ -509,6 +530,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             const uint32_t id_o = (1u << 4) | (fmt << 7) | (fmt << 10) | (1u << 16) | ((HD >> 3) << 17) | (8u << 24);
             const uint32_t tu = __shfl_sync(0xFFFFFFFFu, tm, 0);
             const uint64_t qd = sw128_desc(qbase), kd = sw128_desc(ring), vd = v_desc(ring);
+            const uint32_t n_tiles = static_cast<uint32_t>(u1 - u0);
             uint32_t n = 0, q = 0, np = 0;   // ring slots, items and P tiles taken
             bool ok = true;
             auto issue_s = [&](int g, uint32_t slot) {
@@ -523,59 +545,69 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             // K in ring place n and the V before it are done with once the products issued
             // so far are: one commit for both, after what the softmax waits for
             auto free_pair = [&](uint32_t n) { umma_commit(smem_u32(&sh.kvempty[((n + 1) / 2) % (NS / 2)])); };
-            while (ok && u < u1) {
-                const int j1 = part_end();
-                ok = wait(&sh.qfull, q) && wait(&sh.kvfull[n % NS], n / NS);
-                if (!ok) break;
+            // One loop over all tiles: the next item's first S follows the last P V of the one
+            // before it like any other.
+            ok = wait(&sh.qfull, 0) && wait(&sh.kvfull[0], 0);
+            int left = sh.part[0].j1 - sh.part[0].j0;   // of the item's tiles, this one included
+            if (ok) {
                 tc_fence_after();
                 if (elect_one()) {
-                    issue_s(0, n % NS);
-                    issue_s(1, n % NS);
-                    free_pair(n);
-                    if (j1 - j0 == 1) umma_commit(smem_u32(&sh.qempty));
+                    issue_s(0, 0);
+                    issue_s(1, 0);
+                    free_pair(0);
+                    if (left == 1) umma_commit(smem_u32(&sh.qempty));
                 }
                 __syncwarp();
-                ++n;
-                for (int j = j0; ok && j < j1; ++j) {
-                    const uint32_t vs = n % NS, vpar = n / NS, kn = (n + 1) % NS, kpar = (n + 1) / NS;
-                    const bool more = j + 1 < j1;
-                    const uint64_t vg = vd + ((vs * Cfg::SLOT) >> 4);
+            }
+            bool fresh = true;   // the item's first tile
+            n = 1;
+            for (; ok && np < n_tiles; ++np, n += 2) {
+                const uint32_t vs = n % NS, vpar = n / NS, kn = (n + 1) % NS, kpar = (n + 1) / NS;
+                const bool more = np + 1 < n_tiles, last = left == 1;
+                const uint64_t vg = vd + ((vs * Cfg::SLOT) >> 4);
 #pragma unroll
-                    for (int g = 0; g < 2; ++g) {
-                        const uint32_t od = tu + 256 + g * HD, pa = tu + g * 128;
-                        ok = g == 0 ? wait2(&sh.vready[vs], vpar, &sh.pready[0][0], np) : wait(&sh.pready[1][0], np);
-                        if (!ok) break;
-                        tc_fence_after();
-                        if (elect_one()) {
+                for (int g = 0; g < 2; ++g) {
+                    const uint32_t od = tu + 256 + g * HD, pa = tu + g * 128;
+                    ok = g == 0 ? wait2(&sh.vready[vs], vpar, &sh.pready[0][0], np) : wait(&sh.pready[1][0], np);
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (elect_one()) {
 #pragma unroll
-                            for (int ks = 0; ks < kTileN / 32; ++ks)
-                                umma_f16_ts(od, pa + ks * 8, vg + ks * (2048 >> 4), id_o, (j > j0 || ks > 0) ? 1u : 0u);
-                        }
-                        __syncwarp();
-                        ok = g == 0 && more ? wait2(&sh.kvfull[kn], kpar, &sh.pready[0][1], np) : wait(&sh.pready[g][1], np);
-                        if (!ok) break;
-                        tc_fence_after();
-                        if (elect_one()) {
-#pragma unroll
-                            for (int ks = kTileN / 32; ks < kTileN / 16; ++ks)
-                                umma_f16_ts(od, pa + ks * 8, vg + ks * (2048 >> 4), id_o, 1u);
-                            if (more) {
-                                issue_s(g, kn);
-                                if (g == 1) {
-                                    free_pair(n + 1);
-                                    if (j + 2 == j1) umma_commit(smem_u32(&sh.qempty));
-                                }
-                            } else {
-                                umma_commit(smem_u32(&sh.ofull[g]));
-                            }
-                        }
-                        __syncwarp();
+                        for (int ks = 0; ks < kTileN / 32; ++ks)
+                            umma_f16_ts(od, pa + ks * 8, vg + ks * (2048 >> 4), id_o, (!fresh || ks > 0) ? 1u : 0u);
                     }
-                    ++np;
-                    n += more ? 2 : 1;
+                    __syncwarp();
+                    ok = wait(&sh.pready[g][1], np);
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (elect_one()) {
+#pragma unroll
+                        for (int ks = kTileN / 32; ks < kTileN / 16; ++ks)
+                            umma_f16_ts(od, pa + ks * 8, vg + ks * (2048 >> 4), id_o, 1u);
+                        if (last) umma_commit(smem_u32(&sh.ofull[g]));
+                    }
+                    __syncwarp();
+                    if (!more) continue;
+                    if (g == 0) {
+                        ok = wait(&sh.kvfull[kn], kpar);
+                        if (ok && last) {   // the next item
+                            ok = wait(&sh.qfull, ++q);
+                            left = sh.part[q % 4].j1 - sh.part[q % 4].j0 + 1;
+                        }
+                        if (!ok) break;
+                        tc_fence_after();
+                    }
+                    if (elect_one()) {
+                        issue_s(g, kn);
+                        if (g == 1) {
+                            free_pair(n + 1);
+                            if (left == 2) umma_commit(smem_u32(&sh.qempty));   // that was the item's last S
+                        }
+                    }
+                    __syncwarp();
                 }
-                ++q;
-                next_item(j1);
+                fresh = last;
+                --left;
             }
             // every MMA issued is complete before TMEM is given back
             if (elect_one()) umma_commit(smem_u32(&sh.done));
@@ -591,22 +623,36 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         const int tok_in = lr / a.a.group, hh = lr - tok_in * a.a.group;
         const float sc = a.a.scale2;
         uint32_t cnt = 0, items = 0, joins = 0;
+        int tell = -1;   // the CTA that waits for this one's part
+        auto told = [&]() {   // each softmax warp for its rows
+            __syncwarp();
+            if (lane == 0) {
+                __threadfence();
+                atomicAdd(a.a.arrived + tell, 1u);
+            }
+            __syncwarp();
+            tell = -1;
+        };
         bool ok = true;
         auto join = [&]() {   // of the 256 softmax threads; bounded like every wait
             mbar_arrive(smem_u32(&sh.join));
             ok = wait(&sh.join, joins++);
             return ok;
         };
-        while (ok && u < u1) {
-            const int j1 = part_end();
+        const uint32_t n_tiles = static_cast<uint32_t>(u1 - u0);
+        while (ok && cnt < n_tiles) {
+            ok = wait(&sh.sfull[g], cnt);   // of the item's first tile: its description is there too
+            if (!ok) break;
+            const ManyPart it = sh.part[items % 4];
+            const int j0 = it.j0, j1 = it.j1;
             const int tok = it.t0 + g * a.tpt + tok_in;
             const bool on = tok_in < a.tpt && tok < it.t1;
-            const int p0 = it.q.len - it.q.n, pos = on ? p0 + tok : -1;
+            const int p0 = it.len - it.n, pos = on ? p0 + tok : -1;
             // the group's first and last position
             const int pmin = p0 + it.t0 + g * a.tpt, pmax = p0 + min(it.t1, it.t0 + (g + 1) * a.tpt) - 1;
             float m = -INFINITY, l = 0.f;
             for (int j = j0; j < j1; ++j) {
-                ok = wait(&sh.sfull[g], cnt);
+                if (j > j0) ok = wait(&sh.sfull[g], cnt);
                 if (!ok) break;
                 ++cnt;
                 tc_fence_after();
@@ -619,7 +665,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                 after_wait(s + 32);
                 after_wait(s + 64);
                 after_wait(s + 96);
-                const int k0 = many_tile_pos(it, j);
+                const int k0 = (j < it.ns ? j : j - it.ns + it.lo) * kTileN;
                 if (k0 + kTileN - 1 > pmin) {
                     const int last = pos - k0;   // the last column that the row sees
 #pragma unroll
@@ -685,6 +731,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                     mbar_arrive(smem_u32(&sh.pready[g][h]));
                 }
                 l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+                if (tell >= 0) told();
             }
             if (!ok || !wait(&sh.ofull[g], items)) break;
             ++items;
@@ -705,24 +752,25 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                 part += 256 * HD - row * 3;
                 __stcg(part, m);
                 __stcg(part + 256, *reinterpret_cast<volatile int *>(&sh.bad) ? NAN : l);
-                __threadfence();
-                if (!join()) break;
-                if (tid == 0) atomicAdd(a.a.arrived + static_cast<unsigned>(((u - j0 + 1) * G - 1) / total), 1u);
+                // the stores are under way; that they have arrived is told later
+                tell = static_cast<int>(it.peer);
             } else {
                 // ---- the beginning: the other parts, of the CTAs after this one, are added in
                 // order.  They are waited for (as every wait, within a limit): the ranges run
                 // against blockIdx, so those CTAs were started before this one. ----
-                const unsigned others = static_cast<unsigned>(((u + it.n) * G - 1) / total) - cta;
+                const unsigned others = it.peer;
                 const float *part = a.a.part + static_cast<size_t>(cta + 1) * Cfg::PART;
                 float M = m, L = l;
+                bool odd = *reinterpret_cast<volatile int *>(&sh.bad);
                 if (others > 0) {
+                    // 8 softmax warps of each of the others
                     if (tid == 0) {
                         uint32_t i = 0;
                         unsigned n = 0;
                         do {
                             asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(n) : "l"(a.a.arrived + cta) : "memory");
-                        } while (n < others && ++i < lim && !failed());
-                        if (n < others) {
+                        } while (n < 8 * others && ++i < lim && !failed());
+                        if (n < 8 * others) {
                             if (!failed()) atomicExch(err, ERR_WAIT_TIMEOUT);
                             *reinterpret_cast<volatile int *>(&sh.fail) = 1;
                         }
@@ -738,58 +786,73 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                         const float pm = __ldcg(pp), pl = __ldcg(pp + 256);
                         L += pm == -INFINITY ? pl : ex2(pm - M) * pl;
                     }
+                    // O in TMEM becomes the item's sum
+#pragma unroll 1
+                    for (int c = 0; c < HD; c += 64) {
+                        uint32_t o[64];
+                        float *x = reinterpret_cast<float *>(o);
+                        tmem_ld32(to + c, o);
+                        tmem_ld32(to + c + 32, o + 32);
+                        tmem_wait_ld(o);
+                        after_wait(o + 32);
+#pragma unroll
+                        for (int i = 0; i < 64; ++i) x[i] *= f;
+#pragma unroll 1
+                        for (unsigned k = 0; k < others; ++k) {
+                            const float *pp = part + k * Cfg::PART + row * 4;
+                            float4 v[16];
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) v[i] = __ldcg(reinterpret_cast<const float4 *>(pp) + (c / 4 + i) * 256);
+                            const float pm = __ldcg(part + k * Cfg::PART + 256 * HD + row);
+                            const float pf = pm == -INFINITY ? 0.f : ex2(pm - M);
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) {
+                                x[4 * i] = fmaf(pf, v[i].x, x[4 * i]);
+                                x[4 * i + 1] = fmaf(pf, v[i].y, x[4 * i + 1]);
+                                x[4 * i + 2] = fmaf(pf, v[i].z, x[4 * i + 2]);
+                                x[4 * i + 3] = fmaf(pf, v[i].w, x[4 * i + 3]);
+                            }
+                        }
+                        tmem_st32(to + c, o);
+                        tmem_st32(to + c + 32, o + 32);
+                    }
+                    tmem_wait_st();
                 }
                 I *out = static_cast<I *>(const_cast<void *>(a.a.o.p));
-                const long long off = on ? (it.q.row0 + tok) * a.a.o.row + (it.h * a.a.group + hh) * a.a.o.head : -1;
+                const long long off = on ? (it.row0 + tok) * a.a.o.row + (it.h * a.a.group + hh) * a.a.o.head : -1;
                 I *mine = reinterpret_cast<I *>(stage + warp * Cfg::STAGE);   // [32 rows][64], 16-byte pieces swizzled
-                bool odd = !isfinite(L) || M == INFINITY || *reinterpret_cast<volatile int *>(&sh.bad);
-                const float inv = L == 0.f ? 0.f : 1.0f / L, f = m == -INFINITY ? 0.f : ex2(m - M) * inv;
+                odd = odd | !isfinite(L) | (M == INFINITY);
+                const float inv = L == 0.f ? 0.f : 1.0f / L;
+                // Rolled, since this code comes by once an item: unrolled, it would come from
+                // beyond the instruction cache every time.
 #pragma unroll 1
-                for (int c = 0; c < HD; c += 64) {
-                    uint32_t o[64];
-                    tmem_ld32(to + c, o);
-                    tmem_ld32(to + c + 32, o + 32);
-                    tmem_wait_ld(o);
-                    after_wait(o + 32);
+                for (int c = 0; c < HD; c += 32) {
+                    uint32_t o[32];
                     float *x = reinterpret_cast<float *>(o);
-#pragma unroll
-                    for (int i = 0; i < 64; ++i) x[i] *= f;
-                    for (unsigned k = 0; k < others; ++k) {
-                        const float *pp = part + k * Cfg::PART + row * 4;
-                        const float pm = __ldcg(part + k * Cfg::PART + 256 * HD + row);
-                        const float pf = pm == -INFINITY ? 0.f : ex2(pm - M) * inv;
-                        float4 v[16];
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) v[i] = __ldcg(reinterpret_cast<const float4 *>(pp) + (c / 4 + i) * 256);
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            x[4 * i] = fmaf(pf, v[i].x, x[4 * i]);
-                            x[4 * i + 1] = fmaf(pf, v[i].y, x[4 * i + 1]);
-                            x[4 * i + 2] = fmaf(pf, v[i].z, x[4 * i + 2]);
-                            x[4 * i + 3] = fmaf(pf, v[i].w, x[4 * i + 3]);
-                        }
-                    }
+                    tmem_ld32(to + c, o);
+                    tmem_wait_ld(o);
                     float2 nil = make_float2(0.f, 0.f);   // stays zero where everything is finite
 #pragma unroll
-                    for (int i = 0; i < 64; i += 2) nil = __ffma2_rn(make_float2(x[i], x[i + 1]), make_float2(0.f, 0.f), nil);
+                    for (int i = 0; i < 32; i += 2) nil = __ffma2_rn(make_float2(x[i], x[i + 1]), make_float2(0.f, 0.f), nil);
                     odd = odd | !(nil.x + nil.y == 0.f);
-                    // through shared memory, so that 8 lanes write 128 bytes of a row
 #pragma unroll
-                    for (int i = 0; i < 64; i += 8) {
+                    for (int i = 0; i < 32; i += 8) {
                         float y[8];
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) y[e] = x[i + e];
-                        kv_store8(mine + lane * 64 + (((i >> 3) ^ lane) & 7) * 8, y);
+                        for (int e = 0; e < 8; ++e) y[e] = x[i + e] * inv;
+                        kv_store8(mine + lane * 64 + ((((c + i) >> 3) ^ lane) & 7) * 8, y);
                     }
-                    __syncwarp();
+                    if (c & 32) {   // 64 dimensions through shared memory, so that 8 lanes write 128 bytes of a row
+                        __syncwarp();
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const int r = i * 4 + (lane >> 3), k = lane & 7;
-                        const long long ro = __shfl_sync(0xFFFFFFFFu, off, r);
-                        const uint4 v = *reinterpret_cast<const uint4 *>(mine + r * 64 + ((k ^ r) & 7) * 8);
-                        if (ro >= 0) *reinterpret_cast<uint4 *>(out + ro + c + k * 8) = v;
+                        for (int i = 0; i < 8; ++i) {
+                            const int r = i * 4 + (lane >> 3), k = lane & 7;
+                            const long long ro = __shfl_sync(0xFFFFFFFFu, off, r);
+                            const uint4 v = *reinterpret_cast<const uint4 *>(mine + r * 64 + ((k ^ r) & 7) * 8);
+                            if (ro >= 0) *reinterpret_cast<uint4 *>(out + ro + c - 32 + k * 8) = v;
+                        }
+                        __syncwarp();
                     }
-                    __syncwarp();
                 }
                 // rows that are not finite: V of a position that a row does not see may have been
                 // (0 * NaN), or a page lies outside the pool.  Once more, over their own positions only.
@@ -804,8 +867,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                     __syncwarp();
                 }
             }
-            next_item(j1);
         }
+        if (tell >= 0) told();
     }
     // ---- the end: nothing in flight, TMEM given back ----
     tc_fence_before();
