@@ -192,6 +192,8 @@ __global__ void __launch_bounds__(FewCfg<HD, TI, TC>::W * 32, FewCfg<HD, TI, TC>
     using E = typename KvType<TC>::E;
     constexpr int W = Cfg::W, T = W * 32, NST = Cfg::NST, NQ = Cfg::NQ, NP = Cfg::NP, ES = Cfg::ES;
     constexpr bool X32 = TC == QT_F32;
+    constexpr bool FINE = TI == QT_F32;          // fp32 results
+    constexpr int NC = FINE ? 5 : 2;             // accumulators of a score: 4 and the small products', or 2
     constexpr int KS = X32 ? HD / 8 : HD / 16;   // steps of the product over the head's dimensions
     constexpr int CB = HD * ES / 128;            // 128-byte columns of a row
     constexpr uint32_t kCol = kSlice * 128, kTile = CB * kCol;
@@ -211,6 +213,9 @@ __global__ void __launch_bounds__(FewCfg<HD, TI, TC>::W * 32, FewCfg<HD, TI, TC>
         sh.fail = 0;
         sh.seq = a.b.n_seqs;
     }
+    if (tid < 2) prefetch_map(tid ? &vmap : &kmap);
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     // ---- this CTA's share of all steps: a scan over the sequences ----
     const int per = (a.b.n_seqs + T - 1) / T, sq0 = tid * per, sq1 = min(a.b.n_seqs, sq0 + per);
     unsigned long long mine = 0;
@@ -421,8 +426,14 @@ __global__ void __launch_bounds__(FewCfg<HD, TI, TC>::W * 32, FewCfg<HD, TI, TC>
                     fence_proxy_async_smem();   // before the stage's next copy
                     __syncwarp();
                 }
-                // ---- S^T = K Q^T ----
-                float c[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+                // ---- S^T = K Q^T; the tensor core truncates what it adds to an accumulator, so
+                // fp32 results come from short chains that are added in fp32, the small
+                // products by themselves ----
+                float c[NC][4];
+#pragma unroll
+                for (int i = 0; i < NC; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) c[i][e] = 0.f;
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks) {
                     const uint32_t ch = 2 * ks + kchunk;
@@ -432,17 +443,23 @@ __global__ void __launch_bounds__(FewCfg<HD, TI, TC>::W * 32, FewCfg<HD, TI, TC>
                         uint32_t hi[4], lo[4];
 #pragma unroll
                         for (int e = 0; e < 4; ++e) split_tf32(x[e], hi[e], lo[e]);
-                        mma_tf32(c[ks & 1], lo, qf[0][ks][0], qf[0][ks][1]);
-                        mma_tf32(c[ks & 1], hi, qf[1][ks][0], qf[1][ks][1]);
-                        mma_tf32(c[ks & 1], hi, qf[0][ks][0], qf[0][ks][1]);
+                        mma_tf32(c[NC - 1], lo, qf[0][ks][0], qf[0][ks][1]);
+                        mma_tf32(c[NC - 1], hi, qf[1][ks][0], qf[1][ks][1]);
+                        mma_tf32(c[FINE ? ks & 3 : ks & 1], hi, qf[0][ks][0], qf[0][ks][1]);
                     } else {
 #pragma unroll
-                        for (int n = NQ - 1; n >= 0; --n) mma16<TC>(c[ks & 1], x, qf[n][ks][0], qf[n][ks][1]);
+                        for (int n = NQ - 1; n >= 0; --n)
+                            mma16<TC>(c[n > 0 ? NC - 1 : FINE ? ks & 3 : ks & 1], x, qf[n][ks][0], qf[n][ks][1]);
                     }
                 }
                 float x[4];   // (position g, row 2 t), (g, 2 t + 1), (g + 8, 2 t), (g + 8, 2 t + 1)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x[e] = (c[0][e] + c[1][e]) * rs[e & 1];
+                for (int e = 0; e < 4; ++e) {
+                    float sum = c[NC - 1][e];   // the small products, or the second chain
+                    if constexpr (FINE) sum = ((c[0][e] + c[1][e]) + (c[2][e] + c[3][e])) + sum;
+                    else sum += c[0][e];
+                    x[e] = sum * rs[e & 1];
+                }
                 if (bad || j0 + kSlice - 1 > pmin ||
                     (a.window > 0 && j0 <= pmax - a.window && j0 + kSlice > a.sinks)) {
 #pragma unroll
@@ -503,10 +520,12 @@ __global__ void __launch_bounds__(FewCfg<HD, TI, TC>::W * 32, FewCfg<HD, TI, TC>
                                     const uint4 &w = v[e & 1][e >> 1];
                                     split_tf32(d == 0 ? w.x : d == 1 ? w.y : d == 2 ? w.z : w.w, hi[e], lo[e]);
                                 }
-                                float(&o)[4] = O[jb * 4 + d];
+                                float o[4] = {0.f, 0.f, 0.f, 0.f};   // added in fp32: see S^T
                                 mma_tf32(o, lo, ph[kb8][0], ph[kb8][1]);
                                 mma_tf32(o, hi, pl[kb8][0], pl[kb8][1]);
                                 mma_tf32(o, hi, ph[kb8][0], ph[kb8][1]);
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) O[jb * 4 + d][e] += o[e];
                             }
                         }
                 } else {
@@ -520,8 +539,16 @@ __global__ void __launch_bounds__(FewCfg<HD, TI, TC>::W * 32, FewCfg<HD, TI, TC>
                         const uint32_t ch = 2 * i + vchunk;
                         uint32_t v[4];
                         ldsm4t(vb + (ch >> 3) * kCol + vrow * 128 + (((ch & 7) ^ (vrow & 7)) << 4), v);
+                        if constexpr (FINE) {
+                            float o[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                        for (int n = NP - 1; n >= 0; --n) mma16<TC>(O[i], v, pb[n][0], pb[n][1]);
+                            for (int n = NP - 1; n >= 0; --n) mma16<TC>(o, v, pb[n][0], pb[n][1]);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) O[i][e] += o[e];
+                        } else {
+#pragma unroll
+                            for (int n = NP - 1; n >= 0; --n) mma16<TC>(O[i], v, pb[n][0], pb[n][1]);
+                        }
                     }
                 }
                 __syncwarp();   // every lane has read the stage
@@ -695,8 +722,8 @@ static int few_launch(AttnArgs &a, int sms, cudaStream_t st)
         return 0;
     }
     const int grid = sms * Cfg::CTAS < kMaxCtas ? sms * Cfg::CTAS : kMaxCtas;
-    fn<<<grid, Cfg::W * 32, Cfg::SMEM, st>>>(km, vm, a);
-    return cudaGetLastError() == cudaSuccess ? 1 : 0;
+    void *args[] = {&km, &vm, &a};
+    return kv_launch(reinterpret_cast<const void *>(fn), dim3(grid), Cfg::W * 32, Cfg::SMEM, args, st);
 }
 
 template <int HD, int TI>

@@ -206,11 +206,6 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *map
                  : "memory");
 }
 
-__device__ __forceinline__ void prefetch_map(const CUtensorMap *m)
-{
-    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(m)) : "memory");
-}
-
 // 2^x for two x, on the FMA pipe: the multi-function unit gives 4 results a clock
 // and sub-core, and 128 x 128 scores would hold it as long as the tensor core
 // needs for both products.  x = n + f with n the nearest integer (by adding 1.5 *
@@ -297,6 +292,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     }
     if (warp == 9 && lane < 2) prefetch_map(lane ? &vmap : &kmap);
     if (warp == 10 && lane == 0) prefetch_map(&qmap);
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     // ---- this CTA's share of all units: a scan over the sequences ----
     const int per = (a.a.b.n_seqs + kManyThreads - 1) / kManyThreads;
     const int sq0 = min(a.a.b.n_seqs, tid * per), sq1 = min(a.a.b.n_seqs, sq0 + per);
@@ -325,6 +322,10 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     }
     const unsigned G = total < gridDim.x ? static_cast<unsigned>(total) : gridDim.x;
     if (blockIdx.x >= G) return;
+    if (warp == 8) {
+        tmem_alloc(smem_u32(&sh.tmem), 512);
+        tmem_relinquish();
+    }
     const unsigned cta = G - 1 - blockIdx.x;   // of the units, against blockIdx: see the joining of parts
     const unsigned long long per_cta = total / G;
     const unsigned extra = static_cast<unsigned>(total % G);
@@ -369,10 +370,6 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             rem -= __shfl_sync(0xFFFFFFFFu, c, 31);
         }
         if (lane == src) sh.seq = fs;
-    }
-    if (warp == 8) {
-        tmem_alloc(smem_u32(&sh.tmem), 512);
-        tmem_relinquish();
     }
     tc_fence_before();
     __syncthreads();
@@ -919,8 +916,9 @@ static int many_launch(ManyArgs &m, int tc, int sms, cudaStream_t st)
         cudaGetLastError();
         return 0;
     }
-    fn<<<sms < kManyCtas ? sms : kManyCtas, kManyThreads, ManyCfg<HD>::SMEM, st>>>(qm, km, vm, m);
-    return cudaGetLastError() == cudaSuccess ? 1 : 0;
+    void *args[] = {&qm, &km, &vm, &m};
+    return kv_launch(reinterpret_cast<const void *>(fn), dim3(sms < kManyCtas ? sms : kManyCtas), kManyThreads,
+                     ManyCfg<HD>::SMEM, args, st);
 }
 
 int kv_many_launch(AttnArgs a, int hd, int tc, int few_rows, int sms, cudaStream_t st)

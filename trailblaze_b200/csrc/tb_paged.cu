@@ -59,90 +59,155 @@ struct AppendArgs {
     int n_pos, rot, inter, nh;
     float eps;
     int *err;
+    int parts;   // warps a token
 };
 
-// CTA (token, part of the heads): 8 elements a lane, so HD / 8 lanes hold a head
-// and a warp 32 * 8 / HD heads.  A lane's dimensions are the same for every head
-// that it visits, so the token's cos and sin sit in its registers:
+// One warp per token, or per part of a token's heads when tokens are few; 8
+// elements a lane, so HD / 8 lanes hold a head and a warp 32 * 8 / HD of them.  A
+// lane's dimensions are the same for every head that it visits, so the token's cos
+// and sin sit in its registers:
 //   y[d] = x[d] cos + x[partner] sin', sin' negative for a pair's first element.
-// Interleaved pairs lie in one lane; halves are exchanged through shared memory,
-// which takes any rot_dim.
+// Interleaved pairs lie in one lane; halves are exchanged by shuffles where rot_dim
+// is a multiple of 16 (whole lanes change places), through shared memory else.
+// Bound by the rows' bytes: 4 heads' loads are in flight a lane, the first before
+// the look-up of the token's sequence, page and angles.
+static constexpr int kAppendU = 4;
+
 template <int HD, int TI, int TC>
-__global__ void __launch_bounds__(256) k_kv_append(const AppendArgs a)
+__global__ void __launch_bounds__(256) k_kv_append(const __grid_constant__ AppendArgs a)
 {
     using I = typename KvType<TI>::E;
     using C = typename KvType<TC>::E;
-    constexpr int L = HD / 8, HW = 32 / L;   // lanes a head, heads a warp
-    __shared__ int s_at;
+    constexpr int L = HD / 8, HW = 32 / L, U = kAppendU;   // lanes a head, heads a warp
     __shared__ __align__(16) float xs[8 * HW][HD];
-    const int t = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int s = kv_seq_of_row(a.b, t, &s_at, a.err);
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    if (blockIdx.x == 0)   // ranges that cannot be are reported once, whatever tokens they claim
+        for (int s = threadIdx.x; s < a.b.n_seqs; s += 256) {
+            KvSeq q;
+            kv_seq(a.b, a.c, s, q, a.err);
+        }
+    const uint32_t w = blockIdx.x * 8u + warp, wt = w / static_cast<uint32_t>(a.parts);
+    if (wt >= static_cast<uint32_t>(a.b.n_tokens)) return;
+    const int t = static_cast<int>(wt), part = static_cast<int>(w - wt * a.parts);
+    const int grp = lane / L, d0 = (lane % L) * 8;   // the lane's head of the warp's, its first dimension
+    const int nq = a.nh, nk = a.c.n_kv_heads, items = nq + 2 * nk;   // q heads, k heads, v heads
+    const int step = a.parts * HW;
+    auto source = [&](int it) {
+        const KvRows &r = it < nq ? a.q : it < nq + nk ? a.k : a.v;
+        const int h = it < nq ? it : it < nq + nk ? it - nq : it - nq - nk;
+        return static_cast<const I *>(r.p) + t * r.row + h * r.head + d0;
+    };
+    float x[U][8];
+    auto load = [&](int base) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int it = base + u * step + grp;
+            if (it < items) kv_load8(source(it), x[u]);
+        }
+    };
+    load(part * HW);
+    // ---- the token's sequence, position, page and angles ----
+    int s;
+    if (a.b.n_seqs <= 32) {
+        const unsigned hit = __ballot_sync(0xFFFFFFFFu, lane < a.b.n_seqs && a.b.start[lane] <= t && t < a.b.start[lane + 1]);
+        s = __ffs(hit) - 1;
+    } else {   // the first sequence that ends after t
+        int lo = 0, hi = a.b.n_seqs;
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (a.b.start[mid + 1] > t) hi = mid;
+            else lo = mid + 1;
+        }
+        s = lo < a.b.n_seqs && a.b.start[lo] <= t ? lo : -1;
+    }
     if (s < 0) return;   // a row of no sequence
     KvSeq q;
     const bool ok = kv_seq(a.b, a.c, s, q, a.err);
     const int pos = q.len - q.n + (t - q.row0);
     long long at = -1;
     if (ok && (!a.table || pos < a.n_pos)) at = kv_at(a.b, a.c, s, pos, 0, a.err);
-    else if (ok && threadIdx.x == 0) atomicExch(a.err, ERR_RUNTIME);
-    const int grp = lane / L, d0 = (lane % L) * 8;   // the lane's head of the warp's, its first dimension
+    else if (ok && lane == 0) atomicExch(a.err, ERR_RUNTIME);
     float cs[8], sn[8];
-    int partner[8];
     const int half = a.rot / 2;
+    const bool shuffle = !a.inter && (half & 7) == 0;
+    bool turned[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
         const int d = d0 + e;
-        cs[e] = 1.f, sn[e] = 0.f, partner[e] = -1;
-        if (a.table && at >= 0 && d < a.rot) {
+        cs[e] = 1.f, sn[e] = 0.f;
+        turned[e] = a.table && at >= 0 && d < a.rot;
+        if (turned[e]) {
             const bool second = a.inter ? (d & 1) : d >= half;
             const int pair = a.inter ? d >> 1 : second ? d - half : d;
-            partner[e] = a.inter ? d ^ 1 : second ? d - half : d + half;
-            const float2 w = __ldg(reinterpret_cast<const float2 *>(a.table) + static_cast<long long>(pos) * half + pair);
-            cs[e] = w.x;
-            sn[e] = second ? w.y : -w.y;
+            const float2 v = __ldg(reinterpret_cast<const float2 *>(a.table) + static_cast<long long>(pos) * half + pair);
+            cs[e] = v.x;
+            sn[e] = second ? v.y : -v.y;
         }
     }
-    const int items = a.nh + a.c.n_kv_heads;
-    for (int base = (blockIdx.y * 8 + warp) * HW; base < items; base += gridDim.y * 8 * HW) {
-        const int it = base + grp;
-        const bool on = it < items, isq = it < a.nh;
-        const int h = isq ? it : it - a.nh;
-        const KvRows &src = isq ? a.q : a.k;
-        float x[8];
+    const int mate = !turned[0] ? lane : d0 >= half ? lane - half / 8 : lane + half / 8;   // of whole lanes
+    for (int base = part * HW; base < items; base += U * step) {
+        if (base != part * HW) load(base);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = 0.f;
-        if (on) kv_load8(static_cast<const I *>(src.p) + t * src.row + h * src.head + d0, x);
-        const float *nw = isq ? a.qn : a.kn;
-        float ss = 0.f;
+        for (int u = 0; u < U; ++u) {
+            const int it = base + u * step + grp;
+            if (base + u * step >= items) break;
+            const bool on = it < items, isq = it < nq, isv = it >= nq + nk;
+            float y[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
+            for (int e = 0; e < 8; ++e) y[e] = on ? x[u][e] : 0.f;
+            const float *nw = isq ? a.qn : a.kn;
+            if (a.qn || a.kn) {
+                float ss = 0.f;
 #pragma unroll
-        for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
-        if (nw) {
-            const float sc = 1.0f / sqrtf(ss / static_cast<float>(HD) + a.eps);
-            float w[8];
-            kv_load8(nw + d0, w);
+                for (int e = 0; e < 8; ++e) ss = fmaf(y[e], y[e], ss);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = x[e] * sc * w[e];
-        }
-        float *mine = xs[warp * HW + grp];
-        kv_store8(mine + d0, x);
-        __syncwarp();
-        float y[8];
+                for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
+                if (nw && !isv) {
+                    const float sc = 1.0f / sqrtf(ss / static_cast<float>(HD) + a.eps);
+                    float wv[8];
+                    kv_load8(nw + d0, wv);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = partner[e] >= 0 ? fmaf(mine[partner[e]], sn[e], x[e] * cs[e]) : x[e];
-        __syncwarp();
-        if (!on) continue;
-        if (isq) {
-            if (at < 0) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) y[e] = 0.f;
+                    for (int e = 0; e < 8; ++e) y[e] = y[e] * sc * wv[e];
+                }
             }
-            kv_store8(static_cast<I *>(const_cast<void *>(a.o.p)) + t * a.o.row + h * a.o.head + d0, y);
-        } else if (at >= 0) {
-            const long long to = at + h * a.c.head_stride + d0;
-            kv_store8(static_cast<C *>(const_cast<void *>(a.c.k)) + to, y);
-            kv_load8(static_cast<const I *>(a.v.p) + t * a.v.row + h * a.v.head + d0, x);
-            kv_store8(static_cast<C *>(const_cast<void *>(a.c.v)) + to, x);
+            if (a.table) {
+                float z[8];   // the partners
+                if (a.inter) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) z[e] = y[e ^ 1];
+                } else if (shuffle) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) z[e] = __shfl_sync(0xFFFFFFFFu, y[e], mate);
+                } else {
+                    float *mine = xs[warp * HW + grp];
+                    kv_store8(mine + d0, y);
+                    __syncwarp();
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const int d = d0 + e;
+                        z[e] = mine[!turned[e] ? d : d >= half ? d - half : d + half];
+                    }
+                    __syncwarp();
+                }
+                if (!isv) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (turned[e]) y[e] = fmaf(z[e], sn[e], y[e] * cs[e]);
+                }
+            }
+            if (!on) continue;
+            if (isq) {
+                if (at < 0) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) y[e] = 0.f;
+                }
+                kv_store8(static_cast<I *>(const_cast<void *>(a.o.p)) + t * a.o.row + it * a.o.head + d0, y);
+            } else if (at >= 0) {
+                const long long to = at + (isv ? it - nq - nk : it - nq) * a.c.head_stride + d0;
+                kv_store8(static_cast<C *>(const_cast<void *>(isv ? a.c.v : a.c.k)) + to, y);
+            }
         }
     }
 }
@@ -166,16 +231,13 @@ int kv_append_launch(const KvView &c, const KvBatch &b, int hd, int ti, int tc, 
                                                                                   : append_kernel<128, QT_BF16>(tc))
                          : (ti == QT_F32 ? append_kernel<64, QT_F32>(tc) : ti == QT_F16 ? append_kernel<64, QT_F16>(tc)
                                                                                  : append_kernel<64, QT_BF16>(tc));
-    // few tokens: their heads over several CTAs, one pass of the warps each
-    const int passes = (nh + c.n_kv_heads + 8 * (256 / hd) - 1) / (8 * (256 / hd));
-    int parts = 4 * sms / b.n_tokens;
-    parts = parts < 1 ? 1 : parts > passes ? passes : parts;
+    // few tokens: their heads over several warps, until the GPU has 16 warps an SM
+    const int hw = 256 / hd, passes = (nh + 2 * c.n_kv_heads + hw - 1) / hw;
+    const int parts = 16 * sms / b.n_tokens;
+    a.parts = parts < 1 ? 1 : parts > passes ? passes : parts;
+    const long long warps = static_cast<long long>(b.n_tokens) * a.parts;
     void *args[] = {&a};
-    if (cudaLaunchKernel(fn, dim3(b.n_tokens, parts), dim3(256), args, 0, st) != cudaSuccess) {
-        cudaGetLastError();
-        return 0;
-    }
-    return 1;
+    return kv_launch(fn, dim3(static_cast<unsigned>((warps + 7) / 8)), 256, 0, args, st);
 }
 
 // ---- page copies ----
@@ -184,24 +246,37 @@ static constexpr int kCopyPairs = 480;   // per launch: the pairs travel as a ke
 struct CopyArgs {
     char *k, *v;
     long long layer_stride, page_stride;    // bytes
-    long long run, cnt0, str0, cnt1, str1;  // a page: cnt1 x cnt0 runs of run bytes
-    int n_layers, n;
+    long long str0, str1;                   // a page: runs of run * 16 bytes, cnt0 of them str0 apart, these str1 apart
+    uint32_t vecs, piece;                   // 16-byte pieces of a page; how many of them a CTA copies
+    FastDiv run, cnt0;
     int src[kCopyPairs], dst[kCopyPairs];
 };
 
-// CTA (pair, K or V, layer): one page of one tensor.
+// CTA (pair and part of the page, K or V, layer).
+template <bool WHOLE>   // a page is one run
 __global__ void __launch_bounds__(256) k_kv_copy(const __grid_constant__ CopyArgs a)
 {
-    const int i = blockIdx.x;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const uint32_t parts = (a.vecs + a.piece - 1) / a.piece, i = blockIdx.x / parts, part = blockIdx.x - i * parts;
     char *base = (blockIdx.y ? a.v : a.k) + blockIdx.z * a.layer_stride;
     const char *from = base + a.src[i] * a.page_stride;
     char *to = base + a.dst[i] * a.page_stride;
-    const long long rv = a.run / 16, total = rv * a.cnt0 * a.cnt1;
-    for (long long u = threadIdx.x; u < total; u += 256) {
-        const long long w = u % rv, r = u / rv;
-        const long long off = w * 16 + (r % a.cnt0) * a.str0 + (r / a.cnt0) * a.str1;
-        *reinterpret_cast<uint4 *>(to + off) = *reinterpret_cast<const uint4 *>(from + off);
+    const uint32_t end = min(a.vecs, (part + 1) * a.piece);
+    auto at = [&](uint32_t u) -> long long {
+        if (WHOLE) return u * 16ll;
+        const uint32_t r = fdiv(u, a.run), r1 = fdiv(r, a.cnt0);
+        return (u - r * a.run.d) * 16ll + (r - r1 * a.cnt0.d) * a.str0 + r1 * a.str1;
+    };
+    uint32_t u = part * a.piece + threadIdx.x;
+    for (; u + 3 * 256 < end; u += 4 * 256) {
+        uint4 x[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[k] = __ldcs(reinterpret_cast<const uint4 *>(from + at(u + k * 256)));
+#pragma unroll
+        for (int k = 0; k < 4; ++k) *reinterpret_cast<uint4 *>(to + at(u + k * 256)) = x[k];
     }
+    for (; u < end; u += 256) *reinterpret_cast<uint4 *>(to + at(u)) = __ldcs(reinterpret_cast<const uint4 *>(from + at(u)));
 }
 
 int kv_copy_launch(void *k, void *v, int esize, int n_layers, int n_pages, int page_size, int n_kv_heads, int hd,
@@ -229,7 +304,6 @@ int kv_copy_launch(void *k, void *v, int esize, int n_layers, int n_pages, int p
     a.v = static_cast<char *>(v);
     a.layer_stride = layer_stride * esize;
     a.page_stride = page_stride * esize;
-    a.n_layers = n_layers;
     // a page as runs: the head's row, then the inner and the outer of heads and positions
     long long run = static_cast<long long>(hd) * esize;
     long long c0 = page_size, s0 = pos_stride * esize, c1 = n_kv_heads, s1 = head_stride * esize;
@@ -242,12 +316,26 @@ int kv_copy_launch(void *k, void *v, int esize, int n_layers, int n_pages, int p
         c0 = c1, s0 = s1, c1 = 1, s1 = 0;
         if (s0 == run) run *= c0, c0 = 1, s0 = 0;
     }
-    a.run = run, a.cnt0 = c0, a.str0 = s0, a.cnt1 = c1, a.str1 = s1;
-    for (int i0 = 0; i0 < n; i0 += kCopyPairs) {
-        a.n = n - i0 < kCopyPairs ? n - i0 : kCopyPairs;
-        for (int i = 0; i < a.n; ++i) a.src[i] = src[i0 + i], a.dst[i] = dst[i0 + i];
-        k_kv_copy<<<dim3(a.n, 2, n_layers), 256, 0, st>>>(a);
-        if (cudaGetLastError() != cudaSuccess) return 0;
+    const long long vecs = run / 16 * c0 * c1;
+    if (vecs > 0x40000000) return 0;   // a page of 16 GB
+    const bool whole = c0 == 1 && c1 == 1;
+    a.vecs = static_cast<uint32_t>(vecs);
+    a.run = make_fastdiv(static_cast<uint32_t>(run / 16));
+    a.cnt0 = make_fastdiv(static_cast<uint32_t>(c0));
+    a.str0 = s0, a.str1 = s1;
+    // 16 KB a CTA while that leaves the GPU room, else 64 KB: a fork's few pages spread
+    // over all SMs, and many pages do not pay for a CTA's start every 16 KB
+    const long long small = static_cast<long long>(n) * 2 * n_layers * ((vecs + 1023) / 1024);
+    a.piece = small <= 16 * 148 ? 1024 : 4096;
+    const uint32_t parts = (a.vecs + a.piece - 1) / a.piece;
+    const int per = static_cast<int>(0x7FFFFFFF / parts) < kCopyPairs ? static_cast<int>(0x7FFFFFFF / parts) : kCopyPairs;
+    for (int i0 = 0; i0 < n; i0 += per) {
+        const int m = n - i0 < per ? n - i0 : per;
+        for (int i = 0; i < m; ++i) a.src[i] = src[i0 + i], a.dst[i] = dst[i0 + i];
+        void *args[] = {&a};
+        if (!kv_launch(whole ? reinterpret_cast<void *>(k_kv_copy<true>) : reinterpret_cast<void *>(k_kv_copy<false>),
+                       dim3(m * parts, 2, n_layers), 256, 0, args, st))
+            return 0;
     }
     return 1;
 }

@@ -44,6 +44,26 @@ int kv_attend_launch(const KvView &c, const KvBatch &b, int hd, int ti, int tc, 
                      const KvRows &o, float scale, int window, int sinks, int max_new, int max_len, void *ws, int *err,
                      int sms, uint32_t wait_limit, cudaStream_t st);
 
+// Launch with programmatic stream serialization: the kernels of the paged cache
+// begin with griddepcontrol.wait (after what needs no other kernel's data), so a
+// launch's start-up overlaps the end of the one before it.  1 = launched.
+inline int kv_launch(const void *fn, dim3 grid, unsigned threads, size_t smem, void **args, cudaStream_t st)
+{
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cudaLaunchKernelExC(&cfg, fn, args) == cudaSuccess) return 1;
+    cudaGetLastError();
+    return 0;
+}
+
 // Element types as template arguments.
 template <int T> struct KvType;
 template <> struct KvType<QT_F32> { using E = float; };
@@ -119,22 +139,6 @@ __device__ __forceinline__ bool kv_seq(const KvBatch &b, const KvView &c, int s,
                     q.len <= static_cast<long long>(b.pages_stride) * c.page_size;
     if (!ok && err) atomicExch(err, ERR_RUNTIME);
     return ok;
-}
-
-// The sequence whose rows hold row t (-1: none; the first where ranges overlap),
-// found by the whole CTA, which sees every range pass by and reports those that
-// cannot be; s_at is one shared int.
-__device__ __forceinline__ int kv_seq_of_row(const KvBatch &b, int t, int *s_at, int *err)
-{
-    if (threadIdx.x == 0) *s_at = 0x7FFFFFFF;
-    __syncthreads();
-    for (int s = threadIdx.x; s < b.n_seqs; s += blockDim.x) {
-        const int a = b.start[s], e = b.start[s + 1];
-        if (a <= t && t < e) atomicMin(s_at, s);
-        if (a < 0 || e < a || e > b.n_tokens) atomicExch(err, ERR_RUNTIME);
-    }
-    __syncthreads();
-    return *s_at == 0x7FFFFFFF ? -1 : *s_at;
 }
 
 // Element offset of position p of sequence s for kv head h; -1 (and the error

@@ -25,6 +25,11 @@ import torch
 from . import qtypes as Q
 from ._lib import KvBatch, KvCache, KvRope, KvRows, RopeScale, lib
 
+# the current stream's handle on a device, without a torch.cuda.Stream around it (some microseconds of a
+# call that a decode step makes for every layer)
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else \
+    lambda index: torch.cuda.current_stream(index).cuda_stream
+
 _TYPES = {torch.float32: Q.F32, torch.float16: Q.F16, torch.bfloat16: Q.BF16}
 
 
@@ -35,13 +40,14 @@ def _type(t: torch.Tensor) -> int:
 
 
 def _rows(t: torch.Tensor, heads: int, dim: int, device) -> KvRows:
-    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != dim or (t.shape[2] > 1 and t.stride(2) != 1):
-        raise ValueError(f"rows of shape {tuple(t.shape)}, strides {t.stride()}: [tokens, {heads}, {dim}] with "
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 3 or shape[1] != heads or shape[2] != dim or stride[2] != 1:
+        raise ValueError(f"rows of shape {tuple(shape)}, strides {stride}: [tokens, {heads}, {dim}] with "
                          "contiguous dimensions expected")
     if t.device != device:
         raise ValueError(f"rows on {t.device}: the cache is on {device}")
     # a dimension of one element has no stride of its own
-    return KvRows(t.data_ptr(), t.stride(0) if t.shape[0] > 1 else 0, t.stride(1) if heads > 1 else 0)
+    return KvRows(t.data_ptr(), stride[0] if shape[0] > 1 else 0, stride[1] if heads > 1 else 0)
 
 
 def _vector(t: torch.Tensor | None, n: int, what: str, device) -> int | None:
@@ -183,7 +189,7 @@ class PagedKV:
         self._ref = ctypes.byref(self.struct)
         self.n_layers, self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = k.shape
         self.pool = PagePool(n_pages, page)
-        self._ws: dict[int, torch.Tensor] = {}   # by stream: calls that may overlap have one each
+        self._ws: dict[int, tuple] = {}   # by stream: calls that may overlap have one each
 
     @classmethod
     def alloc(cls, n_layers: int, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int,
@@ -232,7 +238,7 @@ class PagedKV:
         self._tokens(batch, q, k, v)
         rq, rk, rv = _rows(q, heads, dim, dev), _rows(k, self.n_kv_heads, dim, dev), _rows(v, self.n_kv_heads, dim, dev)
         if q_out is None:
-            q_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+            q_out = torch.empty_like(q)
         elif q_out.shape != q.shape or q_out.dtype != q.dtype:
             raise ValueError("q_out: the shape and type of q expected")
         ro = _rows(q_out, heads, dim, dev)
@@ -241,12 +247,10 @@ class PagedKV:
         else:
             qn, kn = _vector(q_norm, dim, "q_norm", dev), _vector(k_norm, dim, "k_norm", dev)
             r = rope.struct(qn, kn, eps) if rope else KvRope(None, qn, kn, 0, 0, 0, eps)
-        with torch.cuda.device(dev):
-            if self.L.tb_cuda_kv_append_dev(self._ref, layer, batch._ref, _type(q), heads, ctypes.byref(rq),
-                                            ctypes.byref(rk), ctypes.byref(rv), ctypes.byref(ro),
-                                            ctypes.byref(r) if r is not None else None,
-                                            torch.cuda.current_stream().cuda_stream) != 1:
-                raise ValueError("tb_cuda_kv_append_dev refused the call")
+        if self._on_device(self.L.tb_cuda_kv_append_dev, self._ref, layer, batch._ref, _type(q), heads,
+                           ctypes.byref(rq), ctypes.byref(rk), ctypes.byref(rv), ctypes.byref(ro),
+                           ctypes.byref(r) if r is not None else None, _raw_stream(dev.index)) != 1:
+            raise ValueError("tb_cuda_kv_append_dev refused the call")
         return q_out
 
     def attend(self, layer: int, batch: Batch, q: torch.Tensor, out: torch.Tensor | None = None,
@@ -256,19 +260,19 @@ class PagedKV:
         self._tokens(batch, q)
         rq = _rows(q, heads, dim, dev)
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+            out = torch.empty_like(q)
         elif out.shape != q.shape or out.dtype != q.dtype:
             raise ValueError("out: the shape and type of q expected")
         ro = _rows(out, heads, dim, dev)
-        with torch.cuda.device(dev):
-            stream = torch.cuda.current_stream().cuda_stream
-            ws = self._ws.get(stream)
-            if ws is None:
-                ws = self._ws[stream] = torch.zeros(self.L.tb_cuda_kv_attend_ws(), dtype=torch.uint8, device=dev)
-            if self.L.tb_cuda_kv_attend_dev(self._ref, layer, batch._ref, _type(q), heads, ctypes.byref(rq),
-                                            ctypes.byref(ro), 1.0 / math.sqrt(dim) if scale is None else scale, window,
-                                            sinks, ws.data_ptr(), ws.numel(), stream) != 1:
-                raise ValueError("tb_cuda_kv_attend_dev refused the call")
+        stream = _raw_stream(dev.index)
+        ws = self._ws.get(stream)
+        if ws is None:
+            ws = torch.zeros(self.L.tb_cuda_kv_attend_ws(), dtype=torch.uint8, device=dev)
+            ws = self._ws[stream] = (ws, ws.data_ptr(), ws.numel())
+        if self._on_device(self.L.tb_cuda_kv_attend_dev, self._ref, layer, batch._ref, _type(q), heads,
+                           ctypes.byref(rq), ctypes.byref(ro), 1.0 / math.sqrt(dim) if scale is None else scale, window,
+                           sinks, ws[1], ws[2], stream) != 1:
+            raise ValueError("tb_cuda_kv_attend_dev refused the call")
         return out
 
     def copy_pages(self, src, dst) -> None:
@@ -276,14 +280,21 @@ class PagedKV:
         src, dst = np.ascontiguousarray(src, dtype=np.int32), np.ascontiguousarray(dst, dtype=np.int32)
         if src.ndim != 1 or src.shape != dst.shape:
             raise ValueError("src and dst: page numbers, one for one")
+        if self._on_device(self.L.tb_cuda_kv_copy_dev, self._ref, src.ctypes.data, dst.ctypes.data, src.size,
+                           _raw_stream(self.device.index)) != 1:
+            raise ValueError("tb_cuda_kv_copy_dev refused the pages")
+
+    def _on_device(self, call, *args) -> int:
+        """The entry points launch on the current device: the cache's, for the length of the call."""
+        if torch.cuda.current_device() == self.device.index:
+            return call(*args)
         with torch.cuda.device(self.device):
-            if self.L.tb_cuda_kv_copy_dev(self._ref, src.ctypes.data, dst.ctypes.data, src.size,
-                                          torch.cuda.current_stream().cuda_stream) != 1:
-                raise ValueError("tb_cuda_kv_copy_dev refused the pages")
+            return call(*args)
 
     def _tokens(self, batch: Batch, *rows: torch.Tensor) -> None:
+        n, dtype = batch.n_tokens, rows[0].dtype
         for t in rows:
-            if t.shape[0] != batch.n_tokens:
-                raise ValueError(f"{t.shape[0]} rows: the batch has {batch.n_tokens}")
-            if t.dtype != rows[0].dtype:
+            if t.dim() != 3 or t.shape[0] != n:
+                raise ValueError(f"rows of shape {tuple(t.shape)}: the batch has {n} rows")
+            if t.dtype != dtype:
                 raise ValueError("q, k and v of one type expected")
