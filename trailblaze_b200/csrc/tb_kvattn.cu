@@ -636,9 +636,15 @@ __global__ void __launch_bounds__(FewCfg<HD, TI, TC>::W * 32, FewCfg<HD, TI, TC>
             const int tok = (r0 + mr) / a.group, hh = (r0 + mr) - tok * a.group;
             I *op = static_cast<I *>(const_cast<void *>(a.o.p)) + (cu.q.row0 + tok) * a.o.row +
                     (cu.h * a.group + hh) * a.o.head + md;
-            const float inv = 1.0f / L;
+            const float inv = L == 0.f ? 0.f : 1.0f / L;
 #pragma unroll
-            for (int d = 0; d < PER; ++d) kv_store1(op + d, L == 0.f ? 0.f : acc[d] * inv);
+            for (int d = 0; d < PER; ++d) acc[d] = L == 0.f ? 0.f : acc[d] * inv;
+            if constexpr (PER == 8) {
+                kv_store8(op, acc);
+            } else {
+#pragma unroll
+                for (int d = 0; d < PER; ++d) kv_store1(op + d, acc[d]);
+            }
         };
         if (from_start && to_end) {
             write_out();
@@ -651,7 +657,8 @@ __global__ void __launch_bounds__(FewCfg<HD, TI, TC>::W * 32, FewCfg<HD, TI, TC>
             float *mp = a.part + static_cast<size_t>(2 * cta + (from_start ? 1 : 0)) * P;
             if (mr < rows) {
 #pragma unroll
-                for (int d = 0; d < PER; ++d) mp[mr * HD + md + d] = acc[d];
+                for (int d = 0; d < PER; d += 4)
+                    *reinterpret_cast<float4 *>(mp + mr * HD + md + d) = make_float4(acc[d], acc[d + 1], acc[d + 2], acc[d + 3]);
                 if (md == 0) mp[8 * HD + mr] = M, mp[8 * HD + 8 + mr] = L;
             }
             __threadfence();
@@ -660,20 +667,50 @@ __global__ void __launch_bounds__(FewCfg<HD, TI, TC>::W * 32, FewCfg<HD, TI, TC>
             __syncthreads();
             if (sh.last) {
                 __threadfence();
-                if (mr < rows) {
-                    M = -INFINITY;
-                    for (unsigned c = c0; c <= c1; ++c)
-                        M = fmaxf(M, __ldcg(a.part + static_cast<size_t>(2 * c + (c == c0 ? 1 : 0)) * P + 8 * HD + mr));
-                    L = 0.f;
+                // m and l of every part in one go, then the sums with several loads ahead
+                constexpr int BATCH = Cfg::MERGE / 4 / 16;
+                float *ml = merge;   // [part][8 m, 8 l]
+                auto pbase = [&](unsigned c) { return a.part + static_cast<size_t>(2 * c + (c == c0 ? 1 : 0)) * P; };
+                M = -INFINITY, L = 0.f;
 #pragma unroll
-                    for (int d = 0; d < PER; ++d) acc[d] = 0.f;
-                    for (unsigned c = c0; c <= c1; ++c) {
-                        const float *pp = a.part + static_cast<size_t>(2 * c + (c == c0 ? 1 : 0)) * P;
-                        const float pm = __ldcg(pp + 8 * HD + mr), pl = __ldcg(pp + 8 * HD + 8 + mr);
-                        const float f = pm == -INFINITY ? 0.f : ex2(pm - M);
-                        L += pm == -INFINITY ? pl : f * pl;
+                for (int d = 0; d < PER; ++d) acc[d] = 0.f;
+                for (unsigned cb = c0; cb <= c1; cb += BATCH) {
+                    const int n = min(static_cast<int>(c1 - cb + 1), BATCH);
+                    __syncthreads();
+                    for (int i = tid; i < n * 16; i += T) ml[i] = __ldcg(pbase(cb + i / 16) + 8 * HD + i % 16);
+                    __syncthreads();
+                    float Mn = M;
+                    for (int i = 0; i < n; ++i) Mn = fmaxf(Mn, ml[i * 16 + mr]);
+                    const float f0 = M == -INFINITY ? 0.f : ex2(M - Mn);
+                    L = M == -INFINITY ? L : L * f0;
 #pragma unroll
-                        for (int d = 0; d < PER; ++d) acc[d] = fmaf(f, __ldcg(pp + mr * HD + md + d), acc[d]);
+                    for (int d = 0; d < PER; ++d) acc[d] *= f0;
+                    M = Mn;
+                    if (mr < rows) {
+                        constexpr int AHEAD = 4;
+                        for (int i0 = 0; i0 < n; i0 += AHEAD) {
+                            float4 v[AHEAD][PER / 4];
+#pragma unroll
+                            for (int i = 0; i < AHEAD; ++i)
+                                if (i0 + i < n)
+#pragma unroll
+                                    for (int d = 0; d < PER / 4; ++d)
+                                        v[i][d] = __ldcg(reinterpret_cast<const float4 *>(pbase(cb + i0 + i) + mr * HD + md) + d);
+#pragma unroll
+                            for (int i = 0; i < AHEAD; ++i) {
+                                if (i0 + i >= n) break;
+                                const float pm = ml[(i0 + i) * 16 + mr], pl = ml[(i0 + i) * 16 + 8 + mr];
+                                const float f = pm == -INFINITY ? 0.f : ex2(pm - M);
+                                L += pm == -INFINITY ? pl : f * pl;
+#pragma unroll
+                                for (int d = 0; d < PER / 4; ++d) {
+                                    acc[4 * d] = fmaf(f, v[i][d].x, acc[4 * d]);
+                                    acc[4 * d + 1] = fmaf(f, v[i][d].y, acc[4 * d + 1]);
+                                    acc[4 * d + 2] = fmaf(f, v[i][d].z, acc[4 * d + 2]);
+                                    acc[4 * d + 3] = fmaf(f, v[i][d].w, acc[4 * d + 3]);
+                                }
+                            }
+                        }
                     }
                 }
                 write_out();

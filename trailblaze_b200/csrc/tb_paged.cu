@@ -63,23 +63,33 @@ struct AppendArgs {
 };
 
 // One warp per token, or per part of a token's heads when tokens are few; 8
-// elements a lane, so HD / 8 lanes hold a head and a warp 32 * 8 / HD of them.  A
+// elements a lane, so HD / 8 lanes hold a head and a warp HW = 256 / HD of them.  A
 // lane's dimensions are the same for every head that it visits, so the token's cos
-// and sin sit in its registers:
+// and sin (and the norm's weights) sit in its registers:
 //   y[d] = x[d] cos + x[partner] sin', sin' negative for a pair's first element.
-// Interleaved pairs lie in one lane; halves are exchanged by shuffles where rot_dim
-// is a multiple of 16 (whole lanes change places), through shared memory else.
-// Bound by the rows' bytes: 4 heads' loads are in flight a lane, the first before
-// the look-up of the token's sequence, page and angles.
-static constexpr int kAppendU = 4;
+// Interleaved pairs lie in one lane; a half's partners are loaded a second time
+// (they are in L1 by then; shuffles took twice the instructions).  Bound by the
+// rows' bytes as long as enough of them are in flight: few instructions a head, two
+// heads' loads ahead a lane, the first of them before the look-up of the token's
+// sequence, page and angles.
+template <class E>
+struct Raw {   // 8 elements
+    uint4 v[sizeof(E) / 2];
+    __device__ __forceinline__ void load(const E *p)
+    {
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(sizeof(E) / 2); ++i) v[i] = reinterpret_cast<const uint4 *>(p)[i];
+    }
+    __device__ __forceinline__ void set(int e, E x) { reinterpret_cast<E *>(v)[e] = x; }
+    __device__ __forceinline__ void to(float (&x)[8]) const { kv_load8(reinterpret_cast<const E *>(v), x); }
+};
 
 template <int HD, int TI, int TC>
-__global__ void __launch_bounds__(256) k_kv_append(const __grid_constant__ AppendArgs a)
+__global__ void __launch_bounds__(256, 3) k_kv_append(const __grid_constant__ AppendArgs a)
 {
     using I = typename KvType<TI>::E;
     using C = typename KvType<TC>::E;
-    constexpr int L = HD / 8, HW = 32 / L, U = kAppendU;   // lanes a head, heads a warp
-    __shared__ __align__(16) float xs[8 * HW][HD];
+    constexpr int L = HD / 8, HW = 32 / L, U = 2;   // lanes a head, heads a warp, heads ahead
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -91,23 +101,38 @@ __global__ void __launch_bounds__(256) k_kv_append(const __grid_constant__ Appen
     const uint32_t w = blockIdx.x * 8u + warp, wt = w / static_cast<uint32_t>(a.parts);
     if (wt >= static_cast<uint32_t>(a.b.n_tokens)) return;
     const int t = static_cast<int>(wt), part = static_cast<int>(w - wt * a.parts);
-    const int grp = lane / L, d0 = (lane % L) * 8;   // the lane's head of the warp's, its first dimension
-    const int nq = a.nh, nk = a.c.n_kv_heads, items = nq + 2 * nk;   // q heads, k heads, v heads
-    const int step = a.parts * HW;
-    auto source = [&](int it) {
-        const KvRows &r = it < nq ? a.q : it < nq + nk ? a.k : a.v;
-        const int h = it < nq ? it : it < nq + nk ? it - nq : it - nq - nk;
-        return static_cast<const I *>(r.p) + t * r.row + h * r.head + d0;
-    };
-    float x[U][8];
-    auto load = [&](int base) {
+    const int d0 = (lane % L) * 8, grp = lane / L, step = a.parts * HW;
+    // passes of HW heads, q's, then k's, then v's: this warp's are part, part + parts, ...
+    const int nk = a.c.n_kv_heads, pq = (a.nh + HW - 1) / HW, pk = (nk + HW - 1) / HW;
+    auto first = [&](int p) { return (part >= p ? part : part + (p - part + a.parts - 1) / a.parts * a.parts) - p; };
+    const int h0 = part * HW + grp, hk = first(pq) * HW + grp, hv = first(pq + pk) * HW + grp;
+    const int half = a.rot / 2;
+    // of the lane's 8 dimensions, the first n_turn rotate; with halves, all or none of
+    // them have their partners 8 elements together, unless half is no multiple of 8
+    const int n_turn = a.table ? min(8, max(0, a.rot - d0)) : 0;
+    const bool apart = n_turn > 0 && !a.inter, together = (half & 7) == 0;
+    const int mate = d0 >= half ? -half : half;
+    Raw<I> x[U], z[U];
+    auto partners = [&](const I *p, Raw<I> &r) {
+        if (together) {
+            r.load(p + mate);
+        } else {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int it = base + u * step + grp;
-            if (it < items) kv_load8(source(it), x[u]);
+            for (int e = 0; e < 8; ++e) r.set(e, p[e < n_turn ? (d0 + e >= half ? e - half : e + half) : e]);
         }
     };
-    load(part * HW);
+    auto load = [&](const I *p, long long inc, int h, int n, bool rotates) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (h + u * step < n) {
+                x[u].load(p + u * inc);
+                if (rotates && apart) partners(p + u * inc, z[u]);
+            }
+        __syncwarp();   // q_out may be q: nothing is stored before its partner is read
+    };
+    const long long q_inc = step * a.q.head, k_inc = step * a.k.head, v_inc = step * a.v.head;
+    const I *qp = static_cast<const I *>(a.q.p) + t * a.q.row + h0 * a.q.head + d0;
+    load(qp, q_inc, h0, a.nh, true);
     // ---- the token's sequence, position, page and angles ----
     int s;
     if (a.b.n_seqs <= 32) {
@@ -123,91 +148,107 @@ __global__ void __launch_bounds__(256) k_kv_append(const __grid_constant__ Appen
         s = lo < a.b.n_seqs && a.b.start[lo] <= t ? lo : -1;
     }
     if (s < 0) return;   // a row of no sequence
-    KvSeq q;
-    const bool ok = kv_seq(a.b, a.c, s, q, a.err);
-    const int pos = q.len - q.n + (t - q.row0);
+    KvSeq sq;
+    const bool ok = kv_seq(a.b, a.c, s, sq, a.err);
+    const int pos = sq.len - sq.n + (t - sq.row0);
     long long at = -1;
     if (ok && (!a.table || pos < a.n_pos)) at = kv_at(a.b, a.c, s, pos, 0, a.err);
     else if (ok && lane == 0) atomicExch(a.err, ERR_RUNTIME);
     float cs[8], sn[8];
-    const int half = a.rot / 2;
-    const bool shuffle = !a.inter && (half & 7) == 0;
-    bool turned[8];
+    if (at >= 0) {
+        const float2 *row = reinterpret_cast<const float2 *>(a.table) + static_cast<long long>(pos) * half;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const int d = d0 + e;
-        cs[e] = 1.f, sn[e] = 0.f;
-        turned[e] = a.table && at >= 0 && d < a.rot;
-        if (turned[e]) {
-            const bool second = a.inter ? (d & 1) : d >= half;
-            const int pair = a.inter ? d >> 1 : second ? d - half : d;
-            const float2 v = __ldg(reinterpret_cast<const float2 *>(a.table) + static_cast<long long>(pos) * half + pair);
-            cs[e] = v.x;
-            sn[e] = second ? v.y : -v.y;
+        for (int e = 0; e < 8; ++e) {
+            const int d = d0 + e;
+            if (e < n_turn) {
+                const bool second = a.inter ? (e & 1) : d >= half;
+                const float2 v = __ldg(row + (a.inter ? d >> 1 : second ? d - half : d));
+                cs[e] = v.x;
+                sn[e] = second ? v.y : -v.y;
+            }
         }
     }
-    const int mate = !turned[0] ? lane : d0 >= half ? lane - half / 8 : lane + half / 8;   // of whole lanes
-    for (int base = part * HW; base < items; base += U * step) {
-        if (base != part * HW) load(base);
+    // norm (of q or k) and rotation of one head's 8 elements
+    auto turn = [&](const Raw<I> &xr, const Raw<I> &zr, const float *nw, float (&y)[8]) {
+        xr.to(y);
+        float sc = 1.f;
+        if (nw) {
+            float ss = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) ss = fmaf(y[e], y[e], ss);
+#pragma unroll
+            for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
+            sc = 1.0f / sqrtf(ss / static_cast<float>(HD) + a.eps);
+            float wv[8];
+            kv_load8(nw + d0, wv);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] = y[e] * sc * wv[e];
+        }
+        if (n_turn == 0) return;
+        float p[8];
+        if (a.inter) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) p[e] = y[e ^ 1];
+        } else {
+            zr.to(p);
+            if (nw) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (e < n_turn) p[e] = p[e] * sc * __ldg(nw + d0 + e + (d0 + e >= half ? -half : half));
+            }
+        }
+        if (n_turn == 8) {
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {
+                const float2 r = __ffma2_rn(make_float2(p[e], p[e + 1]), make_float2(sn[e], sn[e + 1]),
+                                            __fmul2_rn(make_float2(y[e], y[e + 1]), make_float2(cs[e], cs[e + 1])));
+                y[e] = r.x, y[e + 1] = r.y;
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (e < n_turn) y[e] = fmaf(p[e], sn[e], y[e] * cs[e]);
+        }
+    };
+    I *op = static_cast<I *>(const_cast<void *>(a.o.p)) + t * a.o.row + h0 * a.o.head + d0;
+    const long long o_inc = step * a.o.head;
+    for (int h = h0; h - grp < a.nh; h += U * step, qp += U * q_inc, op += U * o_inc) {
+        if (h != h0) load(qp, q_inc, h, a.nh, true);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int it = base + u * step + grp;
-            if (base + u * step >= items) break;
-            const bool on = it < items, isq = it < nq, isv = it >= nq + nk;
             float y[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) y[e] = on ? x[u][e] : 0.f;
-            const float *nw = isq ? a.qn : a.kn;
-            if (a.qn || a.kn) {
-                float ss = 0.f;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) ss = fmaf(y[e], y[e], ss);
-#pragma unroll
-                for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
-                if (nw && !isv) {
-                    const float sc = 1.0f / sqrtf(ss / static_cast<float>(HD) + a.eps);
-                    float wv[8];
-                    kv_load8(nw + d0, wv);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) y[e] = y[e] * sc * wv[e];
-                }
-            }
-            if (a.table) {
-                float z[8];   // the partners
-                if (a.inter) {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) z[e] = y[e ^ 1];
-                } else if (shuffle) {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) z[e] = __shfl_sync(0xFFFFFFFFu, y[e], mate);
-                } else {
-                    float *mine = xs[warp * HW + grp];
-                    kv_store8(mine + d0, y);
-                    __syncwarp();
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const int d = d0 + e;
-                        z[e] = mine[!turned[e] ? d : d >= half ? d - half : d + half];
-                    }
-                    __syncwarp();
-                }
-                if (!isv) {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        if (turned[e]) y[e] = fmaf(z[e], sn[e], y[e] * cs[e]);
-                }
-            }
-            if (!on) continue;
-            if (isq) {
+            turn(x[u], z[u], a.qn, y);
+            if (h + u * step < a.nh) {
                 if (at < 0) {
 #pragma unroll
                     for (int e = 0; e < 8; ++e) y[e] = 0.f;
                 }
-                kv_store8(static_cast<I *>(const_cast<void *>(a.o.p)) + t * a.o.row + it * a.o.head + d0, y);
-            } else if (at >= 0) {
-                const long long to = at + (isv ? it - nq - nk : it - nq) * a.c.head_stride + d0;
-                kv_store8(static_cast<C *>(const_cast<void *>(isv ? a.c.v : a.c.k)) + to, y);
+                kv_store8(op + u * o_inc, y);
             }
+        }
+    }
+    if (at < 0) return;
+    const I *kp = static_cast<const I *>(a.k.p) + t * a.k.row + hk * a.k.head + d0;
+    const I *vp = static_cast<const I *>(a.v.p) + t * a.v.row + hv * a.v.head + d0;
+    const long long c_inc = step * a.c.head_stride;
+    C *kc = static_cast<C *>(const_cast<void *>(a.c.k)) + at + hk * a.c.head_stride + d0;
+    C *vc = static_cast<C *>(const_cast<void *>(a.c.v)) + at + hv * a.c.head_stride + d0;
+    for (int h = hk; h - grp < nk; h += U * step, kp += U * k_inc, kc += U * c_inc) {
+        load(kp, k_inc, h, nk, true);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            float y[8];
+            turn(x[u], z[u], a.kn, y);
+            if (h + u * step < nk) kv_store8(kc + u * c_inc, y);
+        }
+    }
+    for (int h = hv; h - grp < nk; h += U * step, vp += U * v_inc, vc += U * c_inc) {
+        load(vp, v_inc, h, nk, false);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            float y[8];
+            x[u].to(y);
+            if (h + u * step < nk) kv_store8(vc + u * c_inc, y);
         }
     }
 }
@@ -231,10 +272,11 @@ int kv_append_launch(const KvView &c, const KvBatch &b, int hd, int ti, int tc, 
                                                                                   : append_kernel<128, QT_BF16>(tc))
                          : (ti == QT_F32 ? append_kernel<64, QT_F32>(tc) : ti == QT_F16 ? append_kernel<64, QT_F16>(tc)
                                                                                  : append_kernel<64, QT_BF16>(tc));
-    // few tokens: their heads over several warps, until the GPU has 16 warps an SM
-    const int hw = 256 / hd, passes = (nh + 2 * c.n_kv_heads + hw - 1) / hw;
-    const int parts = 16 * sms / b.n_tokens;
-    a.parts = parts < 1 ? 1 : parts > passes ? passes : parts;
+    // a token's heads over several warps until the GPU has four waves of them (8192 tokens
+    // of 48 heads: 53 us in 1.7 waves), at most a pass each
+    const int hw = 256 / hd, passes = (nh + hw - 1) / hw + 2 * ((c.n_kv_heads + hw - 1) / hw);
+    const int parts = (4 * 24 * sms + b.n_tokens - 1) / b.n_tokens;
+    a.parts = parts > passes ? passes : parts;
     const long long warps = static_cast<long long>(b.n_tokens) * a.parts;
     void *args[] = {&a};
     return kv_launch(fn, dim3(static_cast<unsigned>((warps + 7) / 8)), 256, 0, args, st);
