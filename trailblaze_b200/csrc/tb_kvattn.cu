@@ -121,18 +121,21 @@ __device__ __forceinline__ KvSlices kv_slices(const KvSeq &q, int window, int si
 }
 
 struct FewShared {
-    float m[4][8], l[4][8];   // [warp][row]
-    unsigned long long scan[4], at;
+    float m[8][8], l[8][8];   // [warp][row]
+    unsigned long long scan[8], at;
     int seq, fail, last, bad[8];
 };
 
 template <int HD, int TI, int TC>
 struct FewCfg {
     static constexpr int ES = TC == QT_F32 ? 4 : 2;
-    static constexpr int W = 4;                                 // warps
-    static constexpr int SB = 2 * kSlice * HD * ES;             // bytes of a slice, K and V
-    static constexpr int NST = SB >= 16384 ? 3 : SB >= 8192 ? 3 : 6;
-    static constexpr int CTAS = SB >= 16384 ? 1 : 2;            // per SM
+    static constexpr int SB = kSlice * HD * ES;                 // bytes of a slice of K or of V
+    // 8 warps on one CTA an SM for the slices that take the most arithmetic a byte's
+    // copy (fp32, 128 dimensions), else two CTAs of 4: one streams while the other
+    // joins its warps.  24 KB a warp in flight either way.
+    static constexpr int W = SB >= 8192 ? 8 : 4;                // warps
+    static constexpr int CTAS = SB >= 8192 ? 1 : 2;             // per SM
+    static constexpr int NST = SB >= 8192 ? 3 : SB >= 4096 ? 6 : 12;
     static constexpr int NQ = TC == QT_F32 ? 2 : TI == TC ? 1 : TC == QT_BF16 ? 3 : 2;
     static constexpr int NP = TC == QT_BF16 && TI == QT_F32 ? 3 : 2;
     static constexpr int MERGE = W * 8 * HD * 4;
@@ -196,7 +199,7 @@ __global__ void __launch_bounds__(FewCfg<HD, TI, TC>::W * 32, FewCfg<HD, TI, TC>
     constexpr int NC = FINE ? 5 : 2;             // accumulators of a score: 4 and the small products', or 2
     constexpr int KS = X32 ? HD / 8 : HD / 16;   // steps of the product over the head's dimensions
     constexpr int CB = HD * ES / 128;            // 128-byte columns of a row
-    constexpr uint32_t kCol = kSlice * 128, kTile = CB * kCol;
+    constexpr uint32_t kCol = kSlice * 128;
     extern __shared__ __align__(1024) uint8_t sm[];
     float *merge = reinterpret_cast<float *>(sm + W * NST * Cfg::SB);   // [W][8][HD]
     uint64_t *full = reinterpret_cast<uint64_t *>(merge + Cfg::MERGE / 4);
@@ -277,10 +280,26 @@ __global__ void __launch_bounds__(FewCfg<HD, TI, TC>::W * 32, FewCfg<HD, TI, TC>
     const uint32_t bars = smem_u32(full) + warp * NST * 8;
     KvCur ic = cu;                              // the next step to be requested
     unsigned long long iu = u0;
-    uint32_t issued = 0, taken = 0, hidden = 0; // slices requested / consumed; hidden: stages whose page is outside the pool
-    int pg = -1, pg_s = -1, pg_base = 0;   // lane l: the page of the warp's slice in step pg_base + l
-    bool ok = true;
-    auto issue_one = [&]() {   // requests the warp's slice of step iu, if it has one
+    uint32_t issued = 0, taken = 0;             // tiles (K and V of a slice in turn) requested / consumed
+    uint32_t hidden = 0;                        // bit st: stage st's page is outside the pool
+    int pg = -1, pg_s = -1, pg_base = 0;        // lane l: the page of the warp's slice in step pg_base + l
+    int cy = 0, cz = 0, cw = 0;                 // the last slice's coordinates
+    bool v_due = false, cbad = false, ok = true;
+    auto request = [&](const CUtensorMap *map) {
+        const uint32_t st = issued % NST, bar = bars + st * 8, dst = ring + st * Cfg::SB;
+        hidden = cbad ? hidden | (1u << st) : hidden & ~(1u << st);
+        if (lane == 0) {
+            if (cbad) {
+                mbar_arrive(bar);
+            } else {
+                mbar_expect_tx(bar, Cfg::SB);
+#pragma unroll
+                for (int cb = 0; cb < CB; ++cb) tma_load_4d(dst + cb * kCol, map, cb * (128 / ES), cy, cz, cw, bar);
+            }
+        }
+        ++issued;
+    };
+    auto issue_step = [&]() {   // K of the warp's slice of step iu, if it has one
         const int sl = ic.step * W + warp;
         if (sl < ic.sl.n) {
             if (ic.s != pg_s || ic.step >= pg_base + 32 || ic.step < pg_base) {
@@ -296,32 +315,28 @@ __global__ void __launch_bounds__(FewCfg<HD, TI, TC>::W * 32, FewCfg<HD, TI, TC>
             const int page = __shfl_sync(0xFFFFFFFFu, pg, ic.step - pg_base);
             const int j = (sl < ic.sl.ns ? sl : sl - ic.sl.ns + ic.sl.lo) * kSlice;
             const int pos = j - static_cast<int>(fdiv(static_cast<uint32_t>(j), a.c.page_div)) * a.c.page_size;
-            const uint32_t st = issued % NST, bar = bars + st * 8, dst = ring + st * Cfg::SB;
-            const bool bad = page < 0 || page >= a.c.n_pages;
-            hidden = bad ? hidden | (1u << st) : hidden & ~(1u << st);
-            if (lane == 0) {
-                const int y = a.ax_pos == 0 ? pos : a.ax_head == 0 ? ic.h : page;
-                const int z = a.ax_pos == 1 ? pos : a.ax_head == 1 ? ic.h : page;
-                const int w = a.ax_pos == 2 ? pos : a.ax_head == 2 ? ic.h : page;
-                if (bad) {
-                    atomicExch(a.err, ERR_RUNTIME);
-                    mbar_arrive(bar);
-                } else {
-                    mbar_expect_tx(bar, Cfg::SB);
-#pragma unroll
-                    for (int cb = 0; cb < CB; ++cb) {
-                        tma_load_4d(dst + cb * kCol, &kmap, cb * (128 / ES), y, z, w, bar);
-                        tma_load_4d(dst + kTile + cb * kCol, &vmap, cb * (128 / ES), y, z, w, bar);
-                    }
-                }
-            }
-            ++issued;
+            cbad = page < 0 || page >= a.c.n_pages;
+            if (cbad && lane == 0) atomicExch(a.err, ERR_RUNTIME);
+            cy = a.ax_pos == 0 ? pos : a.ax_head == 0 ? ic.h : page;
+            cz = a.ax_pos == 1 ? pos : a.ax_head == 1 ? ic.h : page;
+            cw = a.ax_pos == 2 ? pos : a.ax_head == 2 ? ic.h : page;
+            request(&kmap);
+            v_due = true;
         }
         ++iu;
         if (++ic.step == ic.steps && iu < u1) advance_item(ic);
     };
     auto refill = [&]() {
-        while (ok && iu < u1 && issued - taken < NST) issue_one();
+        while (ok && issued - taken < NST) {
+            if (v_due) {
+                request(&vmap);
+                v_due = false;
+            } else if (iu < u1) {
+                issue_step();
+            } else {
+                break;
+            }
+        }
     };
     refill();
 
@@ -406,7 +421,8 @@ __global__ void __launch_bounds__(FewCfg<HD, TI, TC>::W * 32, FewCfg<HD, TI, TC>
         for (int k = 0; k < nstep; ++k) {
             const int sl = (step0 + k) * W + warp;
             if (sl < cu.sl.n && ok) {
-                const uint32_t st = taken % NST, kb = ring + st * Cfg::SB, vb = kb + kTile;
+                uint32_t st = taken % NST;
+                const uint32_t kb = ring + st * Cfg::SB;
                 const int j0 = (sl < cu.sl.ns ? sl : sl - cu.sl.ns + cu.sl.lo) * kSlice;
                 ok = mbar_wait_bounded(bars + st * 8, (taken / NST) & 1u, a.err, a.wait_limit);
                 ok = __all_sync(0xFFFFFFFFu, ok);
@@ -415,17 +431,6 @@ __global__ void __launch_bounds__(FewCfg<HD, TI, TC>::W * 32, FewCfg<HD, TI, TC>
                     break;
                 }
                 const bool bad = (hidden >> st) & 1u;
-                if (j0 + kSlice > cu.q.len && !bad) {
-                    // positions that no one wrote: whatever V holds there, 0 * it has to be 0
-                    const int r1 = cu.q.len - j0;
-                    for (int i = lane; i < (kSlice - r1) * (HD * ES / 16); i += 32) {
-                        const int r = r1 + i / (HD * ES / 16), c = i % (HD * ES / 16);
-                        const uint32_t at = vb + (c >> 3) * kCol + r * 128 + ((c & 7) << 4);
-                        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory");
-                    }
-                    fence_proxy_async_smem();   // before the stage's next copy
-                    __syncwarp();
-                }
                 // ---- S^T = K Q^T; the tensor core truncates what it adds to an accumulator, so
                 // fp32 results come from short chains that are added in fp32, the small
                 // products by themselves ----
@@ -452,6 +457,9 @@ __global__ void __launch_bounds__(FewCfg<HD, TI, TC>::W * 32, FewCfg<HD, TI, TC>
                             mma16<TC>(c[n > 0 ? NC - 1 : FINE ? ks & 3 : ks & 1], x, qf[n][ks][0], qf[n][ks][1]);
                     }
                 }
+                __syncwarp();   // every lane has read K
+                ++taken;
+                refill();
                 float x[4];   // (position g, row 2 t), (g, 2 t + 1), (g + 8, 2 t), (g + 8, 2 t + 1)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
@@ -489,6 +497,26 @@ __global__ void __launch_bounds__(FewCfg<HD, TI, TC>::W * 32, FewCfg<HD, TI, TC>
                 l[0] += x[0] + x[2];
                 l[1] += x[1] + x[3];
                 // ---- O^T += V^T P^T ----
+                st = taken % NST;
+                const uint32_t vb = ring + st * Cfg::SB;
+                ok = mbar_wait_bounded(bars + st * 8, (taken / NST) & 1u, a.err, a.wait_limit);
+                ok = __all_sync(0xFFFFFFFFu, ok);
+                if (!ok) {
+                    sh.fail = 1;
+                    break;
+                }
+                if (bad || j0 + kSlice > cu.q.len) {
+                    // positions that no one wrote (all of them where the page is none): whatever
+                    // lies there, 0 * it has to be 0
+                    const int r1 = bad ? 0 : cu.q.len - j0;
+                    for (int i = lane; i < (kSlice - r1) * (HD * ES / 16); i += 32) {
+                        const int r = r1 + i / (HD * ES / 16), c = i % (HD * ES / 16);
+                        const uint32_t at = vb + (c >> 3) * kCol + r * 128 + ((c & 7) << 4);
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory");
+                    }
+                    fence_proxy_async_smem();   // before the stage's next copy
+                    __syncwarp();
+                }
                 if constexpr (X32) {
                     uint32_t ph[2][2], pl[2][2];   // [8 positions][2 t and 2 t + 1 of them, row g]
 #pragma unroll
@@ -551,7 +579,7 @@ __global__ void __launch_bounds__(FewCfg<HD, TI, TC>::W * 32, FewCfg<HD, TI, TC>
                         }
                     }
                 }
-                __syncwarp();   // every lane has read the stage
+                __syncwarp();   // every lane has read V
                 ++taken;
                 refill();
             }
@@ -687,7 +715,7 @@ __global__ void __launch_bounds__(FewCfg<HD, TI, TC>::W * 32, FewCfg<HD, TI, TC>
                     for (int d = 0; d < PER; ++d) acc[d] *= f0;
                     M = Mn;
                     if (mr < rows) {
-                        constexpr int AHEAD = 4;
+                        constexpr int AHEAD = 8;
                         for (int i0 = 0; i0 < n; i0 += AHEAD) {
                             float4 v[AHEAD][PER / 4];
 #pragma unroll
