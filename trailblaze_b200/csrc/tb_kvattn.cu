@@ -10,8 +10,9 @@
 // each of the CTA's W warps.  All items' steps, laid end to end, are cut into
 // equal parts, one per CTA, whatever the sequences' lengths: a CTA works through
 // the end of one item, whole items, and the beginning of another.  Items that lie
-// in one CTA are written out directly, the others' parts go to the workspace and
-// the last CTA to arrive adds them in CTA order, so results repeat bit for bit.
+// in one CTA are written out directly, the others' parts go through the workspace to
+// the CTA that has the item's beginning, which adds them in CTA order, so results
+// repeat bit for bit.
 //
 // Each warp streams its own slices of K and V through its own ring of TMA copies
 // (128-byte swizzle, one mbarrier a stage), with no CTA barrier inside an item.
@@ -122,8 +123,8 @@ __device__ __forceinline__ KvSlices kv_slices(const KvSeq &q, int window, int si
 
 struct FewShared {
     float m[8][8], l[8][8];   // [warp][row]
-    unsigned long long scan[8], at;
-    int seq, fail, last, bad[8];
+    unsigned long long scan[8], items[8], at;
+    int seq, fail, bad[8];
 };
 
 template <int HD, int TI, int TC>
@@ -136,6 +137,7 @@ struct FewCfg {
     static constexpr int W = SB >= 8192 ? 8 : 4;                // warps
     static constexpr int CTAS = SB >= 8192 ? 1 : 2;             // per SM
     static constexpr int NST = SB >= 8192 ? 3 : SB >= 4096 ? 6 : 12;
+    static constexpr int MIN = SB >= 8192 ? 2 : 4;              // steps of a CTA, at least
     static constexpr int NQ = TC == QT_F32 ? 2 : TI == TC ? 1 : TC == QT_BF16 ? 3 : 2;
     static constexpr int NP = TC == QT_BF16 && TI == QT_F32 ? 3 : 2;
     static constexpr int MERGE = W * 8 * HD * 4;
@@ -173,7 +175,7 @@ __device__ __forceinline__ void kv_cur_seq(const AttnArgs &a, KvCur &c)
 }
 
 template <int W>
-__device__ __forceinline__ unsigned long long kv_seq_steps(const AttnArgs &a, int s, bool &bad)
+__device__ __forceinline__ unsigned long long kv_seq_steps(const AttnArgs &a, int s, bool &bad, unsigned long long *items)
 {
     KvSeq q;
     if (!kv_seq(a.b, a.c, s, q, nullptr)) {
@@ -183,6 +185,7 @@ __device__ __forceinline__ unsigned long long kv_seq_steps(const AttnArgs &a, in
     if (!few_seq(a, q)) return 0;
     const KvSlices sl = kv_slices(q, a.window, a.sinks);
     const unsigned long long tiles = (static_cast<unsigned long long>(q.n) * a.group + 7) >> 3;
+    if (items) *items += tiles * a.c.n_kv_heads;
     return tiles * a.c.n_kv_heads * static_cast<unsigned>((sl.n + W - 1) / W);
 }
 
@@ -221,9 +224,9 @@ __global__ void __launch_bounds__(FewCfg<HD, TI, TC>::W * 32, FewCfg<HD, TI, TC>
     asm volatile("griddepcontrol.wait;" ::: "memory");
     // ---- this CTA's share of all steps: a scan over the sequences ----
     const int per = (a.b.n_seqs + T - 1) / T, sq0 = tid * per, sq1 = min(a.b.n_seqs, sq0 + per);
-    unsigned long long mine = 0;
+    unsigned long long mine = 0, items = 0;
     bool bad_seq = false;
-    for (int s = sq0; s < sq1; ++s) mine += kv_seq_steps<W>(a, s, bad_seq);
+    for (int s = sq0; s < sq1; ++s) mine += kv_seq_steps<W>(a, s, bad_seq, &items);
     if (__syncthreads_or(bad_seq) && blockIdx.x == 0) kv_zero_bad<HD, I>(a);
     unsigned long long incl = mine;
 #pragma unroll
@@ -231,21 +234,31 @@ __global__ void __launch_bounds__(FewCfg<HD, TI, TC>::W * 32, FewCfg<HD, TI, TC>
         const unsigned long long x = __shfl_up_sync(0xFFFFFFFFu, incl, o);
         if (lane >= o) incl += x;
     }
-    if (lane == 31) sh.scan[warp] = incl;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) items += __shfl_xor_sync(0xFFFFFFFFu, items, o);
+    if (lane == 31) sh.scan[warp] = incl, sh.items[warp] = items;
     __syncthreads();
-    unsigned long long before = incl - mine, total = 0;
+    unsigned long long before = incl - mine, total = 0, all_items = 0;
 #pragma unroll
     for (int w = 0; w < W; ++w) {
+        all_items += sh.items[w];
         before += w < warp ? sh.scan[w] : 0;
         total += sh.scan[w];
     }
-    const unsigned G = total < gridDim.x ? static_cast<unsigned>(total) : gridDim.x, cta = blockIdx.x;
-    if (cta >= G) return;
-    const unsigned long long u0 = total * cta / G, u1 = total * (cta + 1) / G;
+    // A CTA for every item, or more, with at least MIN steps each (128 KB of the cache):
+    // finer cuts gain less than the joining of their parts costs.
+    if (total == 0) return;
+    const unsigned long long most = min(max(all_items, (total + Cfg::MIN - 1) / Cfg::MIN), static_cast<unsigned long long>(gridDim.x));
+    const unsigned long long longest = kv_div(total + most - 1, most);
+    const unsigned G = static_cast<unsigned>(kv_div(total + longest - 1, longest));
+    if (blockIdx.x >= G) return;
+    const unsigned cta = G - 1 - blockIdx.x;   // of the steps, against blockIdx: see the joining of parts
+    const KvShare share(total, G);
+    const unsigned long long u0 = share.start(cta), u1 = share.start(cta + 1);
     if (before <= u0 && u0 < before + mine) {
         unsigned long long at = before;
         for (int s = sq0; s < sq1; ++s) {
-            const unsigned long long n = kv_seq_steps<W>(a, s, bad_seq);
+            const unsigned long long n = kv_seq_steps<W>(a, s, bad_seq, nullptr);
             if (u0 < at + n) {
                 sh.seq = s;
                 sh.at = u0 - at;
@@ -260,10 +273,10 @@ __global__ void __launch_bounds__(FewCfg<HD, TI, TC>::W * 32, FewCfg<HD, TI, TC>
     cu.s = sh.seq;
     kv_cur_seq<W>(a, cu);
     {
-        const unsigned long long r = sh.at, item = r / cu.steps;
-        cu.step = static_cast<int>(r % cu.steps);
-        cu.rt = static_cast<int>(item % cu.tiles);
-        cu.h = static_cast<int>(item / cu.tiles);
+        const unsigned long long r = sh.at, item = kv_div(r, cu.steps), head = kv_div(item, cu.tiles);
+        cu.step = static_cast<int>(r - item * cu.steps);
+        cu.rt = static_cast<int>(item - head * cu.tiles);
+        cu.h = static_cast<int>(head);
     }
     auto advance_item = [&](KvCur &c) {
         c.step = 0;
@@ -324,7 +337,18 @@ __global__ void __launch_bounds__(FewCfg<HD, TI, TC>::W * 32, FewCfg<HD, TI, TC>
             v_due = true;
         }
         ++iu;
-        if (++ic.step == ic.steps && iu < u1) advance_item(ic);
+        if (++ic.step == ic.steps && iu < u1) {
+            advance_item(ic);
+            // its Q towards L2 while this item still runs: a row's bytes by 128 a lane
+            constexpr int LINES = HD * static_cast<int>(sizeof(I)) / 128;
+            const int r = ic.rt * 8 + lane / LINES;
+            if (lane < 8 * LINES && r < ic.q.n * a.group) {
+                const int tok = r / a.group;
+                const I *qp = static_cast<const I *>(a.q.p) + (ic.q.row0 + tok) * a.q.row +
+                              (ic.h * a.group + (r - tok * a.group)) * a.q.head + (lane % LINES) * (128 / sizeof(I));
+                asm volatile("prefetch.global.L2 [%0];" ::"l"(qp));
+            }
+        }
     };
     auto refill = [&]() {
         while (ok && issued - taken < NST) {
@@ -338,8 +362,16 @@ __global__ void __launch_bounds__(FewCfg<HD, TI, TC>::W * 32, FewCfg<HD, TI, TC>
             }
         }
     };
-    refill();
-
+    int tell = -1;   // the CTA that waits for this one's part
+    auto told = [&]() {   // each warp for its stores
+        __syncwarp();
+        if (lane == 0) {
+            __threadfence();
+            atomicAdd(a.arrived + tell, 1u);
+        }
+        __syncwarp();
+        tell = -1;
+    };
     const uint32_t krow = (lane & 7) + ((lane >> 3) & 1) * 8, kchunk = lane >> 4;   // ldmatrix rows of K
     const uint32_t vrow = (lane & 7) + (lane >> 4) * 8, vchunk = (lane >> 3) & 1;   // and of V, transposed
     for (unsigned long long u = u0; u < u1;) {
@@ -350,58 +382,68 @@ __global__ void __launch_bounds__(FewCfg<HD, TI, TC>::W * 32, FewCfg<HD, TI, TC>
         const int nstep = left < static_cast<unsigned>(cu.steps - cu.step) ? static_cast<int>(left) : cu.steps - cu.step;
         const bool to_end = cu.step + nstep == cu.steps;
         const int R = cu.q.n * a.group, p0 = cu.q.len - cu.q.n, r0 = cu.rt * 8;
-        // row g of Q as the B operand; rows past the last are zero
+        // row g of Q as the B operand; rows past the last are zero.  It is requested before
+        // the ring's copies, behind which it would wait.
         uint32_t qf[NQ][KS][2];
         float rscale = a.scale2;
         {
+            constexpr int QE = X32 ? 2 : 4;   // elements of a step
             const int r = r0 + g, tok = r / a.group;
             const bool on = r < R;
             const I *qp = static_cast<const I *>(a.q.p) + (cu.q.row0 + (on ? tok : 0)) * a.q.row +
                           (cu.h * a.group + (on ? r - tok * a.group : 0)) * a.q.head;
-            if constexpr (X32) {
-#pragma unroll
-                for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const float x = on ? kv_f(qp[ks * 8 + t + 4 * e]) : 0.f;
-                        split_tf32(__float_as_uint(x), qf[0][ks][e], qf[1][ks][e]);
-                    }
-            } else if constexpr (NQ == 1) {
+            if constexpr (NQ == 1) {
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
                     for (int e = 0; e < 2; ++e)
                         qf[0][ks][e] = on ? *reinterpret_cast<const uint32_t *>(qp + ks * 16 + 2 * t + 8 * e) : 0u;
+                refill();
             } else {
-                float x[KS][4], big = 0.f;
+                I x[KS][QE];
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        x[ks][e] = on ? kv_f(qp[ks * 16 + 2 * t + 8 * (e >> 1) + (e & 1)]) : 0.f;
-                        big = fmaxf(big, fabsf(x[ks][e]));
+                    for (int e = 0; e < QE; ++e)
+                        x[ks][e] = qp[X32 ? ks * 8 + t + 4 * e : ks * 16 + 2 * t + 8 * (e >> 1) + (e & 1)];
+                refill();
+                float y[KS][QE], big = 0.f;
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                    for (int e = 0; e < QE; ++e) {
+                        y[ks][e] = on ? kv_f(x[ks][e]) : 0.f;
+                        big = fmaxf(big, fabsf(y[ks][e]));
                     }
-                if constexpr (TC == QT_F16) {   // the row times 2^k, its largest element near 2^13
-                    big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 1));
-                    big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 2));
-                    int k = 0;
-                    if (big > 0.f && big < INFINITY) k = 13 - ilogbf(big);
-                    k = max(-100, min(100, k));
-                    const float up = ldexpf(1.f, k);
-                    rscale = ldexpf(a.scale2, -k);
+                if constexpr (X32) {
 #pragma unroll
                     for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) x[ks][e] *= up;
+                        for (int e = 0; e < 2; ++e) split_tf32(__float_as_uint(y[ks][e]), qf[0][ks][e], qf[1][ks][e]);
+                } else {
+                    if constexpr (TC == QT_F16) {   // the row times 2^k, its largest element near 2^13
+                        big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 1));
+                        big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 2));
+                        int k = 0;
+                        if (big > 0.f && big < INFINITY) k = 13 - ilogbf(big);
+                        k = max(-100, min(100, k));
+                        const float up = ldexpf(1.f, k);
+                        rscale = ldexpf(a.scale2, -k);
+#pragma unroll
+                        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                            for (int e = 0; e < QE; ++e) y[ks][e] *= up;
+                    }
+#pragma unroll
+                    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e)
+#pragma unroll
+                            for (int n = 0; n < NQ; ++n) qf[n][ks][e] = pack16<TC>(y[ks][2 * e], y[ks][2 * e + 1]);
                 }
-#pragma unroll
-                for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e)
-#pragma unroll
-                        for (int n = 0; n < NQ; ++n) qf[n][ks][e] = pack16<TC>(x[ks][2 * e], x[ks][2 * e + 1]);
             }
         }
+        if (tell >= 0) told();
         // columns 2 t and 2 t + 1 of S^T and O^T: their positions (-1: no row) and scales
         int pos[2];
         float rs[2];
@@ -674,81 +716,89 @@ __global__ void __launch_bounds__(FewCfg<HD, TI, TC>::W * 32, FewCfg<HD, TI, TC>
                 for (int d = 0; d < PER; ++d) kv_store1(op + d, acc[d]);
             }
         };
-        if (from_start && to_end) {
-            write_out();
-        } else {
-            // ---- the CTAs' parts: the last to arrive adds them, in CTA order ----
-            constexpr int P = few_part(HD);
-            const unsigned long long i0 = u - step0, i1 = i0 + cu.steps;   // the item's steps
-            const unsigned c0 = static_cast<unsigned>(((i0 + 1) * G - 1) / total);
-            const unsigned c1 = static_cast<unsigned>((i1 * G - 1) / total);
-            float *mp = a.part + static_cast<size_t>(2 * cta + (from_start ? 1 : 0)) * P;
+        constexpr int P = few_part(HD);
+        if (!from_start) {
+            // ---- not the item's beginning: the part goes to the CTA that has it ----
+            float *mp = a.part + static_cast<size_t>(cta) * P;
             if (mr < rows) {
 #pragma unroll
                 for (int d = 0; d < PER; d += 4)
-                    *reinterpret_cast<float4 *>(mp + mr * HD + md + d) = make_float4(acc[d], acc[d + 1], acc[d + 2], acc[d + 3]);
-                if (md == 0) mp[8 * HD + mr] = M, mp[8 * HD + 8 + mr] = L;
+                    __stcg(reinterpret_cast<float4 *>(mp + mr * HD + md + d),
+                           make_float4(acc[d], acc[d + 1], acc[d + 2], acc[d + 3]));
+                if (md == 0) __stcg(mp + 8 * HD + mr, M), __stcg(mp + 8 * HD + 8 + mr, L);
             }
-            __threadfence();
-            __syncthreads();
-            if (tid == 0) sh.last = atomicInc(a.arrived + c0, c1 - c0) == c1 - c0;   // wraps back to zero
-            __syncthreads();
-            if (sh.last) {
-                __threadfence();
-                // m and l of every part in one go, then the sums with several loads ahead
-                constexpr int BATCH = Cfg::MERGE / 4 / 16;
-                float *ml = merge;   // [part][8 m, 8 l]
-                auto pbase = [&](unsigned c) { return a.part + static_cast<size_t>(2 * c + (c == c0 ? 1 : 0)) * P; };
-                M = -INFINITY, L = 0.f;
+            // the stores are under way; that they have arrived is told later
+            tell = static_cast<int>(share.of(u - step0));
+        } else {
+            if (!to_end) {
+                // ---- the beginning: the other parts, of the CTAs after this one, in order.  They
+                // are waited for (as every wait, within a limit): the ranges run against blockIdx,
+                // so those CTAs were started before this one. ----
+                const unsigned others = share.of(u + cu.steps - 1) - cta;
+                const float *part = a.part + static_cast<size_t>(cta + 1) * P;
+                if (tid == 0) {
+                    uint32_t i = 0;
+                    unsigned n = 0;
+                    do {
+                        asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(n) : "l"(a.arrived + cta) : "memory");
+                    } while (n < W * others && ++i < a.wait_limit);
+                    if (n < W * others) {
+                        atomicExch(a.err, ERR_WAIT_TIMEOUT);
+                        sh.fail = 1;
+                    }
+                    a.arrived[cta] = 0;   // zero between calls
+                    __threadfence();
+                }
+                __syncthreads();
+                if (mr < rows) {
+                    constexpr int AHEAD = 64 / PER;   // parts whose loads are in flight together
+                    for (unsigned i0 = 0; i0 < others; i0 += AHEAD) {
+                        float4 v[AHEAD][PER / 4];
+                        float pm[AHEAD], pl[AHEAD];
 #pragma unroll
-                for (int d = 0; d < PER; ++d) acc[d] = 0.f;
-                for (unsigned cb = c0; cb <= c1; cb += BATCH) {
-                    const int n = min(static_cast<int>(c1 - cb + 1), BATCH);
-                    __syncthreads();
-                    for (int i = tid; i < n * 16; i += T) ml[i] = __ldcg(pbase(cb + i / 16) + 8 * HD + i % 16);
-                    __syncthreads();
-                    float Mn = M;
-                    for (int i = 0; i < n; ++i) Mn = fmaxf(Mn, ml[i * 16 + mr]);
-                    const float f0 = M == -INFINITY ? 0.f : ex2(M - Mn);
-                    L = M == -INFINITY ? L : L * f0;
+                        for (int i = 0; i < AHEAD; ++i) {
+                            const float *pp = part + (i0 + i) * P;
+                            pm[i] = -INFINITY, pl[i] = 0.f;
+                            if (i0 + i < others) {
+                                pm[i] = __ldcg(pp + 8 * HD + mr);
+                                pl[i] = __ldcg(pp + 8 * HD + 8 + mr);
 #pragma unroll
-                    for (int d = 0; d < PER; ++d) acc[d] *= f0;
-                    M = Mn;
-                    if (mr < rows) {
-                        constexpr int AHEAD = 8;
-                        for (int i0 = 0; i0 < n; i0 += AHEAD) {
-                            float4 v[AHEAD][PER / 4];
+                                for (int d = 0; d < PER / 4; ++d)
+                                    v[i][d] = __ldcg(reinterpret_cast<const float4 *>(pp + mr * HD + md) + d);
+                            }
+                        }
+                        float Mn = M;
 #pragma unroll
-                            for (int i = 0; i < AHEAD; ++i)
-                                if (i0 + i < n)
+                        for (int i = 0; i < AHEAD; ++i) Mn = fmaxf(Mn, pm[i]);
+                        const float f0 = M == -INFINITY ? 0.f : ex2(M - Mn);
+                        L = M == -INFINITY ? L : L * f0;
 #pragma unroll
-                                    for (int d = 0; d < PER / 4; ++d)
-                                        v[i][d] = __ldcg(reinterpret_cast<const float4 *>(pbase(cb + i0 + i) + mr * HD + md) + d);
+                        for (int d = 0; d < PER; ++d) acc[d] *= f0;
+                        M = Mn;
 #pragma unroll
-                            for (int i = 0; i < AHEAD; ++i) {
-                                if (i0 + i >= n) break;
-                                const float pm = ml[(i0 + i) * 16 + mr], pl = ml[(i0 + i) * 16 + 8 + mr];
-                                const float f = pm == -INFINITY ? 0.f : ex2(pm - M);
-                                L += pm == -INFINITY ? pl : f * pl;
+                        for (int i = 0; i < AHEAD; ++i) {
+                            if (i0 + i >= others) break;
+                            const float f = pm[i] == -INFINITY ? 0.f : ex2(pm[i] - M);
+                            L += pm[i] == -INFINITY ? pl[i] : f * pl[i];
 #pragma unroll
-                                for (int d = 0; d < PER / 4; ++d) {
-                                    acc[4 * d] = fmaf(f, v[i][d].x, acc[4 * d]);
-                                    acc[4 * d + 1] = fmaf(f, v[i][d].y, acc[4 * d + 1]);
-                                    acc[4 * d + 2] = fmaf(f, v[i][d].z, acc[4 * d + 2]);
-                                    acc[4 * d + 3] = fmaf(f, v[i][d].w, acc[4 * d + 3]);
-                                }
+                            for (int d = 0; d < PER / 4; ++d) {
+                                acc[4 * d] = fmaf(f, v[i][d].x, acc[4 * d]);
+                                acc[4 * d + 1] = fmaf(f, v[i][d].y, acc[4 * d + 1]);
+                                acc[4 * d + 2] = fmaf(f, v[i][d].z, acc[4 * d + 2]);
+                                acc[4 * d + 3] = fmaf(f, v[i][d].w, acc[4 * d + 3]);
                             }
                         }
                     }
                 }
-                write_out();
             }
+            write_out();
         }
         u += nstep;
         cu.step += nstep;
         if (u < u1) advance_item(cu);
         __syncthreads();   // merge and sh are free again
     }
+    if (tell >= 0) told();
     // after a wait that ran out: the copies still in flight, as far as they come
     while (!ok && taken < issued) {
         mbar_wait_bounded(bars + (taken % NST) * 8, (taken / NST) & 1u, a.err, a.wait_limit);
@@ -760,12 +810,12 @@ __global__ void __launch_bounds__(FewCfg<HD, TI, TC>::W * 32, FewCfg<HD, TI, TC>
 // host side
 // ---------------------------------------------------------------------------
 // Workspace: the arrival counters (the part that stays zero between calls), then
-// the partial results, two a CTA.
+// the partial results, one a CTA.
 static constexpr int kMaxCtas = 512;
 static constexpr size_t kCounterBytes = kMaxCtas * sizeof(unsigned);
 size_t kv_attend_ws()
 {
-    const size_t few = sizeof(float) * 2 * kMaxCtas * few_part(128), many = kManyCtas * kv_many_part_bytes();
+    const size_t few = sizeof(float) * kMaxCtas * few_part(128), many = kManyCtas * kv_many_part_bytes();
     return kCounterBytes + (few > many ? few : many);
 }
 

@@ -19,7 +19,7 @@ struct AttnArgs {
     int *err;
     uint32_t wait_limit;
     int ax_pos, ax_head, ax_page;   // the tensor maps' axes 1..3: which of them is which
-    float *part;                    // [2 * gridDim.x] partial results
+    float *part;                    // [gridDim.x] partial results
     unsigned *arrived;              // [gridDim.x] arrival counters, zero between calls
     int many_rows;                  // k_kv_few: sequences of more rows are the other launch's
 };
@@ -48,6 +48,27 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map
                  "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
                  : "memory");
 }
+
+// Division of counts that are 64 bits wide by type and 32 by size: a 64-bit division
+// takes some hundred instructions, which a launch of a few microseconds sees.
+__device__ __forceinline__ unsigned long long kv_div(unsigned long long a, unsigned long long b)
+{
+    if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+    return a / b;
+}
+
+// total units of work in G parts that differ by one at most, the longer ones first.
+struct KvShare {
+    unsigned long long base;
+    unsigned rem;
+    __device__ __forceinline__ KvShare(unsigned long long total, unsigned G) : base(kv_div(total, G)), rem(static_cast<unsigned>(total - base * G)) {}
+    __device__ __forceinline__ unsigned long long start(unsigned c) const { return base * c + min(c, rem); }
+    __device__ __forceinline__ unsigned of(unsigned long long unit) const   // the part that holds a unit
+    {
+        const unsigned long long longer = (base + 1) * rem;
+        return static_cast<unsigned>(unit < longer ? kv_div(unit, base + 1) : rem + kv_div(unit - longer, base));
+    }
+};
 
 // The rows of sequences whose numbers contradict each other: the error word, and
 // zeros as far as the rows exist (one CTA, all its threads).

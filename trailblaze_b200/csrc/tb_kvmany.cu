@@ -327,9 +327,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         tmem_relinquish();
     }
     const unsigned cta = G - 1 - blockIdx.x;   // of the units, against blockIdx: see the joining of parts
-    const unsigned long long per_cta = total / G;
-    const unsigned extra = static_cast<unsigned>(total % G);
-    const unsigned long long u0 = per_cta * cta + extra * cta / G, u1 = per_cta * (cta + 1) + extra * (cta + 1) / G;
+    const KvShare share(total, G);
+    const unsigned long long u0 = share.start(cta), u1 = share.start(cta + 1);
     const bool mine_u0 = before <= u0 && u0 < before + mine;
     if (__any_sync(0xFFFFFFFFu, mine_u0)) {   // the warp whose sequences hold u0
         unsigned long long at = before;
@@ -348,7 +347,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         fq.n = __shfl_sync(0xFFFFFFFFu, fq.n, src);
         fq.len = __shfl_sync(0xFFFFFFFFu, fq.len, src);
         const unsigned long long r = __shfl_sync(0xFFFFFFFFu, fr, src), f = __shfl_sync(0xFFFFFFFFu, ff, src);
-        unsigned long long rem = r % f;   // units of the head before u0: the row tile, 32 at a time
+        const unsigned long long head = kv_div(r, f);
+        unsigned long long rem = r - head * f;   // units of the head before u0: the row tile, 32 at a time
         const int n_rt = (fq.n + 2 * a.tpt - 1) / (2 * a.tpt);
         for (int base = 0; base < n_rt; base += 32) {
             const unsigned long long k = base + lane < n_rt ? many_tiles(a, fq, base + lane, nullptr) : 0;
@@ -361,7 +361,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             const unsigned hit = __ballot_sync(0xFFFFFFFFu, rem < c);
             if (hit) {
                 if (lane == __ffs(hit) - 1) {
-                    sh.head = static_cast<int>(r / f);
+                    sh.head = static_cast<int>(head);
                     sh.rt = base + lane;
                     sh.off = static_cast<int>(rem - (c - k));
                 }
@@ -477,8 +477,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                     pt.row0 = it.q.row0, pt.len = it.q.len, pt.n = it.q.n, pt.t0 = it.t0;
                     pt.t1 = it.t1, pt.s = it.s, pt.h = it.h, pt.tiles = it.n;
                     pt.ns = it.ns, pt.lo = it.lo, pt.j0 = j0, pt.j1 = j1;
-                    pt.peer = j0 > 0 ? static_cast<unsigned>(((u - j0 + 1) * G - 1) / total)
-                                     : static_cast<unsigned>(((u + it.n) * G - 1) / total) - cta;
+                    pt.peer = j0 > 0 ? share.of(u - j0) : share.of(u + it.n - 1) - cta;
                 }
                 __syncwarp();
                 if (elect_one()) {
