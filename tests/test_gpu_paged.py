@@ -167,6 +167,17 @@ def test_nan_in_k_or_v_alone(paged, kq, io, which):
         assert bool(got[where:].all()) and not bool(got[:where].any()), where
 
 
+@pytest.mark.parametrize("io,cache", TYPES)
+def test_long_chunks_of_all_types(paged, kq, io, cache):
+    """Several row tiles and splits for every pair of types, negative scales among them."""
+    c = Case(paged, [150, 1, 37], [190, 100, 400], 6, 2, 64, io, cache, 48, seed=19)
+    c.check(c.cache.attend(1, c.batch, c.q, window=90, sinks=3), 90, 3)
+    c.check(c.cache.attend(1, c.batch, c.q, scale=-0.1), scale=-0.1)
+    c = Case(paged, [200], [700], 4, 1, 128, io, cache, 16, seed=20)
+    c.check(c.cache.attend(1, c.batch, c.q))
+    assert kq.tb_cuda_last_error() == 0
+
+
 def test_large_scores(paged, kq):
     """Scores up to some thousands: the running maximum keeps every exponent at or below zero."""
     c = Case(paged, [1, 33], [500, 100], 4, 2, 128, F32, F32, 16, seed=7)

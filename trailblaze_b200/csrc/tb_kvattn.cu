@@ -32,75 +32,6 @@
 
 namespace tb {
 
-// ---- PTX ----
-__device__ __forceinline__ void ldsm4(uint32_t a, uint32_t (&r)[4])
-{
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                 : "r"(a)
-                 : "memory");
-}
-__device__ __forceinline__ void ldsm4t(uint32_t a, uint32_t (&r)[4])
-{
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                 : "r"(a)
-                 : "memory");
-}
-__device__ __forceinline__ uint32_t mat_t(uint32_t x)   // transpose of an 8 x 8 matrix of 16-bit elements
-{
-    uint32_t y;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
-    return y;
-}
-template <int TC>
-__device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
-{
-    if constexpr (TC == QT_BF16)
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-                     "{%0, %1, %2, %3};"
-                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-    else
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-                     "{%0, %1, %2, %3};"
-                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
-{
-    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-                 "{%0, %1, %2, %3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-// x = hi + lo, hi rounded to tf32 (10 bits of mantissa); the tensor core reads
-// lo's upper 19 bits: what is lost lies 2^-21 below x and has no preferred sign.
-__device__ __forceinline__ void split_tf32(uint32_t x, uint32_t &hi, uint32_t &lo)
-{
-    hi = (x + 0x1000u) & 0xFFFFE000u;
-    lo = __float_as_uint(__uint_as_float(x) - __uint_as_float(hi));
-}
-// Two fp32 as a pair of 16-bit elements, and what the rounding left over.
-template <int TC>
-__device__ __forceinline__ uint32_t pack16(float &x, float &y)
-{
-    uint32_t w;
-    if constexpr (TC == QT_BF16) {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
-        w = *reinterpret_cast<const uint32_t *>(&h);
-        x -= __uint_as_float(w << 16);
-        y -= __uint_as_float(w & 0xFFFF0000u);
-    } else {
-        const __half2 h = __floats2half2_rn(x, y);
-        w = *reinterpret_cast<const uint32_t *>(&h);
-        const float2 f = __half22float2(h);
-        x -= f.x;
-        y -= f.y;
-    }
-    return w;
-}
-
 // ---- the layout of an item's positions ----
 static constexpr int kSlice = 16;
 
@@ -815,8 +746,10 @@ static constexpr int kMaxCtas = 512;
 static constexpr size_t kCounterBytes = kMaxCtas * sizeof(unsigned);
 size_t kv_attend_ws()
 {
-    const size_t few = sizeof(float) * kMaxCtas * few_part(128), many = kManyCtas * kv_many_part_bytes();
-    return kCounterBytes + (few > many ? few : many);
+    size_t n = sizeof(float) * kMaxCtas * few_part(128);
+    if (n < kManyCtas * kv_many_part_bytes()) n = kManyCtas * kv_many_part_bytes();
+    if (n < kManyCtas * kv_wide_part_bytes()) n = kManyCtas * kv_wide_part_bytes();
+    return kCounterBytes + n;
 }
 
 // Query rows per kv head up to which a sequence's attention is bound by the
@@ -867,16 +800,19 @@ int kv_attend_launch(const KvView &c, const KvBatch &b, int hd, int ti, int tc, 
     a.arrived = static_cast<unsigned *>(ws);
     a.part = reinterpret_cast<float *>(static_cast<char *>(ws) + kCounterBytes);
     a.many_rows = 0x7FFFFFFF;
-    // Chunks go to the tensor-core kernel: 16-bit activations over a cache of their
-    // type, whole groups of heads in 128 rows, and a scale that keeps the order of
-    // scores.  Where the batch holds short sequences besides, both kernels run and
-    // each takes its own; which sequences those are is decided on the device.
-    if (ti == tc && tc != QT_F32 && a.group <= 128 && scale > 0.f &&
-        static_cast<long long>(max_new) * a.group > kFewRows) {
+    // Chunks go to the kernels with 128-row tiles: the tcgen05 one for 16-bit
+    // activations over a cache of their type (whole tokens in 128 rows, a scale that
+    // keeps the order of scores), the other one else.  Where the batch holds short
+    // sequences besides, k_kv_few runs too and each takes its own; which sequences those
+    // are is decided on the device.
+    if (a.group <= 128 && static_cast<long long>(max_new) * a.group > kFewRows) {
         const bool mixed = b.n_tokens < static_cast<long long>(b.n_seqs) * max_new;
-        const int r = kv_many_launch(a, hd, tc, mixed ? kFewRows : 0, sms, st);
-        if (r == 0 || (r == 1 && !mixed)) return r;
-        if (r == 1) a.many_rows = kFewRows;
+        const int few_rows = mixed ? kFewRows : 0;
+        int r = -1;
+        if (ti == tc && tc != QT_F32 && scale > 0.f) r = kv_many_launch(a, hd, tc, few_rows, sms, st);
+        if (r < 0) r = kv_wide_launch(a, hd, ti, tc, few_rows, sms, st);
+        if (r == 0 || !mixed) return r;
+        a.many_rows = kFewRows;
     }
     return hd == 128 ? few<128>(a, ti, tc, sms, st) : few<64>(a, ti, tc, sms, st);
 }

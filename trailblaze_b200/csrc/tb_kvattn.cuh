@@ -29,6 +29,9 @@ struct AttnArgs {
 static constexpr int kManyCtas = 160;
 size_t kv_many_part_bytes();   // a partial result
 int kv_many_launch(AttnArgs a, int hd, int tc, int few_rows, int sms, cudaStream_t st);
+// The same of k_kv_wide (tb_kvwide.cu), for any types.
+size_t kv_wide_part_bytes();
+int kv_wide_launch(AttnArgs a, int hd, int ti, int tc, int few_rows, int sms, cudaStream_t st);
 
 __device__ __forceinline__ float ex2(float x)   // 2^x, 2 ulp; 0 for -inf
 {
@@ -70,6 +73,75 @@ struct KvShare {
     }
 };
 
+// ---- mma.sync and its operands ----
+__device__ __forceinline__ void ldsm4(uint32_t a, uint32_t (&r)[4])
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(a)
+                 : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t a, uint32_t (&r)[4])
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(a)
+                 : "memory");
+}
+__device__ __forceinline__ uint32_t mat_t(uint32_t x)   // transpose of an 8 x 8 matrix of 16-bit elements
+{
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+template <int TC>
+__device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+    if constexpr (TC == QT_BF16)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                     "{%0, %1, %2, %3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                     "{%0, %1, %2, %3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                 "{%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// x = hi + lo, hi rounded to tf32 (10 bits of mantissa); the tensor core reads
+// lo's upper 19 bits: what is lost lies 2^-21 below x and has no preferred sign.
+__device__ __forceinline__ void split_tf32(uint32_t x, uint32_t &hi, uint32_t &lo)
+{
+    hi = (x + 0x1000u) & 0xFFFFE000u;
+    lo = __float_as_uint(__uint_as_float(x) - __uint_as_float(hi));
+}
+// Two fp32 as a pair of 16-bit elements, and what the rounding left over.
+template <int TC>
+__device__ __forceinline__ uint32_t pack16(float &x, float &y)
+{
+    uint32_t w;
+    if constexpr (TC == QT_BF16) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+        w = *reinterpret_cast<const uint32_t *>(&h);
+        x -= __uint_as_float(w << 16);
+        y -= __uint_as_float(w & 0xFFFF0000u);
+    } else {
+        const __half2 h = __floats2half2_rn(x, y);
+        w = *reinterpret_cast<const uint32_t *>(&h);
+        const float2 f = __half22float2(h);
+        x -= f.x;
+        y -= f.y;
+    }
+    return w;
+}
+
 // The rows of sequences whose numbers contradict each other: the error word, and
 // zeros as far as the rows exist (one CTA, all its threads).
 template <int HD, class I>
@@ -87,6 +159,187 @@ __device__ void kv_zero_bad(const AttnArgs &a)
                       0.f);
         }
     }
+}
+
+// ---- row tiles by position tiles: how the chunk kernels cut their work ----
+// An item is (sequence, kv head, tpi of its new tokens); its units are tiles of TILE
+// positions.  All units end to end, in the order sequence, head, row tile, position,
+// are cut into equal parts, one a CTA.
+struct KvItem {
+    int s, h, rt;           // sequence, kv head, row tile
+    KvSeq q;
+    int n_rt;               // row tiles a head
+    int t0, t1;             // new tokens [t0, t1) of the sequence
+    int ns, lo, n;          // its position tiles: [0, ns) and [lo, lo + n - ns)
+};
+
+template <int TILE>
+__device__ __forceinline__ int kv_item_tiles(const AttnArgs &a, int tpi, const KvSeq &q, int rt, KvItem *it)
+{
+    const int t0 = rt * tpi, t1 = min(q.n, t0 + tpi), p0 = q.len - q.n;
+    const KvSpan sp = kv_span(p0 + t0, a.window, a.sinks);
+    const int hi = (p0 + t1 - 1) / TILE + 1;
+    int ns = 0, lo = 0, n = hi;
+    if (a.sinks < sp.lo) {
+        ns = (a.sinks + TILE - 1) / TILE;
+        lo = max(sp.lo / TILE, ns);
+        n = ns + hi - lo;
+    }
+    if (it) it->t0 = t0, it->t1 = t1, it->ns = ns, it->lo = lo, it->n = n;
+    return n;
+}
+template <int TILE>
+__device__ __forceinline__ int kv_item_pos(const KvItem &it, int j)
+{
+    return (j < it.ns ? j : j - it.ns + it.lo) * TILE;
+}
+// True for a sequence of this launch: one of more rows than few_rows.
+__device__ __forceinline__ bool kv_item_seq(const AttnArgs &a, int few_rows, int s, KvSeq &q)
+{
+    return kv_seq(a.b, a.c, s, q, nullptr) && static_cast<long long>(q.n) * a.group > few_rows && q.n > 0;
+}
+__device__ __forceinline__ void kv_item_enter(const AttnArgs &a, int tpi, int few_rows, KvItem &it)   // at sequence it.s, or a later one
+{
+    while (it.s < a.b.n_seqs && !kv_item_seq(a, few_rows, it.s, it.q)) ++it.s;
+    it.n_rt = (it.q.n + tpi - 1) / tpi;
+}
+template <int TILE>
+__device__ __forceinline__ void kv_item_next(const AttnArgs &a, int tpi, int few_rows, KvItem &it)
+{
+    if (++it.rt == it.n_rt) {
+        it.rt = 0;
+        if (++it.h == a.c.n_kv_heads) {
+            it.h = 0;
+            ++it.s;
+            kv_item_enter(a, tpi, few_rows, it);
+        }
+    }
+    kv_item_tiles<TILE>(a, tpi, it.q, it.rt, &it);
+}
+// Units of one head of the lane's sequence q (n = 0: none); the whole warp calls it.
+// Long chunks' row tiles are counted by all lanes together.
+template <int TILE>
+__device__ __forceinline__ unsigned long long kv_head_units(const AttnArgs &a, int tpi, const KvSeq &q)
+{
+    const int lane = threadIdx.x & 31, n_rt = (q.n + tpi - 1) / tpi;
+    unsigned long long f = 0;
+    if (n_rt <= 4)
+        for (int rt = 0; rt < n_rt; ++rt) f += kv_item_tiles<TILE>(a, tpi, q, rt, nullptr);
+    for (unsigned todo = __ballot_sync(0xFFFFFFFFu, n_rt > 4); todo; todo &= todo - 1) {
+        const int src = __ffs(todo) - 1;
+        KvSeq x = q;
+        x.n = __shfl_sync(0xFFFFFFFFu, q.n, src);
+        x.len = __shfl_sync(0xFFFFFFFFu, q.len, src);
+        const int m = __shfl_sync(0xFFFFFFFFu, n_rt, src);
+        unsigned long long c = 0;
+        for (int rt = lane; rt < m; rt += 32) c += kv_item_tiles<TILE>(a, tpi, x, rt, nullptr);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) c += __shfl_xor_sync(0xFFFFFFFFu, c, o);
+        if (lane == src) f = c;
+    }
+    return f;
+}
+
+struct KvScan {   // shared
+    unsigned long long warp[12];
+    int seq, head, rt, off;   // the CTA's first item and its first unit there
+};
+struct KvCtaShare {
+    KvShare share;
+    unsigned cta;             // of the units, against blockIdx: a part's CTA starts before the one that waits for it
+    unsigned long long u0, u1;
+    __device__ __forceinline__ KvCtaShare() : share(1, 1), cta(0), u0(0), u1(0) {}
+};
+
+// The CTA's share of all units, by a scan over the sequences; false when it has none.
+// The first item is in sh after the caller's next __syncthreads().
+template <int TILE, int WARPS, int HD, class I>
+__device__ __forceinline__ bool kv_items_share(const AttnArgs &a, int tpi, int few_rows, KvScan &sh, KvCtaShare &my)
+{
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int per = (a.b.n_seqs + WARPS * 32 - 1) / (WARPS * 32);
+    const int sq0 = min(a.b.n_seqs, tid * per), sq1 = min(a.b.n_seqs, sq0 + per);
+    unsigned long long mine = 0;
+    bool bad_seq = false;
+    for (int k = 0; k < per; ++k) {
+        KvSeq q{};
+        if (sq0 + k < sq1) {
+            bad_seq = bad_seq || !kv_seq(a.b, a.c, sq0 + k, q, nullptr);
+            if (!kv_item_seq(a, few_rows, sq0 + k, q)) q.n = 0;
+        }
+        mine += kv_head_units<TILE>(a, tpi, q) * a.c.n_kv_heads;
+    }
+    unsigned long long incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const unsigned long long x = __shfl_up_sync(0xFFFFFFFFu, incl, o);
+        if (lane >= o) incl += x;
+    }
+    if (lane == 31) sh.warp[warp] = incl;
+    if (__syncthreads_or(bad_seq) && blockIdx.x == 0) kv_zero_bad<HD, I>(a);
+    unsigned long long before = incl - mine, total = 0;
+    for (int w = 0; w < WARPS; ++w) {
+        before += w < warp ? sh.warp[w] : 0;
+        total += sh.warp[w];
+    }
+    const unsigned G = total < gridDim.x ? static_cast<unsigned>(total) : gridDim.x;
+    if (blockIdx.x >= G) return false;
+    my.cta = G - 1 - blockIdx.x;
+    my.share = KvShare(total, G);
+    my.u0 = my.share.start(my.cta), my.u1 = my.share.start(my.cta + 1);
+    const unsigned long long u0 = my.u0;
+    const bool mine_u0 = before <= u0 && u0 < before + mine;
+    if (__any_sync(0xFFFFFFFFu, mine_u0)) {   // the warp whose sequences hold u0
+        unsigned long long at = before;
+        bool found = false;
+        KvSeq fq{};
+        int fs = 0;
+        unsigned long long fr = 0, ff = 1;
+        for (int k = 0; k < per; ++k) {
+            KvSeq q{};
+            if (sq0 + k < sq1 && !kv_item_seq(a, few_rows, sq0 + k, q)) q.n = 0;
+            const unsigned long long f = kv_head_units<TILE>(a, tpi, q), n = f * a.c.n_kv_heads;
+            if (mine_u0 && !found && u0 < at + n) found = true, fq = q, fs = sq0 + k, fr = u0 - at, ff = f;
+            at += n;
+        }
+        const int src = __ffs(__ballot_sync(0xFFFFFFFFu, found)) - 1;
+        fq.n = __shfl_sync(0xFFFFFFFFu, fq.n, src);
+        fq.len = __shfl_sync(0xFFFFFFFFu, fq.len, src);
+        const unsigned long long r = __shfl_sync(0xFFFFFFFFu, fr, src), f = __shfl_sync(0xFFFFFFFFu, ff, src);
+        const unsigned long long head = kv_div(r, f);
+        unsigned long long rem = r - head * f;   // units of the head before u0: the row tile, 32 at a time
+        const int n_rt = (fq.n + tpi - 1) / tpi;
+        for (int base = 0; base < n_rt; base += 32) {
+            const unsigned long long k = base + lane < n_rt ? kv_item_tiles<TILE>(a, tpi, fq, base + lane, nullptr) : 0;
+            unsigned long long c = k;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const unsigned long long x = __shfl_up_sync(0xFFFFFFFFu, c, o);
+                if (lane >= o) c += x;
+            }
+            const unsigned hit = __ballot_sync(0xFFFFFFFFu, rem < c);
+            if (hit) {
+                if (lane == __ffs(hit) - 1) {
+                    sh.head = static_cast<int>(head);
+                    sh.rt = base + lane;
+                    sh.off = static_cast<int>(rem - (c - k));
+                }
+                break;
+            }
+            rem -= __shfl_sync(0xFFFFFFFFu, c, 31);
+        }
+        if (lane == src) sh.seq = fs;
+    }
+    return true;
+}
+template <int TILE>
+__device__ __forceinline__ KvItem kv_item_first(const AttnArgs &a, int tpi, int few_rows, const KvScan &sh)
+{
+    KvItem it{};
+    it.s = sh.seq, it.h = sh.head, it.rt = sh.rt;
+    kv_item_enter(a, tpi, few_rows, it);
+    kv_item_tiles<TILE>(a, tpi, it.q, it.rt, &it);
+    return it;
 }
 
 // The layer's K and V as 4-D tensors: dimension, then position in the page, head

@@ -41,7 +41,7 @@ static constexpr int kPolyOf8 = 3;      // of 8 pairs of scores, how many go thr
 
 struct ManyArgs {
     AttnArgs a;
-    int tpt;         // tokens of a row group: 128 / G
+    int tpt, tpi;    // tokens of a row group, 128 / G, and of an item, twice that
     int few_rows;    // sequences of at most this many rows are another launch's
     int box;         // positions of one K or V box
     int bf16;
@@ -69,80 +69,11 @@ struct alignas(16) ManyPart {
 struct ManyShared {
     ManyPart part[4];
     uint64_t sfull[2], pready[2][2], ofull[2], qfull, qempty, done, join, kvfull[8], kvempty[4], vready[8];
-    unsigned long long scan[12], u0;
+    KvScan scan;
     uint32_t tmem;
-    int seq, head, rt, off, fail, bad, last;
+    int fail, bad;
 };
 static_assert(sizeof(ManyShared) <= 1024, "ManyShared");
-
-// ---- the items ----
-struct ManyItem {
-    int s, h, rt;           // sequence, kv head, row tile
-    KvSeq q;
-    int n_rt;               // row tiles a head
-    int t0, t1;             // new tokens [t0, t1) of the sequence
-    int ns, lo, n;          // its position tiles: [0, ns) and [lo, lo + n - ns)
-};
-
-__device__ __forceinline__ int many_tiles(const ManyArgs &a, const KvSeq &q, int rt, ManyItem *it)
-{
-    const int t0 = rt * 2 * a.tpt, t1 = min(q.n, t0 + 2 * a.tpt), p0 = q.len - q.n;
-    const KvSpan sp = kv_span(p0 + t0, a.a.window, a.a.sinks);
-    const int hi = (p0 + t1 - 1) / kTileN + 1;
-    int ns = 0, lo = 0, n = hi;
-    if (a.a.sinks < sp.lo) {
-        ns = (a.a.sinks + kTileN - 1) / kTileN;
-        lo = max(sp.lo / kTileN, ns);
-        n = ns + hi - lo;
-    }
-    if (it) it->t0 = t0, it->t1 = t1, it->ns = ns, it->lo = lo, it->n = n;
-    return n;
-}
-// True for a sequence of this launch.
-__device__ __forceinline__ bool many_seq(const ManyArgs &a, int s, KvSeq &q)
-{
-    return kv_seq(a.a.b, a.a.c, s, q, nullptr) && static_cast<long long>(q.n) * a.a.group > a.few_rows && q.n > 0;
-}
-__device__ __forceinline__ void many_enter(const ManyArgs &a, ManyItem &it)   // at sequence it.s, or a later one
-{
-    while (it.s < a.a.b.n_seqs && !many_seq(a, it.s, it.q)) ++it.s;
-    it.n_rt = (it.q.n + 2 * a.tpt - 1) / (2 * a.tpt);
-}
-__device__ __forceinline__ void many_next(const ManyArgs &a, ManyItem &it)
-{
-    if (++it.rt == it.n_rt) {
-        it.rt = 0;
-        if (++it.h == a.a.c.n_kv_heads) {
-            it.h = 0;
-            ++it.s;
-            many_enter(a, it);
-        }
-    }
-    many_tiles(a, it.q, it.rt, &it);
-}
-// Units of one head of the lane's sequence q (n = 0: none); the whole warp calls it.
-// Long chunks' row tiles are counted by all lanes together.
-__device__ __forceinline__ unsigned long long many_head_units(const ManyArgs &a, const KvSeq &q)
-{
-    const int lane = threadIdx.x & 31, n_rt = (q.n + 2 * a.tpt - 1) / (2 * a.tpt);
-    unsigned long long f = 0;
-    if (n_rt <= 4)
-        for (int rt = 0; rt < n_rt; ++rt) f += many_tiles(a, q, rt, nullptr);
-    for (unsigned todo = __ballot_sync(0xFFFFFFFFu, n_rt > 4); todo; todo &= todo - 1) {
-        const int src = __ffs(todo) - 1;
-        KvSeq x = q;
-        x.n = __shfl_sync(0xFFFFFFFFu, q.n, src);
-        x.len = __shfl_sync(0xFFFFFFFFu, q.len, src);
-        const int m = __shfl_sync(0xFFFFFFFFu, n_rt, src);
-        unsigned long long c = 0;
-        for (int rt = lane; rt < m; rt += 32) c += many_tiles(a, x, rt, nullptr);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) c += __shfl_xor_sync(0xFFFFFFFFu, c, o);
-        if (lane == src) f = c;
-    }
-    return f;
-}
-__device__ __forceinline__ int many_tile_pos(const ManyItem &it, int j) { return (j < it.ns ? j : j - it.ns + it.lo) * kTileN; }
 
 // ---- TMEM ----
 #define TB_R32(r)                                                                                                       \
@@ -294,103 +225,29 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     if (warp == 10 && lane == 0) prefetch_map(&qmap);
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    // ---- this CTA's share of all units: a scan over the sequences ----
-    const int per = (a.a.b.n_seqs + kManyThreads - 1) / kManyThreads;
-    const int sq0 = min(a.a.b.n_seqs, tid * per), sq1 = min(a.a.b.n_seqs, sq0 + per);
-    unsigned long long mine = 0;
-    bool bad_seq = false;
-    for (int k = 0; k < per; ++k) {
-        KvSeq q{};
-        if (sq0 + k < sq1) {
-            bad_seq = bad_seq || !kv_seq(a.a.b, a.a.c, sq0 + k, q, nullptr);
-            if (!many_seq(a, sq0 + k, q)) q.n = 0;
-        }
-        mine += many_head_units(a, q) * a.a.c.n_kv_heads;
-    }
-    unsigned long long incl = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const unsigned long long x = __shfl_up_sync(0xFFFFFFFFu, incl, o);
-        if (lane >= o) incl += x;
-    }
-    if (lane == 31) sh.scan[warp] = incl;
-    if (__syncthreads_or(bad_seq) && blockIdx.x == 0) kv_zero_bad<HD, I>(a.a);
-    unsigned long long before = incl - mine, total = 0;
-    for (int w = 0; w < kManyThreads / 32; ++w) {
-        before += w < warp ? sh.scan[w] : 0;
-        total += sh.scan[w];
-    }
-    const unsigned G = total < gridDim.x ? static_cast<unsigned>(total) : gridDim.x;
-    if (blockIdx.x >= G) return;
+    KvCtaShare my;
+    if (!kv_items_share<kTileN, kManyThreads / 32, HD, I>(a.a, a.tpi, a.few_rows, sh.scan, my)) return;
     if (warp == 8) {
         tmem_alloc(smem_u32(&sh.tmem), 512);
         tmem_relinquish();
-    }
-    const unsigned cta = G - 1 - blockIdx.x;   // of the units, against blockIdx: see the joining of parts
-    const KvShare share(total, G);
-    const unsigned long long u0 = share.start(cta), u1 = share.start(cta + 1);
-    const bool mine_u0 = before <= u0 && u0 < before + mine;
-    if (__any_sync(0xFFFFFFFFu, mine_u0)) {   // the warp whose sequences hold u0
-        unsigned long long at = before;
-        bool found = false;
-        KvSeq fq{};
-        int fs = 0;
-        unsigned long long fr = 0, ff = 1;
-        for (int k = 0; k < per; ++k) {
-            KvSeq q{};
-            if (sq0 + k < sq1 && !many_seq(a, sq0 + k, q)) q.n = 0;
-            const unsigned long long f = many_head_units(a, q), n = f * a.a.c.n_kv_heads;
-            if (mine_u0 && !found && u0 < at + n) found = true, fq = q, fs = sq0 + k, fr = u0 - at, ff = f;
-            at += n;
-        }
-        const int src = __ffs(__ballot_sync(0xFFFFFFFFu, found)) - 1;
-        fq.n = __shfl_sync(0xFFFFFFFFu, fq.n, src);
-        fq.len = __shfl_sync(0xFFFFFFFFu, fq.len, src);
-        const unsigned long long r = __shfl_sync(0xFFFFFFFFu, fr, src), f = __shfl_sync(0xFFFFFFFFu, ff, src);
-        const unsigned long long head = kv_div(r, f);
-        unsigned long long rem = r - head * f;   // units of the head before u0: the row tile, 32 at a time
-        const int n_rt = (fq.n + 2 * a.tpt - 1) / (2 * a.tpt);
-        for (int base = 0; base < n_rt; base += 32) {
-            const unsigned long long k = base + lane < n_rt ? many_tiles(a, fq, base + lane, nullptr) : 0;
-            unsigned long long c = k;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const unsigned long long x = __shfl_up_sync(0xFFFFFFFFu, c, o);
-                if (lane >= o) c += x;
-            }
-            const unsigned hit = __ballot_sync(0xFFFFFFFFu, rem < c);
-            if (hit) {
-                if (lane == __ffs(hit) - 1) {
-                    sh.head = static_cast<int>(head);
-                    sh.rt = base + lane;
-                    sh.off = static_cast<int>(rem - (c - k));
-                }
-                break;
-            }
-            rem -= __shfl_sync(0xFFFFFFFFu, c, 31);
-        }
-        if (lane == src) sh.seq = fs;
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tm = sh.tmem;
 
-    ManyItem it{};
-    it.s = sh.seq, it.h = sh.head, it.rt = sh.rt;
-    many_enter(a, it);
-    many_tiles(a, it.q, it.rt, &it);
-    int j0 = sh.off;             // the first of the item's tiles that is this CTA's
-    unsigned long long u = u0;
+    KvItem it = kv_item_first<kTileN>(a.a, a.tpi, a.few_rows, sh.scan);
+    int j0 = sh.scan.off;        // the first of the item's tiles that is this CTA's
+    unsigned long long u = my.u0;
     // the item's tiles [j0, j1) are this CTA's
     auto part_end = [&]() {
-        const unsigned long long left = u1 - u;
+        const unsigned long long left = my.u1 - u;
         return left < static_cast<unsigned>(it.n - j0) ? j0 + static_cast<int>(left) : it.n;
     };
     auto next_item = [&](int j1) {
         u += j1 - j0;
         j0 = 0;
-        if (u < u1) many_next(a, it);
+        if (u < my.u1) kv_item_next<kTileN>(a.a, a.tpi, a.few_rows, it);
     };
     auto failed = [&]() { return *reinterpret_cast<volatile int *>(&sh.fail) != 0; };
     // Waits, by a whole warp in step, for one or two barriers; false when the limit runs
@@ -425,10 +282,10 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         if (warp == 9) {
             // ---- K and V ----
             bool ok = true;
-            while (ok && u < u1) {
+            while (ok && u < my.u1) {
                 const int j1 = part_end();
                 for (int j = j0; ok && j < j1; ++j) {
-                    const int p0 = many_tile_pos(it, j), boxes = kTileN / a.box;
+                    const int p0 = kv_item_pos<kTileN>(it, j), boxes = kTileN / a.box;
                     // lane l: box l of the tile, its page (past the end: a page that reads as zeros)
                     int page = a.a.c.n_pages, pos = 0;
                     const int p = p0 + lane * a.box;
@@ -466,7 +323,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         } else if (warp == 10) {
             // ---- Q ----
             bool ok = true;
-            while (ok && u < u1) {
+            while (ok && u < my.u1) {
                 const int j1 = part_end();
                 if (q_issued > 0) ok = wait(&sh.qempty, q_issued - 1u);
                 if (!ok) break;
@@ -477,7 +334,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                     pt.row0 = it.q.row0, pt.len = it.q.len, pt.n = it.q.n, pt.t0 = it.t0;
                     pt.t1 = it.t1, pt.s = it.s, pt.h = it.h, pt.tiles = it.n;
                     pt.ns = it.ns, pt.lo = it.lo, pt.j0 = j0, pt.j1 = j1;
-                    pt.peer = j0 > 0 ? share.of(u - j0) : share.of(u + it.n - 1) - cta;
+                    pt.peer = j0 > 0 ? my.share.of(u - j0) : my.share.of(u + it.n - 1) - my.cta;
                 }
                 __syncwarp();
                 if (elect_one()) {
@@ -497,13 +354,13 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             // holds the sequence's end: whatever V has there, 0 * it has to be 0 ----
             bool ok = true;
             uint32_t n = 1;
-            while (ok && u < u1) {
+            while (ok && u < my.u1) {
                 const int j1 = part_end();
                 for (int j = j0; j < j1; ++j, n += 2) {
                     const uint32_t slot = n % NS;
                     ok = wait(&sh.kvfull[slot], n / NS);
                     if (!ok) break;
-                    const int r1 = it.q.len - many_tile_pos(it, j);
+                    const int r1 = it.q.len - kv_item_pos<kTileN>(it, j);
                     if (r1 < kTileN && r1 % a.box) {
                         const int rows = a.box - r1 % a.box;
                         for (int i = lane; i < rows * (HD / 8); i += 32) {
@@ -526,7 +383,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             const uint32_t id_o = (1u << 4) | (fmt << 7) | (fmt << 10) | (1u << 16) | ((HD >> 3) << 17) | (8u << 24);
             const uint32_t tu = __shfl_sync(0xFFFFFFFFu, tm, 0);
             const uint64_t qd = sw128_desc(qbase), kd = sw128_desc(ring), vd = v_desc(ring);
-            const uint32_t n_tiles = static_cast<uint32_t>(u1 - u0);
+            const uint32_t n_tiles = static_cast<uint32_t>(my.u1 - my.u0);
             uint32_t n = 0, q = 0, np = 0;   // ring slots, items and P tiles taken
             bool ok = true;
             auto issue_s = [&](int g, uint32_t slot) {
@@ -635,7 +492,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             ok = wait(&sh.join, joins++);
             return ok;
         };
-        const uint32_t n_tiles = static_cast<uint32_t>(u1 - u0);
+        const uint32_t n_tiles = static_cast<uint32_t>(my.u1 - my.u0);
         while (ok && cnt < n_tiles) {
             ok = wait(&sh.sfull[g], cnt);   // of the item's first tile: its description is there too
             if (!ok) break;
@@ -735,7 +592,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             const int row = g * 128 + lr;
             if (j0 > 0) {
                 // ---- not the item's beginning: the part goes to the CTA that has it ----
-                float *part = a.a.part + static_cast<size_t>(cta) * Cfg::PART + row * 4;
+                float *part = a.a.part + static_cast<size_t>(my.cta) * Cfg::PART + row * 4;
 #pragma unroll 1
                 for (int c = 0; c < HD; c += 32) {
                     uint32_t o[32];
@@ -755,7 +612,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                 // order.  They are waited for (as every wait, within a limit): the ranges run
                 // against blockIdx, so those CTAs were started before this one. ----
                 const unsigned others = it.peer;
-                const float *part = a.a.part + static_cast<size_t>(cta + 1) * Cfg::PART;
+                const float *part = a.a.part + static_cast<size_t>(my.cta + 1) * Cfg::PART;
                 float M = m, L = l;
                 bool odd = *reinterpret_cast<volatile int *>(&sh.bad);
                 if (others > 0) {
@@ -764,13 +621,13 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                         uint32_t i = 0;
                         unsigned n = 0;
                         do {
-                            asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(n) : "l"(a.a.arrived + cta) : "memory");
+                            asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(n) : "l"(a.a.arrived + my.cta) : "memory");
                         } while (n < 8 * others && ++i < lim && !failed());
                         if (n < 8 * others) {
                             if (!failed()) atomicExch(err, ERR_WAIT_TIMEOUT);
                             *reinterpret_cast<volatile int *>(&sh.fail) = 1;
                         }
-                        a.a.arrived[cta] = 0;   // zero between calls
+                        a.a.arrived[my.cta] = 0;   // zero between calls
                         __threadfence();
                     }
                     if (!join()) break;
@@ -922,7 +779,7 @@ static int many_launch(ManyArgs &m, int tc, int sms, cudaStream_t st)
 
 int kv_many_launch(AttnArgs a, int hd, int tc, int few_rows, int sms, cudaStream_t st)
 {
-    ManyArgs m{a, 128 / a.group, few_rows, 0, tc == QT_BF16};
+    ManyArgs m{a, 128 / a.group, 2 * (128 / a.group), few_rows, 0, tc == QT_BF16};
     if (hd == 128)
         return tc == QT_BF16 ? many_launch<128, __nv_bfloat16>(m, tc, sms, st) : many_launch<128, __half>(m, tc, sms, st);
     return tc == QT_BF16 ? many_launch<64, __nv_bfloat16>(m, tc, sms, st) : many_launch<64, __half>(m, tc, sms, st);
