@@ -395,7 +395,6 @@ __global__ void __launch_bounds__(FewCfg<HD, TI, TC>::W * 32, FewCfg<HD, TI, TC>
             const int sl = (step0 + k) * W + warp;
             if (sl < cu.sl.n && ok) {
                 uint32_t st = taken % NST;
-                const uint32_t kb = ring + st * Cfg::SB;
                 const int j0 = (sl < cu.sl.ns ? sl : sl - cu.sl.ns + cu.sl.lo) * kSlice;
                 ok = mbar_wait_bounded(bars + st * 8, (taken / NST) & 1u, a.err, a.wait_limit);
                 ok = __all_sync(0xFFFFFFFFu, ok);
@@ -403,6 +402,7 @@ __global__ void __launch_bounds__(FewCfg<HD, TI, TC>::W * 32, FewCfg<HD, TI, TC>
                     sh.fail = 1;
                     break;
                 }
+                const uint32_t kb = shared_after(ring + st * Cfg::SB);
                 const bool bad = (hidden >> st) & 1u;
                 // ---- S^T = K Q^T; the tensor core truncates what it adds to an accumulator, so
                 // fp32 results come from short chains that are added in fp32, the small
@@ -430,6 +430,8 @@ __global__ void __launch_bounds__(FewCfg<HD, TI, TC>::W * 32, FewCfg<HD, TI, TC>
                             mma16<TC>(c[n > 0 ? NC - 1 : FINE ? ks & 3 : ks & 1], x, qf[n][ks][0], qf[n][ks][1]);
                     }
                 }
+#pragma unroll
+                for (int i = 0; i < NC; ++i) pin(c[i]);
                 __syncwarp();   // every lane has read K
                 ++taken;
                 refill();
@@ -471,13 +473,13 @@ __global__ void __launch_bounds__(FewCfg<HD, TI, TC>::W * 32, FewCfg<HD, TI, TC>
                 l[1] += x[1] + x[3];
                 // ---- O^T += V^T P^T ----
                 st = taken % NST;
-                const uint32_t vb = ring + st * Cfg::SB;
                 ok = mbar_wait_bounded(bars + st * 8, (taken / NST) & 1u, a.err, a.wait_limit);
                 ok = __all_sync(0xFFFFFFFFu, ok);
                 if (!ok) {
                     sh.fail = 1;
                     break;
                 }
+                uint32_t vb = ring + st * Cfg::SB;
                 if (bad || j0 + kSlice > cu.q.len) {
                     // positions that no one wrote (all of them where the page is none): whatever
                     // lies there, 0 * it has to be 0
@@ -490,6 +492,7 @@ __global__ void __launch_bounds__(FewCfg<HD, TI, TC>::W * 32, FewCfg<HD, TI, TC>
                     fence_proxy_async_smem();   // before the stage's next copy
                     __syncwarp();
                 }
+                vb = shared_after(vb);
                 if constexpr (X32) {
                     uint32_t ph[2][2], pl[2][2];   // [8 positions][2 t and 2 t + 1 of them, row g]
 #pragma unroll
@@ -511,7 +514,7 @@ __global__ void __launch_bounds__(FewCfg<HD, TI, TC>::W * 32, FewCfg<HD, TI, TC>
 #pragma unroll
                                 for (int e = 0; e < 2; ++e) {
                                     const uint32_t r = kb8 * 8 + 2 * t + e;
-                                    v[cc][e] = lds_u128(shared_after(vb + (2 * jb + cc) * kCol + r * 128 + ((g ^ (r & 7)) << 4)));
+                                    v[cc][e] = lds_u128(vb + (2 * jb + cc) * kCol + r * 128 + ((g ^ (r & 7)) << 4));
                                 }
 #pragma unroll
                             for (int d = 0; d < 4; ++d) {
@@ -552,6 +555,8 @@ __global__ void __launch_bounds__(FewCfg<HD, TI, TC>::W * 32, FewCfg<HD, TI, TC>
                         }
                     }
                 }
+#pragma unroll
+                for (int i = 0; i < HD / 16; ++i) pin(O[i]);
                 __syncwarp();   // every lane has read V
                 ++taken;
                 refill();

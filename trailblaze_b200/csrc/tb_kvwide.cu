@@ -5,7 +5,7 @@
 //
 // Items, units and the joining of parts are those of k_kv_many (tb_kvattn.cuh) with
 // 128 query rows and tiles of 32 positions.  A CTA's 8 warps own 16 rows each and
-// read the same K and V tiles, a TMA ring of 6 stages that the warps refill in turn,
+// read the same K and V tiles, a TMA ring of 4 or 6 stages that the warps refill in turn,
 // so the cache is read once for 128 rows.  The products and their splitting into
 // parts of fewer bits are k_kv_few's: S^T = K Q^T, O^T += V^T P^T on mma.sync with
 // the rows as two N = 8 tiles, so that K and V are fetched and split once for 16
@@ -34,10 +34,13 @@ template <int HD, int TI, int TC>
 struct WideCfg {
     static constexpr int ES = TC == QT_F32 ? 4 : 2;
     static constexpr int HALF = kWTile * HD * ES;      // K or V of a tile
-    static constexpr int NST = 6;
+    // fp32 caches: the low parts of Q live in shared memory, in the order of the
+    // products (with both parts in registers 350 bytes a thread were spilled)
+    static constexpr int QLO = TC == QT_F32 ? kWWarps * 2 * (HD / 8) * 32 * 8 : 0;
+    static constexpr int NST = TC == QT_F32 ? 4 : 6;
     static constexpr int NQ = TC == QT_F32 ? 2 : TI == TC ? 1 : TC == QT_BF16 ? 3 : 2;
     static constexpr int NP = TC == QT_BF16 && TI == QT_F32 ? 3 : 2;
-    static constexpr int SMEM = 1024 + NST * 2 * HALF + 2 * NST * 8 + static_cast<int>(sizeof(WideShared));
+    static constexpr int SMEM = 1024 + NST * 2 * HALF + QLO + 2 * NST * 8 + static_cast<int>(sizeof(WideShared));
     static constexpr int PART = kWThreads * (HD / 2 + 8);   // floats of a partial result: O, m, l as the threads hold them
 };
 
@@ -56,7 +59,8 @@ __global__ void __launch_bounds__(kWThreads, 1)
     constexpr uint32_t kCol = kWTile * 128;
     extern __shared__ __align__(1024) uint8_t smraw[];
     uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smraw) + 1023) & ~uintptr_t(1023));
-    uint64_t *full = reinterpret_cast<uint64_t *>(sm + NST * 2 * Cfg::HALF), *empty = full + NST;
+    uint2 *qlo = reinterpret_cast<uint2 *>(sm + NST * 2 * Cfg::HALF);   // [warp][nt][ks][lane]
+    uint64_t *full = reinterpret_cast<uint64_t *>(sm + NST * 2 * Cfg::HALF + Cfg::QLO), *empty = full + NST;
     WideShared &sh = *reinterpret_cast<WideShared *>(empty + NST);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const AttnArgs &aa = a.a;
@@ -149,7 +153,8 @@ __global__ void __launch_bounds__(kWThreads, 1)
         const int j1 = left < static_cast<unsigned>(it.n - j0) ? j0 + static_cast<int>(left) : it.n;
         const int p0 = it.q.len - it.q.n, rows = (it.t1 - it.t0) * aa.group, r0 = warp * 16;
         // rows g and g + 8 of the warp's 16 as the B operands; rows past the last are zero
-        uint32_t qf[NT][NQ][KS][2];
+        constexpr int NR = X32 ? 1 : NQ;   // parts in registers
+        uint32_t qf[NT][NR][KS][2];
         float rs[NT][2];
         int pos[NT][2];
 #pragma unroll
@@ -177,9 +182,12 @@ __global__ void __launch_bounds__(kWThreads, 1)
                     }
                 if constexpr (X32) {
 #pragma unroll
-                    for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) split_tf32(__float_as_uint(y[ks][e]), qf[nt][0][ks][e], qf[nt][1][ks][e]);
+                    for (int ks = 0; ks < KS; ++ks) {
+                        uint2 lo;
+                        split_tf32(__float_as_uint(y[ks][0]), qf[nt][0][ks][0], lo.x);
+                        split_tf32(__float_as_uint(y[ks][1]), qf[nt][0][ks][1], lo.y);
+                        qlo[((warp * NT + nt) * KS + ks) * 32 + lane] = lo;   // read by this lane alone
+                    }
                 } else {
                     if constexpr (TC == QT_F16) {   // the row times 2^k, its largest element near 2^13
                         big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 1));
@@ -230,7 +238,7 @@ __global__ void __launch_bounds__(kWThreads, 1)
             ok = ok && mbar_wait_bounded(fb + st * 8, (taken / NST) & 1u, err, lim);
             ok = __all_sync(0xFFFFFFFFu, ok) && !*reinterpret_cast<volatile int *>(&sh.fail);
             if (!ok) *reinterpret_cast<volatile int *>(&sh.fail) = 1;
-            const uint32_t kb = ring + st * 2 * Cfg::HALF, vb = kb + Cfg::HALF;
+            uint32_t kb = ring + st * 2 * Cfg::HALF, vb = kb + Cfg::HALF;
             const int k0 = kv_item_pos<kWTile>(it, j);
             if (k0 + kWTile > it.q.len) {
                 // the sequence's end: V past it, in the box that holds it, is zeroed: whatever
@@ -244,12 +252,15 @@ __global__ void __launch_bounds__(kWThreads, 1)
                 fence_proxy_async_smem();   // before the stage's next copy
                 __syncthreads();
             }
+            kb = shared_after(kb);
+            vb = shared_after(vb);
             const bool skip = !any || !ok || k0 > pmax ||
                               (aa.window > 0 && k0 + kWTile - 1 <= pmin - aa.window && k0 >= aa.sinks);
             if (!skip) {
 #pragma unroll 1
                 for (int s2 = 0; s2 < kWTile / 16; ++s2) {
                     const int js = k0 + s2 * 16;
+                    if (js > pmax) break;
                     const uint32_t kr = s2 * 16 + krow, vr = s2 * 16 + vrow;
                     // ---- S^T = K Q^T, in short chains (see k_kv_few) ----
                     float c[NT][3][4];
@@ -274,10 +285,13 @@ __global__ void __launch_bounds__(kWThreads, 1)
                                 mma_tf32(c[nt][ks & 1], hi, qf[nt][0][ks][0], qf[nt][0][ks][1]);
                             }
 #pragma unroll
-                            for (int nt = 0; nt < NT; ++nt) mma_tf32(c[nt][2], hi, qf[nt][1][ks][0], qf[nt][1][ks][1]);
+                            for (int nt = 0; nt < NT; ++nt) {
+                                const uint2 lq = qlo[((warp * NT + nt) * KS + ks) * 32 + lane];
+                                mma_tf32(c[nt][2], hi, lq.x, lq.y);
+                            }
                         } else {
 #pragma unroll
-                            for (int n = NQ - 1; n >= 0; --n)
+                            for (int n = NR - 1; n >= 0; --n)
 #pragma unroll
                                 for (int nt = 0; nt < NT; ++nt)
                                     mma16<TC>(c[nt][n > 0 ? 2 : ks & 1], x, qf[nt][n][ks][0], qf[nt][n][ks][1]);
@@ -353,8 +367,7 @@ __global__ void __launch_bounds__(kWThreads, 1)
 #pragma unroll
                                     for (int e = 0; e < 2; ++e) {
                                         const uint32_t r = s2 * 16 + kb8 * 8 + 2 * t + e;
-                                        v[kb8][cc][e] = lds_u128(
-                                            shared_after(vb + (2 * jb + cc) * kCol + r * 128 + ((g ^ (r & 7)) << 4)));
+                                        v[kb8][cc][e] = lds_u128(vb + (2 * jb + cc) * kCol + r * 128 + ((g ^ (r & 7)) << 4));
                                     }
 #pragma unroll
                             for (int d = 0; d < 4; ++d) {
@@ -407,6 +420,10 @@ __global__ void __launch_bounds__(kWThreads, 1)
                     }
                 }
             }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int i = 0; i < HD / 16; ++i) pin(O[nt][i]);
             __syncwarp();   // every lane has read the stage
             if (lane == 0) mbar_arrive(eb + st * 8);
             ++taken;
