@@ -7,8 +7,8 @@
 // An item is (sequence, kv head, 8 query rows): row r of a sequence's n * G rows
 // (G = query heads per kv head) is new token r / G, head r % G of the group.  Its
 // positions come in slices of 16 (16 divides a page), a step is one slice for
-// each of the CTA's W warps.  All items' steps, laid end to end, are cut into
-// equal parts, one per CTA, whatever the sequences' lengths: a CTA works through
+// each of the CTA's W warps.  All items' steps (and some more for each item's own
+// cost), laid end to end, are cut into equal parts, one per CTA, whatever the sequences' lengths: a CTA works through
 // the end of one item, whole items, and the beginning of another.  Items that lie
 // in one CTA are written out directly, the others' parts go through the workspace to
 // the CTA that has the item's beginning, which adds them in CTA order, so results
@@ -69,6 +69,11 @@ struct FewCfg {
     static constexpr int CTAS = SB >= 8192 ? 1 : 2;             // per SM
     static constexpr int NST = SB >= 8192 ? 3 : SB >= 4096 ? 6 : 12;
     static constexpr int MIN = SB >= 8192 ? 2 : 4;              // steps of a CTA, at least
+    // An item's own cost (Q, the joining of the warps, output: some 3 us), in steps at the
+    // rate of a CTA's share of the bandwidth: it counts in the cutting, else the CTAs that
+    // get many short sequences finish last (24 sequences of up to 1733 positions, 16 heads
+    // of 64: 50 us without)
+    static constexpr int COST = 65536 / (W * 2 * SB) > 0 ? 65536 / (W * 2 * SB) : 1;
     static constexpr int NQ = TC == QT_F32 ? 2 : TI == TC ? 1 : TC == QT_BF16 ? 3 : 2;
     static constexpr int NP = TC == QT_BF16 && TI == QT_F32 ? 3 : 2;
     static constexpr int MERGE = W * 8 * HD * 4;
@@ -105,7 +110,7 @@ __device__ __forceinline__ void kv_cur_seq(const AttnArgs &a, KvCur &c)
     c.steps = (c.sl.n + W - 1) / W;
 }
 
-template <int W>
+template <int W, int COST>
 __device__ __forceinline__ unsigned long long kv_seq_steps(const AttnArgs &a, int s, bool &bad, unsigned long long *items)
 {
     KvSeq q;
@@ -117,7 +122,7 @@ __device__ __forceinline__ unsigned long long kv_seq_steps(const AttnArgs &a, in
     const KvSlices sl = kv_slices(q, a.window, a.sinks);
     const unsigned long long tiles = (static_cast<unsigned long long>(q.n) * a.group + 7) >> 3;
     if (items) *items += tiles * a.c.n_kv_heads;
-    return tiles * a.c.n_kv_heads * static_cast<unsigned>((sl.n + W - 1) / W);
+    return tiles * a.c.n_kv_heads * static_cast<unsigned>((sl.n + W - 1) / W + COST);
 }
 
 template <int HD, int TI, int TC>
@@ -157,7 +162,7 @@ __global__ void __launch_bounds__(FewCfg<HD, TI, TC>::W * 32, FewCfg<HD, TI, TC>
     const int per = (a.b.n_seqs + T - 1) / T, sq0 = tid * per, sq1 = min(a.b.n_seqs, sq0 + per);
     unsigned long long mine = 0, items = 0;
     bool bad_seq = false;
-    for (int s = sq0; s < sq1; ++s) mine += kv_seq_steps<W>(a, s, bad_seq, &items);
+    for (int s = sq0; s < sq1; ++s) mine += kv_seq_steps<W, Cfg::COST>(a, s, bad_seq, &items);
     if (__syncthreads_or(bad_seq) && blockIdx.x == 0) kv_zero_bad<HD, I>(a);
     unsigned long long incl = mine;
 #pragma unroll
@@ -189,7 +194,7 @@ __global__ void __launch_bounds__(FewCfg<HD, TI, TC>::W * 32, FewCfg<HD, TI, TC>
     if (before <= u0 && u0 < before + mine) {
         unsigned long long at = before;
         for (int s = sq0; s < sq1; ++s) {
-            const unsigned long long n = kv_seq_steps<W>(a, s, bad_seq, nullptr);
+            const unsigned long long n = kv_seq_steps<W, Cfg::COST>(a, s, bad_seq, nullptr);
             if (u0 < at + n) {
                 sh.seq = s;
                 sh.at = u0 - at;
@@ -204,13 +209,13 @@ __global__ void __launch_bounds__(FewCfg<HD, TI, TC>::W * 32, FewCfg<HD, TI, TC>
     cu.s = sh.seq;
     kv_cur_seq<W>(a, cu);
     {
-        const unsigned long long r = sh.at, item = kv_div(r, cu.steps), head = kv_div(item, cu.tiles);
-        cu.step = static_cast<int>(r - item * cu.steps);
+        const unsigned long long r = sh.at, item = kv_div(r, cu.steps + Cfg::COST), head = kv_div(item, cu.tiles);
+        cu.step = static_cast<int>(r - item * (cu.steps + Cfg::COST)) - Cfg::COST;
         cu.rt = static_cast<int>(item - head * cu.tiles);
         cu.h = static_cast<int>(head);
     }
     auto advance_item = [&](KvCur &c) {
-        c.step = 0;
+        c.step = -Cfg::COST;
         if (++c.rt < c.tiles) return;
         c.rt = 0;
         if (++c.h < a.c.n_kv_heads) return;
@@ -245,7 +250,7 @@ __global__ void __launch_bounds__(FewCfg<HD, TI, TC>::W * 32, FewCfg<HD, TI, TC>
     };
     auto issue_step = [&]() {   // K of the warp's slice of step iu, if it has one
         const int sl = ic.step * W + warp;
-        if (sl < ic.sl.n) {
+        if (ic.step >= 0 && sl < ic.sl.n) {
             if (ic.s != pg_s || ic.step >= pg_base + 32 || ic.step < pg_base) {
                 pg_s = ic.s, pg_base = ic.step;
                 const int my = (ic.step + lane) * W + warp;
@@ -270,14 +275,14 @@ __global__ void __launch_bounds__(FewCfg<HD, TI, TC>::W * 32, FewCfg<HD, TI, TC>
         ++iu;
         if (++ic.step == ic.steps && iu < u1) {
             advance_item(ic);
-            // its Q towards L2 while this item still runs: a row's bytes by 128 a lane
+            // its Q towards L1 while this item still runs: a row's bytes by 128 a lane
             constexpr int LINES = HD * static_cast<int>(sizeof(I)) / 128;
             const int r = ic.rt * 8 + lane / LINES;
             if (lane < 8 * LINES && r < ic.q.n * a.group) {
                 const int tok = r / a.group;
                 const I *qp = static_cast<const I *>(a.q.p) + (ic.q.row0 + tok) * a.q.row +
                               (ic.h * a.group + (r - tok * a.group)) * a.q.head + (lane % LINES) * (128 / sizeof(I));
-                asm volatile("prefetch.global.L2 [%0];" ::"l"(qp));
+                asm volatile("prefetch.global.L1 [%0];" ::"l"(qp));
             }
         }
     };
@@ -307,11 +312,18 @@ __global__ void __launch_bounds__(FewCfg<HD, TI, TC>::W * 32, FewCfg<HD, TI, TC>
     const uint32_t vrow = (lane & 7) + (lane >> 4) * 8, vchunk = (lane >> 3) & 1;   // and of V, transposed
     for (unsigned long long u = u0; u < u1;) {
         // ---- one item, or this CTA's part of it ----
-        const bool from_start = cu.step == 0;
-        const int step0 = cu.step;
+        const int step0 = max(cu.step, 0);
         const unsigned long long left = u1 - u;
-        const int nstep = left < static_cast<unsigned>(cu.steps - cu.step) ? static_cast<int>(left) : cu.steps - cu.step;
-        const bool to_end = cu.step + nstep == cu.steps;
+        const int end = left < static_cast<unsigned>(cu.steps - cu.step) ? cu.step + static_cast<int>(left) : cu.steps;
+        const int nstep = end - step0;
+        const unsigned long long first = u - cu.step;   // the unit of the item's step 0 (cu.step may be negative)
+        if (nstep <= 0) {   // of this item the CTA has only units that stand for its cost
+            u += end - cu.step;
+            cu.step = end;
+            if (u < u1 && cu.step == cu.steps) advance_item(cu);
+            continue;
+        }
+        const bool from_start = cu.step <= 0, to_end = end == cu.steps;
         const int R = cu.q.n * a.group, p0 = cu.q.len - cu.q.n, r0 = cu.rt * 8;
         // row g of Q as the B operand; rows past the last are zero.  It is requested before
         // the ring's copies, behind which it would wait.
@@ -664,13 +676,13 @@ __global__ void __launch_bounds__(FewCfg<HD, TI, TC>::W * 32, FewCfg<HD, TI, TC>
                 if (md == 0) __stcg(mp + 8 * HD + mr, M), __stcg(mp + 8 * HD + 8 + mr, L);
             }
             // the stores are under way; that they have arrived is told later
-            tell = static_cast<int>(share.of(u - step0));
+            tell = static_cast<int>(share.of(first));
         } else {
             if (!to_end) {
                 // ---- the beginning: the other parts, of the CTAs after this one, in order.  They
                 // are waited for (as every wait, within a limit): the ranges run against blockIdx,
                 // so those CTAs were started before this one. ----
-                const unsigned others = share.of(u + cu.steps - 1) - cta;
+                const unsigned others = share.of(first + cu.steps - 1) - cta;
                 const float *part = a.part + static_cast<size_t>(cta + 1) * P;
                 if (tid == 0) {
                     uint32_t i = 0;
@@ -729,8 +741,8 @@ __global__ void __launch_bounds__(FewCfg<HD, TI, TC>::W * 32, FewCfg<HD, TI, TC>
             }
             write_out();
         }
-        u += nstep;
-        cu.step += nstep;
+        u += end - cu.step;
+        cu.step = end;
         if (u < u1) advance_item(cu);
         __syncthreads();   // merge and sh are free again
     }
