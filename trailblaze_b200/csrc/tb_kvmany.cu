@@ -37,7 +37,6 @@ namespace tb {
 
 static constexpr int kTileN = 128;      // positions of a tile
 static constexpr int kManyThreads = 384;
-static constexpr int kPolyOf8 = 3;      // of 8 pairs of scores, how many go through exp2_poly
 
 struct ManyArgs {
     AttnArgs a;
@@ -135,33 +134,6 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *map
                  "[%5];" ::"r"(dst),
                  "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
                  : "memory");
-}
-
-// 2^x for two x, on the FMA pipe: the multi-function unit gives 4 results a clock
-// and sub-core, and 128 x 128 scores would hold it as long as the tensor core
-// needs for both products.  x = n + f with n the nearest integer (by adding 1.5 *
-// 2^23), 2^f on [-0.5, 0.5] by a polynomial of least relative error (Remez
-// exchange; degree 3: 7.5e-5, 4: 2.6e-6, to be rounded to bf16 or fp16), n into
-// the exponent.  x below -126 gives about 2^-126.
-template <int DEG>
-__device__ __forceinline__ float2 exp2_poly(float2 x)
-{
-    constexpr float C3[4] = {0.9999280735f, 0.6932609855f, 0.2426111222f, 0.05517166906f};
-    constexpr float C4[5] = {0.9999992614f, 0.6931218147f, 0.2402474482f, 0.05591786032f, 0.009570101912f};
-    auto c = [&](int i) { return DEG == 3 ? make_float2(C3[i > 3 ? 0 : i], C3[i > 3 ? 0 : i]) : make_float2(C4[i], C4[i]); };
-    // a NaN stays one here and leaves as 2^127 or more, which P's rounding makes
-    // infinite: the row is then done again
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-126.f));
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-126.f));
-    const float2 big = make_float2(12582912.f, 12582912.f), nbig = make_float2(-12582912.f, -12582912.f);
-    const float2 t = __fadd2_rn(x, big);
-    const float2 n = __fadd2_rn(t, nbig);
-    const float2 f = __ffma2_rn(n, make_float2(-1.f, -1.f), x);
-    float2 p = c(DEG);
-#pragma unroll
-    for (int i = DEG - 1; i >= 0; --i) p = __ffma2_rn(p, f, c(i));
-    return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)),
-                       __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
 }
 
 // One row again, over its visible positions only, by the whole warp: res = the sum
@@ -557,18 +529,16 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                 const float nm = m == -INFINITY ? 0.f : -m;
                 const float2 sc2 = make_float2(sc, sc), nm2 = make_float2(nm, nm);
                 float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-                // P in two halves: the product of the first starts while the second is computed
+                // P in two halves: the product of the first runs while the second is computed.
+                // (All exponentials go to the multi-function unit: a polynomial on the FMA pipe for
+                // 1 to 4 of 8 measured slower, and so did a first part of three quarters.)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
 #pragma unroll
                     for (int c = h * 32; c < h * 32 + 32; ++c) {   // the pairs take the places of scores that are done with
                         float2 x = __ffma2_rn(make_float2(__uint_as_float(s[2 * c]), __uint_as_float(s[2 * c + 1])), sc2, nm2);
-                        if ((c & 7) < kPolyOf8) {
-                            x = exp2_poly<BF ? 3 : 4>(x);
-                        } else {
-                            x.x = ex2(x.x);
-                            x.y = ex2(x.y);
-                        }
+                        x.x = ex2(x.x);
+                        x.y = ex2(x.y);
                         sum[c & 1] = __fadd2_rn(sum[c & 1], x);
                         if constexpr (BF) {
                             const __nv_bfloat162 w = __floats2bfloat162_rn(x.x, x.y);
