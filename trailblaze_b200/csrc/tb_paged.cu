@@ -2,6 +2,7 @@
 // append and page copies, and the rotary table (include/tb_gguf_dequant.h
 // part 4).
 #include <cstdio>
+#include <type_traits>
 #include <vector>
 
 #include "tb_paged.cuh"
@@ -66,12 +67,13 @@ struct AppendArgs {
 // elements a lane, so HD / 8 lanes hold a head and a warp HW = 256 / HD of them.  A
 // lane's dimensions are the same for every head that it visits, so the token's cos
 // and sin (and the norm's weights) sit in its registers:
-//   y[d] = x[d] cos + x[partner] sin', sin' negative for a pair's first element.
-// Interleaved pairs lie in one lane; a half's partners are loaded a second time
-// (they are in L1 by then; shuffles took twice the instructions).  Bound by the
-// rows' bytes as long as enough of them are in flight: few instructions a head, two
-// heads' loads ahead a lane, the first of them before the look-up of the token's
-// sequence, page and angles.
+//   y[d] = x[d] cos + x[partner] sin', sin' negative for a pair's first element;
+// a dimension that does not rotate has cos = 1 and a partner of zero.  Interleaved pairs lie in one lane; a half's partners are loaded a second
+// time (they are in L1 by then; shuffles took twice the instructions).  The rows'
+// bytes bound it, and next the instructions, hence the forms of the loop: norm or
+// not, none, pairs, halves 8 partners together, or halves that split a lane's 8.
+enum AppendMode { TURN_NONE, TURN_PAIRS, TURN_HALVES, TURN_SPLIT };
+
 template <class E>
 struct Raw {   // 8 elements
     uint4 v[sizeof(E) / 2];
@@ -80,16 +82,21 @@ struct Raw {   // 8 elements
 #pragma unroll
         for (int i = 0; i < static_cast<int>(sizeof(E) / 2); ++i) v[i] = reinterpret_cast<const uint4 *>(p)[i];
     }
+    __device__ __forceinline__ void clear()
+    {
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(sizeof(E) / 2); ++i) v[i] = make_uint4(0, 0, 0, 0);
+    }
     __device__ __forceinline__ void set(int e, E x) { reinterpret_cast<E *>(v)[e] = x; }
     __device__ __forceinline__ void to(float (&x)[8]) const { kv_load8(reinterpret_cast<const E *>(v), x); }
 };
 
 template <int HD, int TI, int TC>
-__global__ void __launch_bounds__(256, 3) k_kv_append(const __grid_constant__ AppendArgs a)
+__global__ void __launch_bounds__(256, 2) k_kv_append(const __grid_constant__ AppendArgs a)
 {
     using I = typename KvType<TI>::E;
     using C = typename KvType<TC>::E;
-    constexpr int L = HD / 8, HW = 32 / L, U = 2;   // lanes a head, heads a warp, heads ahead
+    constexpr int L = HD / 8, HW = 32 / L, U = 4;   // lanes a head, heads a warp, heads ahead
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -106,33 +113,30 @@ __global__ void __launch_bounds__(256, 3) k_kv_append(const __grid_constant__ Ap
     const int nk = a.c.n_kv_heads, pq = (a.nh + HW - 1) / HW, pk = (nk + HW - 1) / HW;
     auto first = [&](int p) { return (part >= p ? part : part + (p - part + a.parts - 1) / a.parts * a.parts) - p; };
     const int h0 = part * HW + grp, hk = first(pq) * HW + grp, hv = first(pq + pk) * HW + grp;
-    const int half = a.rot / 2;
-    // of the lane's 8 dimensions, the first n_turn rotate; with halves, all or none of
-    // them have their partners 8 elements together, unless half is no multiple of 8
-    const int n_turn = a.table ? min(8, max(0, a.rot - d0)) : 0;
-    const bool apart = n_turn > 0 && !a.inter, together = (half & 7) == 0;
-    const int mate = d0 >= half ? -half : half;
+    const int half = a.rot / 2, n_turn = a.table ? min(8, max(0, a.rot - d0)) : 0;   // of the lane's 8, those that rotate
+    const int mode = !a.table ? TURN_NONE : a.inter ? TURN_PAIRS : (half & 7) == 0 ? TURN_HALVES : TURN_SPLIT;
+    const int mate = n_turn == 0 ? 0 : d0 >= half ? -half : half;   // TURN_HALVES
     Raw<I> x[U], z[U];
-    auto partners = [&](const I *p, Raw<I> &r) {
-        if (together) {
-            r.load(p + mate);
-        } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) r.set(e, p[e < n_turn ? (d0 + e >= half ? e - half : e + half) : e]);
-        }
-    };
-    auto load = [&](const I *p, long long inc, int h, int n, bool rotates) {
+    for (int u = 0; u < U; ++u) z[u].clear();
+    auto load = [&](auto mode_, const I *p, long long inc, int h, int n) {
+        constexpr int MODE = decltype(mode_)::value;
 #pragma unroll
         for (int u = 0; u < U; ++u)
             if (h + u * step < n) {
                 x[u].load(p + u * inc);
-                if (rotates && apart) partners(p + u * inc, z[u]);
+                if constexpr (MODE == TURN_HALVES)
+                    if (n_turn > 0) z[u].load(p + u * inc + mate);
+                if constexpr (MODE == TURN_SPLIT) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (e < n_turn) z[u].set(e, p[u * inc + e + (d0 + e >= half ? -half : half)]);
+                }
             }
         __syncwarp();   // q_out may be q: nothing is stored before its partner is read
     };
-    const long long q_inc = step * a.q.head, k_inc = step * a.k.head, v_inc = step * a.v.head;
     const I *qp = static_cast<const I *>(a.q.p) + t * a.q.row + h0 * a.q.head + d0;
-    load(qp, q_inc, h0, a.nh, true);
+    if (h0 < a.nh) asm volatile("prefetch.global.L1 [%0];" ::"l"(qp));   // on its way during the look-up
     // ---- the token's sequence, position, page and angles ----
     int s;
     if (a.b.n_seqs <= 32) {
@@ -154,103 +158,99 @@ __global__ void __launch_bounds__(256, 3) k_kv_append(const __grid_constant__ Ap
     long long at = -1;
     if (ok && (!a.table || pos < a.n_pos)) at = kv_at(a.b, a.c, s, pos, 0, a.err);
     else if (ok && lane == 0) atomicExch(a.err, ERR_RUNTIME);
+    if (at < 0) {   // nowhere to go: zeros for q
+        const float zero[8] = {};
+        I *op = static_cast<I *>(const_cast<void *>(a.o.p)) + t * a.o.row + d0;
+        for (int h = h0; h < a.nh; h += step) kv_store8(op + h * a.o.head, zero);
+        return;
+    }
     float cs[8], sn[8];
-    if (at >= 0) {
-        const float2 *row = reinterpret_cast<const float2 *>(a.table) + static_cast<long long>(pos) * half;
+    const float2 *angles = reinterpret_cast<const float2 *>(a.table) + static_cast<long long>(pos) * half;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const int d = d0 + e;
-            if (e < n_turn) {
-                const bool second = a.inter ? (e & 1) : d >= half;
-                const float2 v = __ldg(row + (a.inter ? d >> 1 : second ? d - half : d));
-                cs[e] = v.x;
-                sn[e] = second ? v.y : -v.y;
-            }
+    for (int e = 0; e < 8; ++e) {
+        const int d = d0 + e;
+        cs[e] = 1.f, sn[e] = 0.f;
+        if (e < n_turn) {
+            const bool second = a.inter ? (e & 1) : d >= half;
+            const float2 v = __ldg(angles + (a.inter ? d >> 1 : second ? d - half : d));
+            cs[e] = v.x;
+            sn[e] = second ? v.y : -v.y;
         }
     }
-    // norm (of q or k) and rotation of one head's 8 elements
-    auto turn = [&](const Raw<I> &xr, const Raw<I> &zr, const float *nw, float (&y)[8]) {
-        xr.to(y);
-        float sc = 1.f;
-        if (nw) {
-            float ss = 0.f;
+    float wd[8], wm[8];   // a norm's weights at this lane's dimensions and at their partners
+    // heads h, h + step, ... of n, from p to o
+    auto heads = [&](auto norm_, auto mode_, const I *p, long long inc, auto *o, long long o_inc, int h, int n, const float *nw) {
+        constexpr bool NORM = decltype(norm_)::value;
+        constexpr int MODE = decltype(mode_)::value;
+        if constexpr (NORM) {   // this norm's weights, in the place of the last one's
 #pragma unroll
-            for (int e = 0; e < 8; ++e) ss = fmaf(y[e], y[e], ss);
-#pragma unroll
-            for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
-            sc = 1.0f / sqrtf(ss / static_cast<float>(HD) + a.eps);
-            float wv[8];
-            kv_load8(nw + d0, wv);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) y[e] = y[e] * sc * wv[e];
-        }
-        if (n_turn == 0) return;
-        float p[8];
-        if (a.inter) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) p[e] = y[e ^ 1];
-        } else {
-            zr.to(p);
-            if (nw) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (e < n_turn) p[e] = p[e] * sc * __ldg(nw + d0 + e + (d0 + e >= half ? -half : half));
+            for (int e = 0; e < 8; ++e) {
+                const int d = d0 + e, m = e >= n_turn ? d : MODE == TURN_PAIRS ? d ^ 1 : d >= half ? d - half : d + half;
+                wd[e] = __ldg(nw + d);
+                wm[e] = __ldg(nw + m);
             }
         }
-        if (n_turn == 8) {
+        for (; h - grp < n; h += U * step, p += U * inc, o += U * o_inc) {
+            load(mode_, p, inc, h, n);
 #pragma unroll
-            for (int e = 0; e < 8; e += 2) {
-                const float2 r = __ffma2_rn(make_float2(p[e], p[e + 1]), make_float2(sn[e], sn[e + 1]),
-                                            __fmul2_rn(make_float2(y[e], y[e + 1]), make_float2(cs[e], cs[e + 1])));
-                y[e] = r.x, y[e + 1] = r.y;
+            for (int u = 0; u < U; ++u) {
+                float y[8], w[8];
+                x[u].to(y);
+                float sc = 1.f;
+                if constexpr (NORM) {
+                    float ss = 0.f;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) ss = fmaf(y[e], y[e], ss);
+#pragma unroll
+                    for (int k = L / 2; k > 0; k >>= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, k);
+                    sc = 1.0f / sqrtf(ss / static_cast<float>(HD) + a.eps);
+                }
+                if constexpr (NORM) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) y[e] *= sc * wd[e];
+                }
+                if constexpr (MODE == TURN_PAIRS) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) w[e] = e < n_turn ? y[e ^ 1] : 0.f;
+                } else if constexpr (MODE != TURN_NONE) {
+                    z[u].to(w);
+                    if constexpr (NORM) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) w[e] *= sc * wm[e];
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 8; e += 2) {
+                    if constexpr (MODE == TURN_NONE) break;
+                    const float2 r = __ffma2_rn(make_float2(w[e], w[e + 1]), make_float2(sn[e], sn[e + 1]),
+                                                __fmul2_rn(make_float2(y[e], y[e + 1]), make_float2(cs[e], cs[e + 1])));
+                    y[e] = r.x, y[e + 1] = r.y;
+                }
+                if (h + u * step < n) kv_store8(o + u * o_inc, y);
             }
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (e < n_turn) y[e] = fmaf(p[e], sn[e], y[e] * cs[e]);
         }
     };
     I *op = static_cast<I *>(const_cast<void *>(a.o.p)) + t * a.o.row + h0 * a.o.head + d0;
-    const long long o_inc = step * a.o.head;
-    for (int h = h0; h - grp < a.nh; h += U * step, qp += U * q_inc, op += U * o_inc) {
-        if (h != h0) load(qp, q_inc, h, a.nh, true);
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            float y[8];
-            turn(x[u], z[u], a.qn, y);
-            if (h + u * step < a.nh) {
-                if (at < 0) {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) y[e] = 0.f;
-                }
-                kv_store8(op + u * o_inc, y);
-            }
-        }
-    }
-    if (at < 0) return;
     const I *kp = static_cast<const I *>(a.k.p) + t * a.k.row + hk * a.k.head + d0;
     const I *vp = static_cast<const I *>(a.v.p) + t * a.v.row + hv * a.v.head + d0;
-    const long long c_inc = step * a.c.head_stride;
     C *kc = static_cast<C *>(const_cast<void *>(a.c.k)) + at + hk * a.c.head_stride + d0;
     C *vc = static_cast<C *>(const_cast<void *>(a.c.v)) + at + hv * a.c.head_stride + d0;
-    for (int h = hk; h - grp < nk; h += U * step, kp += U * k_inc, kc += U * c_inc) {
-        load(kp, k_inc, h, nk, true);
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            float y[8];
-            turn(x[u], z[u], a.kn, y);
-            if (h + u * step < nk) kv_store8(kc + u * c_inc, y);
-        }
-    }
-    for (int h = hv; h - grp < nk; h += U * step, vp += U * v_inc, vc += U * c_inc) {
-        load(vp, v_inc, h, nk, false);
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            float y[8];
-            x[u].to(y);
-            if (h + u * step < nk) kv_store8(vc + u * c_inc, y);
-        }
-    }
+    const long long q_inc = step * a.q.head, k_inc = step * a.k.head, v_inc = step * a.v.head;
+    const long long o_inc = step * a.o.head, c_inc = step * a.c.head_stride;
+    using std::integral_constant;
+    auto all = [&](auto MODE) {
+        using T1 = integral_constant<bool, true>;
+        using T0 = integral_constant<bool, false>;
+        if (a.qn) heads(T1(), MODE, qp, q_inc, op, o_inc, h0, a.nh, a.qn);
+        else heads(T0(), MODE, qp, q_inc, op, o_inc, h0, a.nh, a.qn);
+        if (a.kn) heads(T1(), MODE, kp, k_inc, kc, c_inc, hk, nk, a.kn);
+        else heads(T0(), MODE, kp, k_inc, kc, c_inc, hk, nk, a.kn);
+        heads(T0(), integral_constant<int, TURN_NONE>(), vp, v_inc, vc, c_inc, hv, nk, nullptr);
+    };
+    if (mode == TURN_HALVES) all(integral_constant<int, TURN_HALVES>());
+    else if (mode == TURN_PAIRS) all(integral_constant<int, TURN_PAIRS>());
+    else if (mode == TURN_NONE) all(integral_constant<int, TURN_NONE>());
+    else all(integral_constant<int, TURN_SPLIT>());
 }
 
 template <int HD, int TI>
@@ -272,10 +272,11 @@ int kv_append_launch(const KvView &c, const KvBatch &b, int hd, int ti, int tc, 
                                                                                   : append_kernel<128, QT_BF16>(tc))
                          : (ti == QT_F32 ? append_kernel<64, QT_F32>(tc) : ti == QT_F16 ? append_kernel<64, QT_F16>(tc)
                                                                                  : append_kernel<64, QT_BF16>(tc));
-    // a token's heads over several warps until the GPU has four waves of them (8192 tokens
-    // of 48 heads: 53 us in 1.7 waves), at most a pass each
+    // A token's heads over several warps until the GPU has two waves of 16 an SM, at most
+    // a pass each (8192 tokens of 48 heads: 47 us with four heads ahead at two CTAs an SM,
+    // 52 with two at three CTAs and four waves, 105 with a CTA a token).
     const int hw = 256 / hd, passes = (nh + hw - 1) / hw + 2 * ((c.n_kv_heads + hw - 1) / hw);
-    const int parts = (4 * 24 * sms + b.n_tokens - 1) / b.n_tokens;
+    const int parts = (2 * 16 * sms + b.n_tokens - 1) / b.n_tokens;
     a.parts = parts > passes ? passes : parts;
     const long long warps = static_cast<long long>(b.n_tokens) * a.parts;
     void *args[] = {&a};
