@@ -413,7 +413,7 @@ typedef struct {
  * the most new tokens and positions of any sequence; they only choose between
  * kernels, and the results are right for any value.
  * A sequence whose range leaves [0, n_tokens], whose new tokens outnumber its
- * positions or whose positions outnumber its table's sets the error word (2)
+ * positions or whose positions outnumber its table's (or 2^31 - 256) sets the error word (2)
  * and is skipped, its rows of the output zero; so does a page outside the
  * pool, whose positions then count as hidden and are not stored to. */
 typedef struct {

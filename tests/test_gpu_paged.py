@@ -257,6 +257,26 @@ def test_bad_tables_are_errors_not_faults(paged, kq):
             assert bool((qo[2:5] == 0).all()) or "page" in what
 
 
+@pytest.mark.parametrize("io", [F32, BF16])
+def test_bad_page_of_a_split_chunk(paged, kq, io):
+    """A page outside the pool in a chunk whose positions are shared out over several CTAs: its positions are
+    hidden from every row, whichever CTA joins the parts."""
+    c = Case(paged, [256], [1500], 4, 1, 64, io, io, 16, seed=21)
+    for bad in (3, 40, 70):   # seen by all rows
+        table = c.table.to(torch.int32).clone()
+        table[0, bad] = -5
+        b = paged.Batch(torch.tensor(c.start, dtype=torch.int32, device="cuda"),
+                        torch.tensor(c.lens, dtype=torch.int32, device="cuda"), table, 256, 256, 1500)
+        out = c.cache.attend(1, b, c.q)
+        torch.cuda.synchronize()
+        assert kq.tb_cuda_last_error() == 2
+        rows = [0, 1, 100, 255]   # without the page the other positions close up: same scores, 16 fewer
+        keep = torch.cat([c.table[0, :bad], c.table[0, bad + 1:94]])
+        ref, bound = R.attend(c.q[rows], c.k[1], c.v[1], [0, 1, 2, 3, 4], [1500 - 256 + r + 1 - 16 for r in rows],
+                              [keep] * 4, 1 / 8)
+        assert bool(((out[rows].double() - ref).abs() <= bound).all()), bad
+
+
 @pytest.mark.parametrize("n", [0, 1])
 def test_empty_batches(paged, kq, n):
     c = Case(paged, [0] * n, [7] * n, 4, 2, 64, BF16, BF16, 16, seed=11)

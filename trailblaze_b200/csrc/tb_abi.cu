@@ -655,8 +655,8 @@ int tb_cuda_kv_attend_dev(const tb_kv_cache *cache, int layer, const tb_kv_batch
     const int ok = tb::kv_attend_launch(kv_view(cache, layer), kv_batch(batch), hd, io_type, cache->type, n_heads,
                                         kv_rows(q), kv_rows(out), scale, window, sinks, batch->max_new, batch->max_len,
                                         d_ws, derr, nsm, lim, static_cast<cudaStream_t>(stream));
-    if (ok) g_launches.fetch_add(1, std::memory_order_relaxed);
-    return ok;
+    g_launches.fetch_add(ok, std::memory_order_relaxed);   // one, or two for a mixed batch
+    return ok > 0 ? 1 : 0;
 }
 
 int tb_cuda_kv_copy_dev(const tb_kv_cache *cache, const int *src, const int *dst, int n, void *stream)

@@ -817,6 +817,7 @@ int kv_attend_launch(const KvView &c, const KvBatch &b, int hd, int ti, int tc, 
     a.arrived = static_cast<unsigned *>(ws);
     a.part = reinterpret_cast<float *>(static_cast<char *>(ws) + kCounterBytes);
     a.many_rows = 0x7FFFFFFF;
+    int before = 0;   // launches
     // Chunks go to the kernels with 128-row tiles: the tcgen05 one for 16-bit
     // activations over a cache of their type (whole tokens in 128 rows, a scale that
     // keeps the order of scores), the other one else.  Where the batch holds short
@@ -830,8 +831,10 @@ int kv_attend_launch(const KvView &c, const KvBatch &b, int hd, int ti, int tc, 
         if (r < 0) r = kv_wide_launch(a, hd, ti, tc, few_rows, sms, st);
         if (r == 0 || !mixed) return r;
         a.many_rows = kFewRows;
+        before = 1;
     }
-    return hd == 128 ? few<128>(a, ti, tc, sms, st) : few<64>(a, ti, tc, sms, st);
+    const int r = hd == 128 ? few<128>(a, ti, tc, sms, st) : few<64>(a, ti, tc, sms, st);
+    return r ? r + before : 0;
 }
 
 }  // namespace tb

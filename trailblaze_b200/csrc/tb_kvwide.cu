@@ -439,13 +439,16 @@ __global__ void __launch_bounds__(kWThreads, 1)
                 for (int o = 4; o < 32; o <<= 1) l[nt][e] += __shfl_xor_sync(0xFFFFFFFFu, l[nt][e], o);
         if (j0 > 0) {
             // not the item's beginning: the part goes to the CTA that has it, as the threads hold it
+            // (a page outside the pool: as NaN, so that the rows are done again there)
+            const bool bad = *reinterpret_cast<volatile int *>(&sh.bad) != 0;
             float4 *mp = reinterpret_cast<float4 *>(aa.part + static_cast<size_t>(my.cta) * Cfg::PART) + tid;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
                 for (int i = 0; i < HD / 16; ++i)
                     __stcg(mp + (nt * (HD / 16) + i) * kWThreads, make_float4(O[nt][i][0], O[nt][i][1], O[nt][i][2], O[nt][i][3]));
-                __stcg(mp + (NT * (HD / 16) + nt) * kWThreads, make_float4(m[nt][0], m[nt][1], l[nt][0], l[nt][1]));
+                __stcg(mp + (NT * (HD / 16) + nt) * kWThreads, 
+                       bad ? make_float4(m[nt][0], m[nt][1], NAN, NAN) : make_float4(m[nt][0], m[nt][1], l[nt][0], l[nt][1]));
             }
             tell = static_cast<int>(my.share.of(u - j0));
         } else {

@@ -68,10 +68,13 @@ struct AppendArgs {
 // lane's dimensions are the same for every head that it visits, so the token's cos
 // and sin (and the norm's weights) sit in its registers:
 //   y[d] = x[d] cos + x[partner] sin', sin' negative for a pair's first element;
-// a dimension that does not rotate has cos = 1 and a partner of zero.  Interleaved pairs lie in one lane; a half's partners are loaded a second
-// time (they are in L1 by then; shuffles took twice the instructions).  The rows'
-// bytes bound it, and next the instructions, hence the forms of the loop: norm or
-// not, none, pairs, halves 8 partners together, or halves that split a lane's 8.
+// a dimension that does not rotate has cos = 1 and a partner of zero.  Interleaved
+// pairs lie in one lane; a half's partners are loaded a second time (they are in L1 by
+// then; shuffles took twice the instructions).  The rows' bytes bound it, and next the
+// instructions, hence the forms of the loop: norm or not; no rotation, pairs, halves
+// whose partners lie 8 together, or halves that split a lane's 8.  8192 tokens of 32 q
+// and 8 kv bf16 heads, half of each rotated: 47 us, 4.3 TB/s of 6.5 that a copy
+// reaches; one token: 4.3 us, the launch and a chain of five loads.
 enum AppendMode { TURN_NONE, TURN_PAIRS, TURN_HALVES, TURN_SPLIT };
 
 template <class E>

@@ -30,7 +30,7 @@ struct KvRows {
 };
 
 // Launchers (tb_paged.cu, tb_kvattn.cu): arguments checked by the C entry
-// points; 1 = launched.  hd: head_dim, ti / tc: types of the rows and the cache.
+// points; 1 = launched (attention: the number of launches).  hd: head_dim, ti / tc: types of the rows and the cache.
 int rope_table_launch(float *t, int n_pos, int rot, double base, double factor, double fast, double slow,
                       double orig_len, double attn, int mode, cudaStream_t st);
 int kv_append_launch(const KvView &c, const KvBatch &b, int hd, int ti, int tc, int nh, const KvRows &q,
@@ -135,7 +135,8 @@ __device__ __forceinline__ bool kv_seq(const KvBatch &b, const KvView &c, int s,
     q.row0 = a;
     q.n = e - a;
     q.len = b.len[s];
-    const bool ok = a >= 0 && e >= a && e <= b.n_tokens && q.len >= 0 && q.n <= q.len &&
+    // (lengths near 2^31 would overflow where they are rounded up to tiles)
+    const bool ok = a >= 0 && e >= a && e <= b.n_tokens && q.len >= 0 && q.len <= 0x7FFFFF00 && q.n <= q.len &&
                     q.len <= static_cast<long long>(b.pages_stride) * c.page_size;
     if (!ok && err) atomicExch(err, ERR_RUNTIME);
     return ok;
