@@ -8,8 +8,9 @@
 // (G = query heads per kv head) is new token r / G, head r % G of the group.  Its
 // positions come in slices of 16 (16 divides a page), a step is one slice for
 // each of the CTA's W warps.  All items' steps (and some more for each item's own
-// cost), laid end to end, are cut into equal parts, one per CTA, whatever the sequences' lengths: a CTA works through
-// the end of one item, whole items, and the beginning of another.  Items that lie
+// cost), laid end to end, are cut into equal parts, one per CTA, whatever the
+// sequences' lengths: a CTA works through the end of one item, whole items, and the
+// beginning of another.  Items that lie
 // in one CTA are written out directly, the others' parts go through the workspace to
 // the CTA that has the item's beginning, which adds them in CTA order, so results
 // repeat bit for bit.
@@ -28,6 +29,11 @@
 // so that its largest element is near 2^13); an fp32 cache is split into two
 // tf32 parts, of which the low-low product is dropped (2^-22).  Scores, softmax and
 // sums are fp32.
+//
+// Measured (8 kv heads of 128, 4 query heads each): 64 sequences of up to 16384 bf16
+// positions, 2.07 GB, in 306 us, 6.76 TB/s, what a copy reaches; one sequence of 4096
+// fp32 positions, 33.6 MB, in 19 us against 5 us of bytes: launch, scan, the first
+// page, Q and the joining of 16 parts stand one behind the other there.
 #include "tb_kvattn.cuh"
 
 namespace tb {
@@ -769,9 +775,21 @@ size_t kv_attend_ws()
     return kCounterBytes + n;
 }
 
-// Query rows per kv head up to which a sequence's attention is bound by the
-// cache's bytes in k_kv_few.
-static constexpr int kFewRows = 16;
+// Query rows per kv head up to which a sequence goes to k_kv_few, which passes over
+// the cache once for 8 rows; the chunk kernels take as long for one row as for their
+// tile.  Measured at 4096 positions, 8 kv heads of 128, 4 query heads each:
+//                 1 sequence            16 sequences
+//   rows        8    16   32   64       8    16    32    64
+//   bf16 few   17    17   21   30      59    90   169   312   us
+//        many  29    29   30   29      70    71    72    73
+//   f32  few   20    27   41   64     125   232   441   848
+//        wide  52    52   52   56     471   470   473   480
+// In k_kv_many's types the crossing moves with the load (sequences x kv heads), from
+// past 32 rows to past 8; in the others it stays past 32.
+static int few_rows_of(bool many, long long load)
+{
+    return !many || load < 24 ? 32 : load < 96 ? 16 : 8;
+}
 
 template <int HD, int TI, int TC>
 static int few_launch(AttnArgs &a, int sms, cudaStream_t st)
@@ -823,14 +841,15 @@ int kv_attend_launch(const KvView &c, const KvBatch &b, int hd, int ti, int tc, 
     // keeps the order of scores), the other one else.  Where the batch holds short
     // sequences besides, k_kv_few runs too and each takes its own; which sequences those
     // are is decided on the device.
-    if (a.group <= 128 && static_cast<long long>(max_new) * a.group > kFewRows) {
+    const bool many = ti == tc && tc != QT_F32 && scale > 0.f;
+    const int rows = few_rows_of(many, static_cast<long long>(b.n_seqs) * c.n_kv_heads);
+    if (a.group <= 128 && static_cast<long long>(max_new) * a.group > rows) {
         const bool mixed = b.n_tokens < static_cast<long long>(b.n_seqs) * max_new;
-        const int few_rows = mixed ? kFewRows : 0;
-        int r = -1;
-        if (ti == tc && tc != QT_F32 && scale > 0.f) r = kv_many_launch(a, hd, tc, few_rows, sms, st);
+        const int few_rows = mixed ? rows : 0;
+        int r = many ? kv_many_launch(a, hd, tc, few_rows, sms, st) : -1;
         if (r < 0) r = kv_wide_launch(a, hd, ti, tc, few_rows, sms, st);
         if (r == 0 || !mixed) return r;
-        a.many_rows = kFewRows;
+        a.many_rows = rows;
         before = 1;
     }
     const int r = hd == 128 ? few<128>(a, ti, tc, sms, st) : few<64>(a, ti, tc, sms, st);

@@ -247,7 +247,7 @@ __device__ __forceinline__ unsigned long long kv_head_units(const AttnArgs &a, i
 }
 
 struct KvScan {   // shared
-    unsigned long long warp[12];
+    unsigned long long warp[12], items[12];
     int seq, head, rt, off;   // the CTA's first item and its first unit there
 };
 struct KvCtaShare {
@@ -259,13 +259,15 @@ struct KvCtaShare {
 
 // The CTA's share of all units, by a scan over the sequences; false when it has none.
 // The first item is in sh after the caller's next __syncthreads().
-template <int TILE, int WARPS, int HD, class I>
+// A CTA for every item, or more, with at least MIN units each: what a finer cut saves
+// in products it spends on joining parts.
+template <int TILE, int MIN, int WARPS, int HD, class I>
 __device__ __forceinline__ bool kv_items_share(const AttnArgs &a, int tpi, int few_rows, KvScan &sh, KvCtaShare &my)
 {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int per = (a.b.n_seqs + WARPS * 32 - 1) / (WARPS * 32);
     const int sq0 = min(a.b.n_seqs, tid * per), sq1 = min(a.b.n_seqs, sq0 + per);
-    unsigned long long mine = 0;
+    unsigned long long mine = 0, items = 0;
     bool bad_seq = false;
     for (int k = 0; k < per; ++k) {
         KvSeq q{};
@@ -274,6 +276,7 @@ __device__ __forceinline__ bool kv_items_share(const AttnArgs &a, int tpi, int f
             if (!kv_item_seq(a, few_rows, sq0 + k, q)) q.n = 0;
         }
         mine += kv_head_units<TILE>(a, tpi, q) * a.c.n_kv_heads;
+        items += static_cast<unsigned long long>((q.n + tpi - 1) / tpi) * a.c.n_kv_heads;
     }
     unsigned long long incl = mine;
 #pragma unroll
@@ -281,14 +284,18 @@ __device__ __forceinline__ bool kv_items_share(const AttnArgs &a, int tpi, int f
         const unsigned long long x = __shfl_up_sync(0xFFFFFFFFu, incl, o);
         if (lane >= o) incl += x;
     }
-    if (lane == 31) sh.warp[warp] = incl;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) items += __shfl_xor_sync(0xFFFFFFFFu, items, o);
+    if (lane == 31) sh.warp[warp] = incl, sh.items[warp] = items;
     if (__syncthreads_or(bad_seq) && blockIdx.x == 0) kv_zero_bad<HD, I>(a);
-    unsigned long long before = incl - mine, total = 0;
+    unsigned long long before = incl - mine, total = 0, most = 0;
     for (int w = 0; w < WARPS; ++w) {
         before += w < warp ? sh.warp[w] : 0;
         total += sh.warp[w];
+        most += sh.items[w];
     }
-    const unsigned G = total < gridDim.x ? static_cast<unsigned>(total) : gridDim.x;
+    most = max(most, (total + MIN - 1) / MIN);
+    const unsigned G = most < gridDim.x ? static_cast<unsigned>(most) : gridDim.x;
     if (blockIdx.x >= G) return false;
     my.cta = G - 1 - blockIdx.x;
     my.share = KvShare(total, G);

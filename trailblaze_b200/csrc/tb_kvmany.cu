@@ -31,12 +31,20 @@
 // type for the second product, whose unit takes nothing wider: 2^-9 (bf16) of
 // each term, unbiased, about what the output's own rounding is; sums are fp32 of
 // the unrounded P.
+//
+// Measured (32 query and 8 kv heads of 128, bf16): 8192 tokens from the start in 504
+// us, 1092 TFLOP/s of the pairs that are seen; 512 tokens at 4096 in 48 us.  A unit
+// takes some 3000 cycles, 2048 of them tensor pipe: what is left is the way from the
+// last P over P V and the next S back to the softmax warps (1200) and their 128
+// exponentials a row (1024 of the multi-function unit), which the other group's
+// products cover in part.
 #include "tb_kvattn.cuh"
 
 namespace tb {
 
 static constexpr int kTileN = 128;      // positions of a tile
 static constexpr int kManyThreads = 384;
+static constexpr int kManyMin = 3;      // units of a CTA, at least (16 tokens at 4096: 29 us; with 1: 62)
 
 struct ManyArgs {
     AttnArgs a;
@@ -198,7 +206,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     KvCtaShare my;
-    if (!kv_items_share<kTileN, kManyThreads / 32, HD, I>(a.a, a.tpi, a.few_rows, sh.scan, my)) return;
+    if (!kv_items_share<kTileN, kManyMin, kManyThreads / 32, HD, I>(a.a, a.tpi, a.few_rows, sh.scan, my)) return;
     if (warp == 8) {
         tmem_alloc(smem_u32(&sh.tmem), 512);
         tmem_relinquish();
@@ -568,13 +576,17 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                     uint32_t o[32];
                     tmem_ld32(to + c, o);
                     tmem_wait_ld(o);
+                    if (on) {
 #pragma unroll
-                    for (int i = 0; i < 32; i += 4)
-                        __stcg(reinterpret_cast<uint4 *>(part) + ((c + i) / 4) * 256, make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]));
+                        for (int i = 0; i < 32; i += 4)
+                            __stcg(reinterpret_cast<uint4 *>(part) + ((c + i) / 4) * 256, make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]));
+                    }
                 }
                 part += 256 * HD - row * 3;
-                __stcg(part, m);
-                __stcg(part + 256, *reinterpret_cast<volatile int *>(&sh.bad) ? NAN : l);
+                if (on) {   // rows that there are not stay out of the traffic
+                    __stcg(part, m);
+                    __stcg(part + 256, *reinterpret_cast<volatile int *>(&sh.bad) ? NAN : l);
+                }
                 // the stores are under way; that they have arrived is told later
                 tell = static_cast<int>(it.peer);
             } else {
@@ -601,10 +613,13 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                         __threadfence();
                     }
                     if (!join()) break;
-                    for (unsigned c = 0; c < others; ++c) M = fmaxf(M, __ldcg(part + c * Cfg::PART + 256 * HD + row));
+                    const unsigned mine_others = on ? others : 0;
+#pragma unroll 4
+                    for (unsigned c = 0; c < mine_others; ++c) M = fmaxf(M, __ldcg(part + c * Cfg::PART + 256 * HD + row));
                     const float f = m == -INFINITY ? 0.f : ex2(m - M);
                     L = m == -INFINITY ? l : f * l;
-                    for (unsigned c = 0; c < others; ++c) {
+#pragma unroll 4
+                    for (unsigned c = 0; c < mine_others; ++c) {
                         const float *pp = part + c * Cfg::PART + 256 * HD + row;
                         const float pm = __ldcg(pp), pl = __ldcg(pp + 256);
                         L += pm == -INFINITY ? pl : ex2(pm - M) * pl;
@@ -621,7 +636,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
 #pragma unroll
                         for (int i = 0; i < 64; ++i) x[i] *= f;
 #pragma unroll 1
-                        for (unsigned k = 0; k < others; ++k) {
+                        for (unsigned k = 0; k < mine_others; ++k) {
                             const float *pp = part + k * Cfg::PART + row * 4;
                             float4 v[16];
 #pragma unroll
