@@ -188,7 +188,7 @@ class PagedKV:
                               st[2], st[3])
         self._ref = ctypes.byref(self.struct)
         self.n_layers, self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = k.shape
-        self.pool = PagePool(n_pages, page)
+        self._pool: PagePool | None = None
         self._ws: dict[int, tuple] = {}   # by stream: calls that may overlap have one each
 
     @classmethod
@@ -198,6 +198,14 @@ class PagedKV:
         return cls(torch.empty(shape, dtype=dtype, device=device), torch.empty(shape, dtype=dtype, device=device))
 
     # ---- the sequences ----
+    @property
+    def pool(self) -> PagePool:
+        """The bookkeeping of this cache's pages, made at its first use (a caller with page tables of its
+        own has none)."""
+        if self._pool is None:
+            self._pool = PagePool(self.n_pages, self.page_size)
+        return self._pool
+
     def extend(self, new: dict[int, int]) -> None:
         """Room for new[seq] more positions of each sequence; part-filled pages that are shared are copied."""
         moves = [m for m in (self.pool.extend(s, n) for s, n in new.items()) if m]
