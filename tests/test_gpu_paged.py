@@ -212,6 +212,18 @@ def test_repeatable_and_streams(paged, kq):
     assert all(torch.equal(o, want) for o in outs)
 
 
+@pytest.mark.parametrize("heads,kv_heads", [(12, 4), (25, 5), (28, 4), (5, 1), (33, 3)])
+def test_repeatable_chunks_of_odd_groups(paged, kq, heads, kv_heads):
+    """Groups of heads that do not divide a row tile leave rows unused; what lies there must not show."""
+    c = Case(paged, [300, 33, 1, 70], [900, 33, 500, 1234], heads, kv_heads, 64, BF16, BF16, 16, seed=22)
+    want = c.cache.attend(1, c.batch, c.q)
+    c.check(want)
+    other = Case(paged, [128], [512], 8, 1, 64, BF16, BF16, 16, seed=23)
+    for i in range(12):
+        other.cache.attend(1, other.batch, other.q * (10.0 ** (i - 6)))   # other leftovers in shared memory
+        assert torch.equal(c.cache.attend(1, c.batch, c.q), want)
+
+
 def test_bad_tables_are_errors_not_faults(paged, kq):
     """Ranges, lengths and pages that cannot be: the error word is set, the sequence's rows are zero (a page
     outside the pool only hides its positions), the other sequences are right."""

@@ -517,7 +517,9 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                     mxs[(c >> 1) & 3] = fmaxf(fmaxf(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), mxs[(c >> 1) & 3]);
                 float mx = fmaxf(fmaxf(mxs[0], mxs[1]), fmaxf(mxs[2], mxs[3]));
                 mx *= sc;
-                if (__any_sync(0xFFFFFFFFu, mx > m + 8.f)) {
+                // (rows that there are not hold whatever shared memory held: they have no say in
+                // when the others rescale, or results would not repeat)
+                if (__any_sync(0xFFFFFFFFu, on && mx > m + 8.f)) {
                     const float mn = fmaxf(m, mx);
                     const float corr = m == -INFINITY ? 0.f : ex2(m - mn);
                     l *= corr;
