@@ -182,6 +182,9 @@ class PagedKV:
         self.L = lib()
         self.k, self.v, self.device = k, v, k.device
         n_layers, n_pages, heads, page, dim = k.shape
+        if 0 in k.shape or page % 16 or page > 65536 or dim not in (64, 128):
+            raise ValueError(f"a cache of shape {tuple(k.shape)}: pages of a multiple of 16 positions up to 65536, heads "
+                             "of 64 or 128 dimensions expected")
         # a dimension of one element has no stride of its own
         st = [s if n > 1 else dim for s, n in zip(k.stride(), k.shape)]
         self.struct = KvCache(k.data_ptr(), v.data_ptr(), _type(k), n_layers, n_pages, page, heads, dim, st[0], st[1],
