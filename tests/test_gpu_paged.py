@@ -224,6 +224,18 @@ def test_repeatable_chunks_of_odd_groups(paged, kq, heads, kv_heads):
         assert torch.equal(c.cache.attend(1, c.batch, c.q), want)
 
 
+@pytest.mark.parametrize("cache", [F32, BF16])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(12, 4, 64), (25, 5, 128), (28, 4, 128)])
+def test_repeatable_fp32_chunks(paged, kq, cache, heads, kv_heads, dim):
+    c = Case(paged, [300, 33, 1, 70], [900, 33, 500, 1234], heads, kv_heads, dim, F32, cache, 16, seed=24)
+    want = c.cache.attend(1, c.batch, c.q)
+    c.check(want)
+    other = Case(paged, [128], [512], 8, 1, 64, F32, cache, 16, seed=25)
+    for i in range(12):
+        other.cache.attend(1, other.batch, other.q * (10.0 ** (i - 6)))
+        assert torch.equal(c.cache.attend(1, c.batch, c.q), want)
+
+
 def test_bad_tables_are_errors_not_faults(paged, kq):
     """Ranges, lengths and pages that cannot be: the error word is set, the sequence's rows are zero (a page
     outside the pool only hides its positions), the other sequences are right."""

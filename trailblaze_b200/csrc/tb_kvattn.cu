@@ -771,7 +771,7 @@ size_t kv_attend_ws()
 {
     size_t n = sizeof(float) * kMaxCtas * few_part(128);
     if (n < kManyCtas * kv_many_part_bytes()) n = kManyCtas * kv_many_part_bytes();
-    if (n < kManyCtas * kv_wide_part_bytes()) n = kManyCtas * kv_wide_part_bytes();
+    if (n < kManyCtas * kv_tf32_part_bytes()) n = kManyCtas * kv_tf32_part_bytes();
     return kCounterBytes + n;
 }
 
@@ -783,12 +783,15 @@ size_t kv_attend_ws()
 //   bf16 few   17    17   21   30      59    90   169   312   us
 //        many  29    29   30   29      70    71    72    73
 //   f32  few   20    27   41   64     125   232   441   848
-//        wide  52    52   52   56     471   470   473   480
-// In k_kv_many's types the crossing moves with the load (sequences x kv heads), from
-// past 32 rows to past 8; in the others it stays past 32.
-static int few_rows_of(bool many, long long load)
+//        tf32  65    65   64   63     195   196   197   199
+//   f32 over bf16
+//        few         19   25   36           108   203   390
+//        tf32        64   62   62           147   148   150
+// The crossing moves with the load (sequences x kv heads), from past 32 rows to past 8; a
+// 16-bit cache under other activations, cheap in k_kv_few, leaves it at 16.
+static int few_rows_of(bool narrow, long long load)
 {
-    return !many || load < 24 ? 32 : load < 96 ? 16 : 8;
+    return load < 24 ? 32 : load < 96 || narrow ? 16 : 8;
 }
 
 template <int HD, int TI, int TC>
@@ -842,12 +845,12 @@ int kv_attend_launch(const KvView &c, const KvBatch &b, int hd, int ti, int tc, 
     // sequences besides, k_kv_few runs too and each takes its own; which sequences those
     // are is decided on the device.
     const bool many = ti == tc && tc != QT_F32 && scale > 0.f;
-    const int rows = few_rows_of(many, static_cast<long long>(b.n_seqs) * c.n_kv_heads);
+    const int rows = few_rows_of(!many && tc != QT_F32, static_cast<long long>(b.n_seqs) * c.n_kv_heads);
     if (a.group <= 128 && static_cast<long long>(max_new) * a.group > rows) {
         const bool mixed = b.n_tokens < static_cast<long long>(b.n_seqs) * max_new;
         const int few_rows = mixed ? rows : 0;
         int r = many ? kv_many_launch(a, hd, tc, few_rows, sms, st) : -1;
-        if (r < 0) r = kv_wide_launch(a, hd, ti, tc, few_rows, sms, st);
+        if (r < 0) r = kv_tf32_launch(a, hd, ti, tc, few_rows, sms, st);
         if (r == 0 || !mixed) return r;
         a.many_rows = rows;
         before = 1;

@@ -1,4 +1,4 @@
-// tb_kvattn.cuh — what the two attention kernels over the paged cache share.
+// tb_kvattn.cuh — what the attention kernels over the paged cache share.
 #pragma once
 
 #include <cmath>
@@ -29,9 +29,9 @@ struct AttnArgs {
 static constexpr int kManyCtas = 160;
 size_t kv_many_part_bytes();   // a partial result
 int kv_many_launch(AttnArgs a, int hd, int tc, int few_rows, int sms, cudaStream_t st);
-// The same of k_kv_wide (tb_kvwide.cu), for any types.
-size_t kv_wide_part_bytes();
-int kv_wide_launch(AttnArgs a, int hd, int ti, int tc, int few_rows, int sms, cudaStream_t st);
+// The same of k_kv_tf32 (tb_kvtf32.cu), for any types.
+size_t kv_tf32_part_bytes();
+int kv_tf32_launch(AttnArgs a, int hd, int ti, int tc, int few_rows, int sms, cudaStream_t st);
 
 __device__ __forceinline__ float ex2(float x)   // 2^x, 2 ulp; 0 for -inf
 {
@@ -148,6 +148,36 @@ __device__ __forceinline__ uint32_t pack16(float &x, float &y)
     return w;
 }
 
+// ---- TMEM ----
+#define TB_R32(r)                                                                                                       \
+    "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),       \
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),     \
+        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),     \
+        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+#define TB_W32(c, r)                                                                                                    \
+    c(r[0]), c(r[1]), c(r[2]), c(r[3]), c(r[4]), c(r[5]), c(r[6]), c(r[7]), c(r[8]), c(r[9]), c(r[10]), c(r[11]),       \
+        c(r[12]), c(r[13]), c(r[14]), c(r[15]), c(r[16]), c(r[17]), c(r[18]), c(r[19]), c(r[20]), c(r[21]), c(r[22]),   \
+        c(r[23]), c(r[24]), c(r[25]), c(r[26]), c(r[27]), c(r[28]), c(r[29]), c(r[30]), c(r[31])
+#define TB_LIST32                                                                                                       \
+    "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, "   \
+    "%24, %25, %26, %27, %28, %29, %30, %31}"
+__device__ __forceinline__ void tmem_ld32(uint32_t at, uint32_t *r)
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 " TB_LIST32 ", [%32];" : TB_W32("=r", r) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t at, const uint32_t *r)
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], " TB_LIST32 ";" ::TB_R32(r), "r"(at) : "memory");
+}
+// The loads before it are complete; the registers pass through, so that nothing
+// that uses them moves ahead.
+__device__ __forceinline__ void tmem_wait_ld(uint32_t *r)
+{
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : TB_W32("+r", r)::"memory");
+}
+__device__ __forceinline__ void after_wait(uint32_t *r) { asm volatile("" : TB_W32("+r", r)::"memory"); }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
 // The rows of sequences whose numbers contradict each other: the error word, and
 // zeros as far as the rows exist (one CTA, all its threads).
 template <int HD, class I>
@@ -247,7 +277,7 @@ __device__ __forceinline__ unsigned long long kv_head_units(const AttnArgs &a, i
 }
 
 struct KvScan {   // shared
-    unsigned long long warp[12], items[12];
+    unsigned long long warp[16], items[16];
     int seq, head, rt, off;   // the CTA's first item and its first unit there
 };
 struct KvCtaShare {
