@@ -839,9 +839,9 @@ int kv_attend_launch(const KvView &c, const KvBatch &b, int hd, int ti, int tc, 
     a.part = reinterpret_cast<float *>(static_cast<char *>(ws) + kCounterBytes);
     a.many_rows = 0x7FFFFFFF;
     int before = 0;   // launches
-    // Chunks go to the kernels with 128-row tiles: the tcgen05 one for 16-bit
+    // Chunks go to the kernels with 128-row tiles: k_kv_many for 16-bit
     // activations over a cache of their type (whole tokens in 128 rows, a scale that
-    // keeps the order of scores), the other one else.  Where the batch holds short
+    // keeps the order of scores), k_kv_tf32 else.  Where the batch holds short
     // sequences besides, k_kv_few runs too and each takes its own; which sequences those
     // are is decided on the device.
     const bool many = ti == tc && tc != QT_F32 && scale > 0.f;
