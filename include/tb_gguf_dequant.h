@@ -511,6 +511,10 @@ int    tb_cuda_kv_pool_fork(void *pool, int seq);
  * such copies (0 or 1), or -1 with nothing changed (unknown sequence, n < 0,
  * too few free pages, or more than INT_MAX positions). */
 int    tb_cuda_kv_pool_extend(void *pool, int seq, int n, int *src, int *dst);
+/* The same for count sequences, in order and all or nothing: n[i] more
+ * positions for seqs[i].  src and dst hold count entries.  Returns the number
+ * of copies, or -1 with nothing changed. */
+int    tb_cuda_kv_pool_extend_all(void *pool, const int *seqs, const int *n, int count, int *src, int *dst);
 /* Drops the positions from len on (0 <= len <= its length).  1 = ok. */
 int    tb_cuda_kv_pool_truncate(void *pool, int seq, int len);
 /* Ends the sequence; its unshared pages are free again.  1 = ok. */

@@ -135,6 +135,7 @@ def lib() -> ctypes.CDLL:
         "tb_cuda_kv_pool_new": (c_int, [c_void_p]),
         "tb_cuda_kv_pool_fork": (c_int, [c_void_p, c_int]),
         "tb_cuda_kv_pool_extend": (c_int, [c_void_p, c_int, c_int, ctypes.POINTER(c_int), ctypes.POINTER(c_int)]),
+        "tb_cuda_kv_pool_extend_all": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p]),
         "tb_cuda_kv_pool_truncate": (c_int, [c_void_p, c_int, c_int]),
         "tb_cuda_kv_pool_free": (c_int, [c_void_p, c_int]),
         "tb_cuda_kv_pool_compact": (c_int, [c_void_p, c_void_p, c_void_p, c_int]),
@@ -167,6 +168,7 @@ def exported_symbols() -> list[str]:
         "tb_cuda_dec_destroy",
         "tb_cuda_rope_table_dev", "tb_cuda_kv_append_dev", "tb_cuda_kv_attend_ws", "tb_cuda_kv_attend_dev",
         "tb_cuda_kv_copy_dev", "tb_cuda_kv_pool_create", "tb_cuda_kv_pool_destroy", "tb_cuda_kv_pool_new",
-        "tb_cuda_kv_pool_fork", "tb_cuda_kv_pool_extend", "tb_cuda_kv_pool_truncate", "tb_cuda_kv_pool_free",
+        "tb_cuda_kv_pool_fork", "tb_cuda_kv_pool_extend", "tb_cuda_kv_pool_extend_all",
+        "tb_cuda_kv_pool_truncate", "tb_cuda_kv_pool_free",
         "tb_cuda_kv_pool_compact", "tb_cuda_kv_pool_len", "tb_cuda_kv_pool_pages", "tb_cuda_kv_pool_free_pages",
     ])

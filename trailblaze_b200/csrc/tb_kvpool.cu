@@ -153,6 +153,51 @@ int tb_cuda_kv_pool_extend(void *pool, int seq, int n, int *src, int *dst)
     return own ? 1 : 0;
 }
 
+int tb_cuda_kv_pool_extend_all(void *pool, const int *seqs, const int *n, int count, int *src, int *dst)
+{
+    if (!pool || count < 0 || (count > 0 && (!seqs || !n || !src || !dst))) return -1;
+    Pool &p = *pool_of(pool);
+    struct Step {
+        int len;        // before
+        size_t pages;
+        int from;       // the shared page that got a copy, -1: none
+    };
+    std::vector<Step> done;
+    try {
+        done.reserve(static_cast<size_t>(count));
+    } catch (const std::exception &e) {
+        fprintf(stderr, "[tb_cuda] kv_pool_extend_all: %s\n", e.what());
+        return -1;
+    }
+    int copies = 0;
+    for (int i = 0; i < count; ++i) {
+        const Seq *s = p.at(seqs[i]);
+        const Step before{s ? s->len : 0, s ? s->pages.size() : 0, -1};
+        int a = -1, b = -1;
+        const int r = tb_cuda_kv_pool_extend(pool, seqs[i], n[i], &a, &b);
+        if (r >= 0) {
+            done.push_back(before);
+            if (r == 1) done.back().from = src[copies] = a, dst[copies] = b, ++copies;
+            continue;
+        }
+        for (int k = i - 1; k >= 0; --k) {   // what the ones before it took goes back, last first
+            Seq &t = p.seqs[seqs[k]];
+            while (t.pages.size() > done[k].pages) {
+                p.drop(t.pages.back());
+                t.pages.pop_back();
+            }
+            if (done[k].from >= 0) {
+                p.drop(t.pages.back());
+                ++p.refs[done[k].from];   // still held by the sequences that it was shared with
+                t.pages.back() = done[k].from;
+            }
+            t.len = done[k].len;
+        }
+        return -1;
+    }
+    return copies;
+}
+
 int tb_cuda_kv_pool_truncate(void *pool, int seq, int len)
 {
     if (!pool) return 0;

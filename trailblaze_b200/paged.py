@@ -142,6 +142,15 @@ class PagePool:
                      f"extend({seq}, {n})")
         return (a.value, b.value) if r else None
 
+    def extend_all(self, new: dict[int, int]) -> tuple[np.ndarray, np.ndarray]:
+        """Room for new[seq] more positions of each sequence, or of none where one cannot have it; the (sources,
+        destinations) of the pages to copy first."""
+        seqs, n = np.asarray(list(new), np.int32), np.asarray(list(new.values()), np.int32)
+        src, dst = np.empty(len(new), np.int32), np.empty(len(new), np.int32)
+        m = self._id(self.L.tb_cuda_kv_pool_extend_all(self.p, seqs.ctypes.data, n.ctypes.data, len(new), src.ctypes.data,
+                                                       dst.ctypes.data), f"extend({new})")
+        return src[:m], dst[:m]
+
     def truncate(self, seq: int, length: int) -> None:
         if self.L.tb_cuda_kv_pool_truncate(self.p, seq, length) != 1:
             raise RuntimeError(f"truncate({seq}, {length}) failed")
@@ -210,10 +219,9 @@ class PagedKV:
         return self._pool
 
     def extend(self, new: dict[int, int]) -> None:
-        """Room for new[seq] more positions of each sequence; part-filled pages that are shared are copied."""
-        moves = [m for m in (self.pool.extend(s, n) for s, n in new.items()) if m]
-        if moves:
-            self.copy_pages(*zip(*moves))
+        """Room for new[seq] more positions of each sequence; part-filled pages that are shared are copied.  Where
+        one of them cannot have it, none gets any (and the call raises)."""
+        self.copy_pages(*self.pool.extend_all(new))
 
     def fork(self, seq: int) -> int:
         return self.pool.fork(seq)
