@@ -66,7 +66,7 @@ class Rope:
         if table.dim() != 3 or table.shape[2] != 2 or table.dtype != torch.float32 or not table.is_contiguous() \
                 or not table.is_cuda:
             raise ValueError("a contiguous float32 CUDA table [positions, pairs, 2] expected")
-        self.table, self.interleaved = table, bool(interleaved)
+        self.table, self.interleaved, self.device = table, bool(interleaved), table.device
         self._plain = self.struct(None, None, 0.0)
 
     def struct(self, q_norm, k_norm, eps) -> KvRope:
@@ -102,7 +102,7 @@ class Batch:
                 raise ValueError(f"int32 CUDA tensors [S + 1], [S], [S, width] expected, got {t.dtype} {tuple(t.shape)}")
         if n and (not start.is_contiguous() or not lens.is_contiguous() or (pages.shape[1] > 1 and pages.stride(1) != 1)):
             raise ValueError("start and lens contiguous, rows of pages contiguous")
-        self.start, self.lens, self.pages = start, lens, pages
+        self.start, self.lens, self.pages, self.device = start, lens, pages, start.device
         self.n_tokens = n_tokens
         self.struct = KvBatch(start.data_ptr(), lens.data_ptr(), pages.data_ptr(), n, n_tokens, max_new, max_len,
                               pages.stride(0) if n > 1 else pages.shape[1])
@@ -255,6 +255,8 @@ class PagedKV:
         """Norms and rotates q (returned, or in q_out) and k, and stores k and v at the batch's positions."""
         heads, dim, dev = q.shape[1] if q.dim() == 3 else 0, self.head_dim, self.device
         self._tokens(batch, q, k, v)
+        if rope is not None and rope.device != dev:
+            raise ValueError(f"rotary table on {rope.device}: the cache is on {dev}")
         rq, rk, rv = _rows(q, heads, dim, dev), _rows(k, self.n_kv_heads, dim, dev), _rows(v, self.n_kv_heads, dim, dev)
         if q_out is None:
             q_out = torch.empty_like(q)
@@ -312,6 +314,8 @@ class PagedKV:
 
     def _tokens(self, batch: Batch, *rows: torch.Tensor) -> None:
         n, dtype = batch.n_tokens, rows[0].dtype
+        if batch.device != self.device:
+            raise ValueError(f"batch on {batch.device}: the cache is on {self.device}")
         for t in rows:
             if t.dim() != 3 or t.shape[0] != n:
                 raise ValueError(f"rows of shape {tuple(t.shape)}: the batch has {n} rows")
