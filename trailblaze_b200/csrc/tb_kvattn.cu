@@ -24,7 +24,10 @@
 // tensor pipe idles either way.
 //
 // Precision: 16-bit activations over a cache of their type multiply as they are;
-// P goes in as a high and a low 16-bit part.  fp32 activations are split into
+// P goes in as a high and a low 16-bit part.  fp16 ends at 2^-24, so over an F16 cache the
+// numerators are kept just below the other end of its range, the largest at 2^15: what both
+// parts lose of one lies 2^-40 below the largest (at 1, 2^-25 below it: where one position
+// outweighs the rest by 2^25, the rest would vanish).  fp32 activations are split into
 // parts of the cache's type (3 bf16, or 2 fp16 of a row scaled by a power of two
 // so that its largest element is near 2^13); an fp32 cache is split into two
 // tf32 parts, of which the low-low product is dropped (2^-22).  Scores, softmax and
@@ -142,6 +145,9 @@ __global__ void __launch_bounds__(FewCfg<HD, TI, TC>::W * 32, FewCfg<HD, TI, TC>
     constexpr bool X32 = TC == QT_F32;
     constexpr bool FINE = TI == QT_F32;          // fp32 results
     constexpr int NC = FINE ? 5 : 2;             // accumulators of a score: 4 and the small products', or 2
+    // Numerators are 2^(score - m): m follows the running maximum, moved when a score passes
+    // it by 2^TOP, to 2^UP below the largest score then.
+    constexpr float TOP = TC == QT_F16 ? 15.f : 8.f, UP = TC == QT_F16 ? 15.f : 0.f;
     constexpr int KS = X32 ? HD / 8 : HD / 16;   // steps of the product over the head's dimensions
     constexpr int CB = HD * ES / 128;            // 128-byte columns of a row
     constexpr uint32_t kCol = kSlice * 128;
@@ -470,14 +476,14 @@ __global__ void __launch_bounds__(FewCfg<HD, TI, TC>::W * 32, FewCfg<HD, TI, TC>
                         x[e] = see ? x[e] : -INFINITY;
                     }
                 }
-                // ---- the running maximum: moved only when a score passes it by 2^8 ----
-                if (__any_sync(0xFFFFFFFFu, fmaxf(x[0], x[2]) > m[0] + 8.f || fmaxf(x[1], x[3]) > m[1] + 8.f)) {
+                // ---- m: see TOP and UP ----
+                if (__any_sync(0xFFFFFFFFu, fmaxf(x[0], x[2]) > m[0] + TOP || fmaxf(x[1], x[3]) > m[1] + TOP)) {
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
                         float mx = fmaxf(x[e], x[e + 2]);
 #pragma unroll
                         for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, o));
-                        mx = fmaxf(mx, m[e]);
+                        mx = fmaxf(mx - UP, m[e]);
                         const float corr = m[e] == -INFINITY ? 0.f : ex2(m[e] - mx);
                         m[e] = mx;
                         l[e] *= corr;

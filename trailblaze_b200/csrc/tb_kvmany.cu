@@ -26,11 +26,12 @@
 // execute in order; when S_g(j) is complete so is PV_g(j - 1), which is why the
 // softmax threads may rescale O_g between seeing S_g and handing over P_g.
 //
-// The running maximum moves only when a score passes it by 2^8 (exponents stay
-// far inside fp32 and fp16), so rescaling O is rare.  P is rounded to the cache's
-// type for the second product, whose unit takes nothing wider: 2^-9 (bf16) of
-// each term, unbiased, about what the output's own rounding is; sums are fp32 of
-// the unrounded P.
+// The running maximum moves only when a score passes it by 2^8, so rescaling O is
+// rare.  P is rounded to the cache's type for the second product, whose unit takes
+// nothing wider: 2^-9 (bf16) or 2^-12 (fp16) of each term, unbiased, about what the
+// output's own rounding is; sums are fp32 of the unrounded P.  fp16 ends at 2^-24: its
+// numerators lie 2^7 higher, up to 2^15, so that what it cannot hold lies 2^-32 below
+// the largest.
 //
 // Measured (32 query and 8 kv heads of 128, bf16): 8192 tokens from the start in 504
 // us, 1092 TFLOP/s of the pairs that are seen; 512 tokens at 4096 in 48 us.  A unit
@@ -142,6 +143,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     constexpr int CB = HD / 64;   // 128-byte columns
     constexpr int NS = Cfg::NS;
     constexpr bool BF = std::is_same<I, __nv_bfloat16>::value;
+    // m is moved when a score passes it by 2^TOP, to 2^UP below the largest score then
+    constexpr float TOP = BF ? 8.f : 15.f, UP = BF ? 0.f : 7.f;
     extern __shared__ __align__(1024) uint8_t smraw[];
     uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smraw) + 1023) & ~uintptr_t(1023));
     uint8_t *stage = sm + 2 * Cfg::QG + NS * Cfg::SLOT;
@@ -489,8 +492,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                 mx *= sc;
                 // (rows that there are not hold whatever shared memory held: they have no say in
                 // when the others rescale, or results would not repeat)
-                if (__any_sync(0xFFFFFFFFu, on && mx > m + 8.f)) {
-                    const float mn = fmaxf(m, mx);
+                if (__any_sync(0xFFFFFFFFu, on && mx > m + TOP)) {
+                    const float mn = fmaxf(m, mx - UP);
                     const float corr = m == -INFINITY ? 0.f : ex2(m - mn);
                     l *= corr;
                     m = mn;
