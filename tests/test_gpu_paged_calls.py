@@ -29,3 +29,45 @@ def test_tables_on_another_device_are_refused(paged, kq):  # noqa: F811
         c.cache.append(1, c.batch, c.q, c.nk, c.nv)
     with pytest.raises(ValueError, match="batch"):
         c.cache.attend(1, c.batch, c.q)
+
+
+CHILD = r"""
+import sys
+sys.path[:0] = [{repo!r}, {tests!r}]
+import torch
+from trailblaze_b200 import load, paged as P
+from test_gpu_paged import BF16, F32, Case
+kq = load()
+assert kq.tb_cuda_init() == 1
+"""
+
+
+def child(body, **env):
+    """A process of its own: the wait limit is read once, when the library starts."""
+    import subprocess
+    here = os.path.dirname(os.path.abspath(__file__))
+    code = CHILD.format(repo=os.path.dirname(here), tests=here) + body
+    r = subprocess.run([sys.executable, "-c", code], env=dict(os.environ, **env), capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-3000:]
+    return [ln.split()[1:] for ln in r.stdout.splitlines() if ln.startswith("RESULT")]
+
+
+def test_a_failed_wait_drains_what_is_in_flight():
+    """A one-poll limit makes waits of the three attention kernels run out while copies and products are under
+    way: each call ends with the error word 1 (or 0, where every poll found its work done), what was in flight has
+    landed, and the process and its device memory are as they should be."""
+    res = child(r"""
+for io, new, lens in ((BF16, [1] * 9, [3000] * 9), (F32, [1, 1], [5000, 33]), (BF16, [300, 40], [4000, 900]),
+                      (F32, [200, 40], [3000, 900])):
+    c = Case(P, new, lens, 8, 2, 128, io, io, 16, seed=31)
+    guard = torch.full((1 << 20,), 7, dtype=torch.int32, device="cuda")
+    k, v, q = c.k.clone(), c.v.clone(), c.q.clone()
+    for _ in range(5):
+        c.cache.attend(1, c.batch, c.q)
+    torch.cuda.synchronize()
+    same = all(torch.equal(a.view(torch.uint8), b.contiguous().view(torch.uint8)) for a, b in ((k, c.k), (v, c.v), (q, c.q)))
+    print("RESULT", kq.tb_cuda_last_error(), int(same), int((guard == 7).all()))
+""", TB_WAIT_LIMIT="1")
+    assert len(res) == 4
+    for err, same, guard in res:
+        assert err in ("0", "1") and same == "1" and guard == "1", res

@@ -759,9 +759,9 @@ __global__ void __launch_bounds__(FewCfg<HD, TI, TC>::W * 32, FewCfg<HD, TI, TC>
         __syncthreads();   // merge and sh are free again
     }
     if (tell >= 0) told();
-    // after a wait that ran out: the copies still in flight, as far as they come
+    // after a wait that ran out: the copies still in flight
     while (!ok && taken < issued) {
-        mbar_wait_bounded(bars + (taken % NST) * 8, (taken / NST) & 1u, a.err, a.wait_limit);
+        mbar_wait_bounded(bars + (taken % NST) * 8, (taken / NST) & 1u, nullptr, kKvDrain);
         ++taken;
     }
 }

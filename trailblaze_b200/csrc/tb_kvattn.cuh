@@ -10,6 +10,11 @@
 
 namespace tb {
 
+// Bound of the waits after a failed one, for what is still in flight (copies into
+// shared memory, MMAs): it is no part of the wait limit, which a user may set, since a
+// CTA that ended before its copies landed would leave them to the next one's memory.
+static constexpr uint32_t kKvDrain = 1u << 26;
+
 struct AttnArgs {
     KvView c;
     KvBatch b;

@@ -418,7 +418,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             // every MMA issued is complete before TMEM is given back
             if (elect_one()) umma_commit(smem_u32(&sh.done));
             __syncwarp();
-            mbar_wait_bounded(smem_u32(&sh.done), 0, err, lim);
+            mbar_wait_bounded(smem_u32(&sh.done), 0, err, kKvDrain);
         }
     } else {
         // ---- softmax: thread = row ----
@@ -686,11 +686,11 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     // ---- the end: nothing in flight, TMEM given back ----
     tc_fence_before();
     __syncthreads();
-    if (sh.fail) {   // a wait ran out: the copies still in flight, as far as they come
+    if (sh.fail) {   // a wait ran out: the copies still in flight
         if (warp == 9)
             for (uint32_t n = kv_issued > NS ? kv_issued - NS : 0; n < kv_issued; ++n)
-                mbar_wait_bounded(smem_u32(&sh.kvfull[n % NS]), (n / NS) & 1u, err, lim);
-        if (warp == 10 && q_issued > 0) mbar_wait_bounded(smem_u32(&sh.qfull), (q_issued - 1) & 1u, err, lim);
+                mbar_wait_bounded(smem_u32(&sh.kvfull[n % NS]), (n / NS) & 1u, nullptr, kKvDrain);
+        if (warp == 10 && q_issued > 0) mbar_wait_bounded(smem_u32(&sh.qfull), (q_issued - 1) & 1u, nullptr, kKvDrain);
     }
     __syncthreads();
     if (warp == 8) {

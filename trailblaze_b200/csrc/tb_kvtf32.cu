@@ -344,7 +344,7 @@ __global__ void __launch_bounds__(kTfThreads, 1)
             // every MMA issued is complete before TMEM is given back
             if (elect_one()) umma_commit(smem_u32(&sh.done));
             __syncwarp();
-            mbar_wait_bounded(smem_u32(&sh.done), 0, err, lim);
+            mbar_wait_bounded(smem_u32(&sh.done), 0, err, kKvDrain);
         }
     } else if (warp >= 8) {
         // ---- operands: K in two parts, V transposed and in two parts ----
@@ -744,8 +744,8 @@ __global__ void __launch_bounds__(kTfThreads, 1)
     // ---- the end: nothing in flight, TMEM given back ----
     tc_fence_before();
     __syncthreads();
-    if (sh.fail && issued > 0)   // a wait ran out: the copies still in flight, as far as they come
-        mbar_wait_bounded(smem_u32(warp == 15 ? &sh.vfull : &sh.kfull), (issued - 1) & 1u, err, lim);
+    if (sh.fail && issued > 0)   // a wait ran out: the copies still in flight
+        mbar_wait_bounded(smem_u32(warp == 15 ? &sh.vfull : &sh.kfull), (issued - 1) & 1u, nullptr, kKvDrain);
     __syncthreads();
     if (warp == 12) {
         tc_fence_after();
