@@ -71,3 +71,29 @@ for io, new, lens in ((BF16, [1] * 9, [3000] * 9), (F32, [1, 1], [5000, 33]), (B
     assert len(res) == 4
     for err, same, guard in res:
         assert err in ("0", "1") and same == "1" and guard == "1", res
+
+
+def test_counters_balance_after_a_wait_that_ran_out():
+    """Arrival counters that start far below zero make every join's wait run out.  The call reports it (error word
+    1) and takes from the counters what arrives there, no more and no less: zeroed, they serve the next call."""
+    res = child(r"""
+for io, cache, new, lens in ((BF16, BF16, [1] * 9, [3000] * 9), (F32, F32, [1, 1], [5000, 33]),
+                             (BF16, BF16, [300, 40, 1], [4000, 900, 700]), (F32, F32, [200, 40, 2], [3000, 900, 700]),
+                             (F32, BF16, [200], [3000])):
+    c = Case(P, new, lens, 8, 2, 128, io, cache, 16, seed=32)
+    want = c.cache.attend(1, c.batch, c.q)
+    torch.cuda.synchronize()
+    first = kq.tb_cuda_last_error()
+    (ws, *_), = c.cache._ws.values()
+    n = ws[:2048].view(torch.int32)
+    zero = bool((n == 0).all())
+    n.fill_(-1000)
+    c.cache.attend(1, c.batch, c.q)
+    torch.cuda.synchronize()
+    err, kept = kq.tb_cuda_last_error(), bool((n == -1000).all())
+    n.zero_()
+    again = c.cache.attend(1, c.batch, c.q)
+    torch.cuda.synchronize()
+    print("RESULT", first, int(zero), err, int(kept), kq.tb_cuda_last_error(), int(torch.equal(again, want)))
+""", TB_WAIT_LIMIT="200000")
+    assert res == [["0", "1", "1", "1", "0", "1"]] * 5, res

@@ -311,13 +311,8 @@ __global__ void __launch_bounds__(FewCfg<HD, TI, TC>::W * 32, FewCfg<HD, TI, TC>
         }
     };
     int tell = -1;   // the CTA that waits for this one's part
-    auto told = [&]() {   // each warp for its stores
-        __syncwarp();
-        if (lane == 0) {
-            __threadfence();
-            atomicAdd(a.arrived + tell, 1u);
-        }
-        __syncwarp();
+    auto told = [&]() {
+        kv_arrive(a, tell);
         tell = -1;
     };
     const uint32_t krow = (lane & 7) + ((lane >> 3) & 1) * 8, kchunk = lane >> 4;   // ldmatrix rows of K
@@ -696,18 +691,9 @@ __global__ void __launch_bounds__(FewCfg<HD, TI, TC>::W * 32, FewCfg<HD, TI, TC>
                 // so those CTAs were started before this one. ----
                 const unsigned others = share.of(first + cu.steps - 1) - cta;
                 const float *part = a.part + static_cast<size_t>(cta + 1) * P;
-                if (tid == 0) {
-                    uint32_t i = 0;
-                    unsigned n = 0;
-                    do {
-                        asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(n) : "l"(a.arrived + cta) : "memory");
-                    } while (n < W * others && ++i < a.wait_limit);
-                    if (n < W * others) {
-                        atomicExch(a.err, ERR_WAIT_TIMEOUT);
-                        sh.fail = 1;
-                    }
-                    a.arrived[cta] = 0;   // zero between calls
-                    __threadfence();
+                if (tid == 0 && !kv_await(a, cta, W * others, [] { return false; })) {
+                    atomicExch(a.err, ERR_WAIT_TIMEOUT);
+                    sh.fail = 1;
                 }
                 __syncthreads();
                 if (mr < rows) {
@@ -772,7 +758,7 @@ __global__ void __launch_bounds__(FewCfg<HD, TI, TC>::W * 32, FewCfg<HD, TI, TC>
 // Workspace: the arrival counters (the part that stays zero between calls), then
 // the partial results, one a CTA.
 static constexpr int kMaxCtas = 512;
-static constexpr size_t kCounterBytes = kMaxCtas * sizeof(unsigned);
+static constexpr size_t kCounterBytes = kMaxCtas * sizeof(int);
 size_t kv_attend_ws()
 {
     size_t n = sizeof(float) * kMaxCtas * few_part(128);
@@ -841,7 +827,7 @@ int kv_attend_launch(const KvView &c, const KvBatch &b, int hd, int ti, int tc, 
     const NvtxRange nvtx("tb.kv_attend");
     (void)max_len;
     AttnArgs a{c, b, q, o, nh, nh / c.n_kv_heads, window, sinks, scale * 1.4426950408889634f, err, wait_limit};
-    a.arrived = static_cast<unsigned *>(ws);
+    a.arrived = static_cast<int *>(ws);
     a.part = reinterpret_cast<float *>(static_cast<char *>(ws) + kCounterBytes);
     a.many_rows = 0x7FFFFFFF;
     int before = 0;   // launches

@@ -25,7 +25,7 @@ struct AttnArgs {
     uint32_t wait_limit;
     int ax_pos, ax_head, ax_page;   // the tensor maps' axes 1..3: which of them is which
     float *part;                    // [gridDim.x] partial results
-    unsigned *arrived;              // [gridDim.x] arrival counters, zero between calls
+    int *arrived;                   // [gridDim.x] arrival counters, zero between calls: see kv_await
     int many_rows;                  // k_kv_few: sequences of more rows are the other launch's
 };
 
@@ -183,6 +183,34 @@ __device__ __forceinline__ void tmem_wait_ld(uint32_t *r)
 __device__ __forceinline__ void after_wait(uint32_t *r) { asm volatile("" : TB_W32("+r", r)::"memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// ---- joining the parts of an item ----
+// Each part's warps add one to the counter of the CTA that has the item's beginning,
+// which waits for all of them and takes that number off again.  Every CTA does its share
+// of both, once, after a failed wait as well: a call leaves the counters at zero however
+// it ends, since a part that comes after its joiner has given up finds the number gone
+// already.
+__device__ __forceinline__ void kv_arrive(const AttnArgs &a, int cta)   // by a whole warp, for its stores
+{
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) {
+        __threadfence();
+        atomicAdd(a.arrived + cta, 1);
+    }
+    __syncwarp();
+}
+// One thread: true when want warps have arrived, false when the limit ran out or stop().
+template <class F>
+__device__ __forceinline__ bool kv_await(const AttnArgs &a, int cta, int want, F stop)
+{
+    int n = 0;
+    uint32_t i = 0;
+    do {
+        asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(n) : "l"(a.arrived + cta) : "memory");
+    } while (n < want && ++i < a.wait_limit && !stop());
+    atomicSub(a.arrived + cta, want);
+    return n >= want;
+}
+
 // The rows of sequences whose numbers contradict each other: the error word, and
 // zeros as far as the rows exist (one CTA, all its threads).
 template <int HD, class I>
@@ -282,7 +310,8 @@ __device__ __forceinline__ unsigned long long kv_head_units(const AttnArgs &a, i
 }
 
 struct KvScan {   // shared
-    unsigned long long warp[16], items[16];
+    unsigned long long warp[16], items[16], total;
+    unsigned parts;           // the CTAs with a share of the total
     int seq, head, rt, off;   // the CTA's first item and its first unit there
 };
 struct KvCtaShare {
@@ -332,6 +361,7 @@ __device__ __forceinline__ bool kv_items_share(const AttnArgs &a, int tpi, int f
     most = max(most, (total + MIN - 1) / MIN);
     const unsigned G = most < gridDim.x ? static_cast<unsigned>(most) : gridDim.x;
     if (blockIdx.x >= G) return false;
+    if (tid == 0) sh.total = total, sh.parts = G;
     my.cta = G - 1 - blockIdx.x;
     my.share = KvShare(total, G);
     my.u0 = my.share.start(my.cta), my.u1 = my.share.start(my.cta + 1);
@@ -388,6 +418,31 @@ __device__ __forceinline__ KvItem kv_item_first(const AttnArgs &a, int tpi, int 
     kv_item_enter(a, tpi, few_rows, it);
     kv_item_tiles<TILE>(a, tpi, it.q, it.rt, &it);
     return it;
+}
+
+// What a CTA that gave up owes the counters, by one thread: the arrivals of its warps that
+// have not told of their parts, and its own number, where it has not come to its join.
+struct KvOwed {
+    int joined, told[8];   // shared, zero at first
+};
+template <int TILE, int WARPS>
+__device__ __noinline__ void kv_leave(const AttnArgs &a, int tpi, int few_rows, const KvScan &sh, const KvOwed &owed)
+{
+    const KvShare share(sh.total, sh.parts);
+    const unsigned cta = sh.parts - 1 - blockIdx.x;
+    unsigned long long u = share.start(cta);
+    const unsigned long long u1 = share.start(cta + 1);
+    KvItem it = kv_item_first<TILE>(a, tpi, few_rows, sh);
+    int j0 = sh.off, told = 0;
+    for (int w = 0; w < WARPS; ++w) told += owed.told[w];
+    if (j0 > 0) atomicAdd(a.arrived + share.of(u - j0), WARPS - told);
+    while (u1 - u > static_cast<unsigned>(it.n - j0)) {
+        u += it.n - j0;
+        j0 = 0;
+        kv_item_next<TILE>(a, tpi, few_rows, it);
+    }
+    if (!owed.joined && j0 == 0 && u1 - u < static_cast<unsigned>(it.n))
+        atomicSub(a.arrived + cta, WARPS * static_cast<int>(share.of(u + it.n - 1) - cta));
 }
 
 // The layer's K and V as 4-D tensors: dimension, then position in the page, head

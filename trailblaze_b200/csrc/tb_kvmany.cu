@@ -80,6 +80,7 @@ struct ManyShared {
     KvScan scan;
     uint32_t tmem;
     int fail, bad;
+    KvOwed owed;
 };
 static_assert(sizeof(ManyShared) <= 1024, "ManyShared");
 
@@ -173,6 +174,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         fence_mbar_init();
         sh.fail = 0;
         sh.bad = 0;
+        sh.owed = KvOwed{};
     }
     if (warp == 9 && lane < 2) prefetch_map(lane ? &vmap : &kmap);
     if (warp == 10 && lane == 0) prefetch_map(&qmap);
@@ -431,12 +433,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         uint32_t cnt = 0, items = 0, joins = 0;
         int tell = -1;   // the CTA that waits for this one's part
         auto told = [&]() {   // each softmax warp for its rows
-            __syncwarp();
-            if (lane == 0) {
-                __threadfence();
-                atomicAdd(a.a.arrived + tell, 1u);
-            }
-            __syncwarp();
+            kv_arrive(a.a, tell);
+            sh.owed.told[warp] = 1;
             tell = -1;
         };
         bool ok = true;
@@ -575,17 +573,11 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                 if (others > 0) {
                     // 8 softmax warps of each of the others
                     if (tid == 0) {
-                        uint32_t i = 0;
-                        unsigned n = 0;
-                        do {
-                            asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(n) : "l"(a.a.arrived + my.cta) : "memory");
-                        } while (n < 8 * others && ++i < lim && !failed());
-                        if (n < 8 * others) {
+                        if (!kv_await(a.a, my.cta, 8 * others, failed)) {
                             if (!failed()) atomicExch(err, ERR_WAIT_TIMEOUT);
                             *reinterpret_cast<volatile int *>(&sh.fail) = 1;
                         }
-                        a.a.arrived[my.cta] = 0;   // zero between calls
-                        __threadfence();
+                        sh.owed.joined = 1;
                     }
                     if (!join()) break;
                     const unsigned mine_others = on ? others : 0;
@@ -686,7 +678,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     // ---- the end: nothing in flight, TMEM given back ----
     tc_fence_before();
     __syncthreads();
-    if (sh.fail) {   // a wait ran out: the copies still in flight
+    if (sh.fail) {   // a wait ran out: the counters, and the copies still in flight
+        if (tid == 0) kv_leave<kTileN, 8>(a.a, a.tpi, a.few_rows, sh.scan, sh.owed);
         if (warp == 9)
             for (uint32_t n = kv_issued > NS ? kv_issued - NS : 0; n < kv_issued; ++n)
                 mbar_wait_bounded(smem_u32(&sh.kvfull[n % NS]), (n / NS) & 1u, nullptr, kKvDrain);

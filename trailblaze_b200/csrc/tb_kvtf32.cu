@@ -52,6 +52,7 @@ struct TfShared {
     KvScan scan;
     uint32_t tmem;
     int fail, bad;
+    KvOwed owed;
     float corr[2][128];      // a tile's factor of the rows' sums so far
     float fin[2][2][128];    // an item's m and l
 };
@@ -190,6 +191,7 @@ __global__ void __launch_bounds__(kTfThreads, 1)
         fence_mbar_init();
         sh.fail = 0;
         sh.bad = 0;
+        sh.owed = KvOwed{};
     }
     if (warp >= 14 && lane == 0) prefetch_map(warp == 15 ? &vmap : &kmap);
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -606,12 +608,8 @@ __global__ void __launch_bounds__(kTfThreads, 1)
         uint32_t cnt = 0, items = 0, joins = 0;
         int tell = -1;   // the CTA that waits for this one's part
         auto told = [&]() {   // each warp for its rows
-            __syncwarp();
-            if (lane == 0) {
-                __threadfence();
-                atomicAdd(aa.arrived + tell, 1u);
-            }
-            __syncwarp();
+            kv_arrive(aa, tell);
+            sh.owed.told[warp - 4] = 1;
             tell = -1;
         };
         while (ok && u < my.u1) {
@@ -660,17 +658,11 @@ __global__ void __launch_bounds__(kTfThreads, 1)
                 if (j1 < it.n) {
                     const unsigned others = my.share.of(u + it.n - 1) - my.cta;
                     if (row == 0) {
-                        uint32_t i = 0;
-                        unsigned n = 0;
-                        do {
-                            asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(n) : "l"(aa.arrived + my.cta) : "memory");
-                        } while (n < 4 * others && ++i < lim && !failed());
-                        if (n < 4 * others) {
+                        if (!kv_await(aa, my.cta, 4 * others, failed)) {
                             if (!failed()) atomicExch(err, ERR_WAIT_TIMEOUT);
                             *reinterpret_cast<volatile int *>(&sh.fail) = 1;
                         }
-                        aa.arrived[my.cta] = 0;   // zero between calls
-                        __threadfence();
+                        sh.owed.joined = 1;
                     }
                     __syncwarp();
                     mbar_arrive(smem_u32(&sh.join));
@@ -744,7 +736,9 @@ __global__ void __launch_bounds__(kTfThreads, 1)
     // ---- the end: nothing in flight, TMEM given back ----
     tc_fence_before();
     __syncthreads();
-    if (sh.fail && issued > 0)   // a wait ran out: the copies still in flight
+    // a wait ran out: the counters, and the copies still in flight
+    if (sh.fail && tid == 0) kv_leave<kTfTile, 4>(aa, a.tpi, a.few_rows, sh.scan, sh.owed);
+    if (sh.fail && issued > 0)
         mbar_wait_bounded(smem_u32(warp == 15 ? &sh.vfull : &sh.kfull), (issued - 1) & 1u, nullptr, kKvDrain);
     __syncthreads();
     if (warp == 12) {
