@@ -482,10 +482,11 @@ int    tb_cuda_kv_append_dev(const tb_kv_cache *cache, int layer, const tb_kv_ba
  * softmax and sums are fp32; fp32 activations keep fp32 accuracy over any
  * cache type; 16-bit activations over a cache of the same type may round the
  * softmax numerators to that type before the second product.  d_ws: workspace
- * of tb_cuda_kv_attend_ws() bytes, 16-byte aligned, zeroed once before its
- * first call; every call leaves it ready for the next, one that ends with an
+ * of tb_cuda_kv_attend_ws() bytes, 16-byte aligned, its first
+ * TB_KV_WS_ZEROED bytes zeroed once before its first call; every call leaves it ready for the next, one that ends with an
  * error word too.  Calls that may overlap on the GPU need one each.
  * Stream-ordered.  1 = issued. */
+#define TB_KV_WS_ZEROED 2048
 size_t tb_cuda_kv_attend_ws(void);
 int    tb_cuda_kv_attend_dev(const tb_kv_cache *cache, int layer, const tb_kv_batch *batch, int io_type, int n_heads,
                              const tb_kv_rows *q, const tb_kv_rows *out, float scale, int window, int sinks,

@@ -97,3 +97,83 @@ for io, cache, new, lens in ((BF16, BF16, [1] * 9, [3000] * 9), (F32, F32, [1, 1
     print("RESULT", first, int(zero), err, int(kept), kq.tb_cuda_last_error(), int(torch.equal(again, want)))
 """, TB_WAIT_LIMIT="200000")
     assert res == [["0", "1", "1", "1", "0", "1"]] * 5, res
+
+
+def captured(c, stream, **kw):
+    """The append and attention of c's batch as a graph, and its output."""
+    graph = torch.cuda.CUDAGraph()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.graph(graph, stream=stream):
+        out = c.cache.attend(1, c.batch, c.cache.append(1, c.batch, c.q, c.nk, c.nv), **kw)
+    return graph, out
+
+
+@pytest.mark.parametrize("io,cache,new,lens", [(BF16, BF16, [1] * 5, [2000, 17, 900, 64, 333]),
+                                               (BF16, BF16, [200, 1], [1500, 700]), (F32, F32, [100, 3], [900, 2000])])
+def test_captured_calls_have_workspaces_of_their_own(paged, kq, io, cache, new, lens):  # noqa: F811
+    """Two graphs captured on one stream, the second replayed first, both replayed on streams of their own beside
+    eager calls on the capture stream: no call has another's counters or parts."""
+    cases = [Case(paged, new, lens, 8, 2, 128, io, cache, 16, seed=33 + i) for i in range(2)]
+    for c in cases:
+        c.want = c.cache.attend(1, c.batch, c.cache.append(1, c.batch, c.q, c.nk, c.nv)).clone()
+    torch.cuda.synchronize()
+    stream, side = torch.cuda.Stream(), [torch.cuda.Stream(), torch.cuda.Stream()]
+    one = cases[0]
+    made = [(one, *captured(one, stream)), (one, *captured(one, stream)), (cases[1], *captured(cases[1], stream))]
+    assert stream.cuda_stream not in one.cache._ws and stream.cuda_stream not in cases[1].cache._ws
+    for c, graph, out in reversed(made):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, c.want)
+        out.zero_()
+    with torch.cuda.stream(stream):
+        one.cache.attend(1, one.batch, one.q)   # the capture stream's own, from here on
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for (c, graph, out), s in zip(made, side):
+            with torch.cuda.stream(s):
+                graph.replay()
+        with torch.cuda.stream(stream):
+            eager = one.cache.attend(1, one.batch, one.q)
+    torch.cuda.synchronize()
+    assert torch.equal(eager, one.want) and all(torch.equal(out, c.want) for c, _, out in made[:2])
+    assert kq.tb_cuda_last_error() == 0
+
+
+def test_a_workspace_of_the_callers(paged, kq):  # noqa: F811
+    c = Case(paged, [1, 40], [700, 333], 8, 2, 128, BF16, BF16, 16, seed=36)
+    c.cache.append(1, c.batch, c.q, c.nk, c.nv)   # as the captured step does
+    want = c.cache.attend(1, c.batch, c.q)
+    ws = c.cache.workspace()
+    before = dict(c.cache._ws)
+    for _ in range(3):
+        assert torch.equal(c.cache.attend(1, c.batch, c.q, workspace=ws), want)
+    torch.cuda.synchronize()
+    graph, out = captured(c, torch.cuda.Stream(), workspace=ws)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+    assert c.cache._ws == before
+    for bad in (ws[:-16], ws[8:], ws.view(torch.int32), ws[::2], ws.cpu()):
+        with pytest.raises(ValueError):
+            c.cache.attend(1, c.batch, c.q, workspace=bad)
+
+
+def test_a_captured_step_follows_its_tables(paged, kq):  # noqa: F811
+    """The kernels find their work from the tables on the device: a replay after they changed is a call of the
+    changed batch."""
+    c = Case(paged, [1, 1, 1], [400, 90, 33], 8, 2, 128, BF16, BF16, 16, seed=37)
+    ws, out = c.cache.workspace(), torch.empty_like(c.q)
+    c.cache.attend(1, c.batch, c.q, workspace=ws)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        c.cache.attend(1, c.batch, c.q, out=out, workspace=ws)
+    for lens in ([400, 90, 33], [1, 64, 17], [399, 16, 32]):
+        c.batch.lens.copy_(torch.tensor(lens, dtype=torch.int32))
+        c.lens = lens
+        graph.replay()
+        torch.cuda.synchronize()
+        c.check(out)
+    assert kq.tb_cuda_last_error() == 0

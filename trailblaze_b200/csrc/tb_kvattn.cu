@@ -37,6 +37,7 @@
 // positions, 2.07 GB, in 306 us, 6.76 TB/s, what a copy reaches; one sequence of 4096
 // fp32 positions, 33.6 MB, in 19 us against 5 us of bytes: launch, scan, the first
 // page, Q and the joining of 16 parts stand one behind the other there.
+#include "../../include/tb_gguf_dequant.h"
 #include "tb_kvattn.cuh"
 
 namespace tb {
@@ -759,6 +760,7 @@ __global__ void __launch_bounds__(FewCfg<HD, TI, TC>::W * 32, FewCfg<HD, TI, TC>
 // the partial results, one a CTA.
 static constexpr int kMaxCtas = 512;
 static constexpr size_t kCounterBytes = kMaxCtas * sizeof(int);
+static_assert(kCounterBytes == TB_KV_WS_ZEROED, "the header's number");
 size_t kv_attend_ws()
 {
     size_t n = sizeof(float) * kMaxCtas * few_part(128);

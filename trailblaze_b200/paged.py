@@ -30,6 +30,8 @@ from ._lib import KvBatch, KvCache, KvRope, KvRows, RopeScale, lib
 _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else \
     lambda index: torch.cuda.current_stream(index).cuda_stream
 
+_WS_ZEROED = 2048   # TB_KV_WS_ZEROED
+
 _TYPES = {torch.float32: Q.F32, torch.float16: Q.F16, torch.bfloat16: Q.BF16}
 
 
@@ -274,8 +276,28 @@ class PagedKV:
             raise ValueError("tb_cuda_kv_append_dev refused the call")
         return q_out
 
+    def workspace(self) -> torch.Tensor:
+        """A workspace for attend(), zeroed.  Calls that may overlap on the GPU need one each.  Without one, calls on
+        a stream share that stream's, and a call that is captured into a graph gets its own, filled with zeros
+        in the graph: a graph that takes one from outside has a launch less for every call."""
+        return torch.zeros(self.L.tb_cuda_kv_attend_ws(), dtype=torch.uint8, device=self.device)
+
+    def _own_workspace(self, stream: int) -> tuple:
+        if torch.cuda.is_current_stream_capturing():
+            # from the graph's memory and not kept: what ran on the stream before, another graph captured on
+            # it and this graph's replays on any stream have nothing of it in common
+            ws = torch.empty(self.L.tb_cuda_kv_attend_ws(), dtype=torch.uint8, device=self.device)
+            ws[:_WS_ZEROED].zero_()
+            return ws, ws.data_ptr(), ws.numel()
+        ws = self._ws.get(stream)
+        if ws is None:
+            ws = self.workspace()
+            ws = self._ws[stream] = (ws, ws.data_ptr(), ws.numel())
+        return ws
+
     def attend(self, layer: int, batch: Batch, q: torch.Tensor, out: torch.Tensor | None = None,
-               scale: float | None = None, window: int = 0, sinks: int = 0) -> torch.Tensor:
+               scale: float | None = None, window: int = 0, sinks: int = 0,
+               workspace: torch.Tensor | None = None) -> torch.Tensor:
         """Attention of the batch's new tokens over their sequences' positions (tb_cuda_kv_attend_dev)."""
         heads, dim, dev = q.shape[1] if q.dim() == 3 else 0, self.head_dim, self.device
         self._tokens(batch, q)
@@ -286,10 +308,12 @@ class PagedKV:
             raise ValueError("out: the shape and type of q expected")
         ro = _rows(out, heads, dim, dev)
         stream = _raw_stream(dev.index)
-        ws = self._ws.get(stream)
-        if ws is None:
-            ws = torch.zeros(self.L.tb_cuda_kv_attend_ws(), dtype=torch.uint8, device=dev)
-            ws = self._ws[stream] = (ws, ws.data_ptr(), ws.numel())
+        if workspace is None:
+            ws = self._own_workspace(stream)
+        elif workspace.dtype != torch.uint8 or workspace.device != dev or not workspace.is_contiguous():
+            raise ValueError(f"workspace: a contiguous uint8 tensor on {dev} expected")
+        else:
+            ws = workspace, workspace.data_ptr(), workspace.numel()
         if self._on_device(self.L.tb_cuda_kv_attend_dev, self._ref, layer, batch._ref, _type(q), heads,
                            ctypes.byref(rq), ctypes.byref(ro), 1.0 / math.sqrt(dim) if scale is None else scale, window,
                            sinks, ws[1], ws[2], stream) != 1:
