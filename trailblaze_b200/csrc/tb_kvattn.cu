@@ -626,28 +626,33 @@ __global__ void __launch_bounds__(FewCfg<HD, TI, TC>::W * 32, FewCfg<HD, TI, TC>
             const int ja = step0 * W, jb = min(cu.sl.n, (step0 + nstep) * W);   // the part's slices
             for (int r = warp; r < rows; r += W) {
                 if (!sh.bad[r]) continue;
-                constexpr int D = HD / 32;
                 const int tok = (r0 + r) / a.group, hh = (r0 + r) - tok * a.group;
-                const I *qp = static_cast<const I *>(a.q.p) + (cu.q.row0 + tok) * a.q.row +
-                              (cu.h * a.group + hh) * a.q.head + lane * D;
-                float q[D], am[2], al[2], ac[2][D];
-#pragma unroll
-                for (int d = 0; d < D; ++d) q[d] = kv_f(qp[d]) * a.scale2;
+                const I *qp = static_cast<const I *>(a.q.p) + (cu.q.row0 + tok) * a.q.row + (cu.h * a.group + hh) * a.q.head;
                 // its slices before and after the gap between the first tokens and the window
                 const int b0 = min(ja, cu.sl.ns), b1 = min(jb, cu.sl.ns);
                 const int c0 = max(ja, cu.sl.ns) - cu.sl.ns + cu.sl.lo, c1 = max(jb, cu.sl.ns) - cu.sl.ns + cu.sl.lo;
-                kv_row_attend<HD, E>(a.b, a.c, cu.s, cu.h, p0 + tok, b0 * kSlice, b1 * kSlice, a.window, a.sinks, q,
-                                     am[0], al[0], ac[0], a.err);
-                kv_row_attend<HD, E>(a.b, a.c, cu.s, cu.h, p0 + tok, c0 * kSlice, min(c1 * kSlice, cu.q.len), a.window,
-                                     a.sinks, q, am[1], al[1], ac[1], a.err);
-                const float mm = fmaxf(am[0], am[1]);
-                const float f0 = am[0] == -INFINITY ? 0.f : ex2(am[0] - mm), f1 = am[1] == -INFINITY ? 0.f : ex2(am[1] - mm);
+                float m = -INFINITY, l = 0.f, o[8];
 #pragma unroll
-                for (int d = 0; d < D; ++d) merge[r * HD + lane * D + d] = ac[0][d] * f0 + ac[1][d] * f1;
-                if (lane == 0) {
-                    sh.m[0][r] = mm;
-                    sh.l[0][r] = (am[0] == -INFINITY ? al[0] : al[0] * f0) + (am[1] == -INFINITY ? al[1] : al[1] * f1);
+                for (int d = 0; d < 8; ++d) o[d] = 0.f;
+#pragma unroll 1
+                for (int part = 0; part < 2; ++part) {
+                    const I *const q1[1] = {qp};
+                    const int i1[1] = {p0 + tok};
+                    float xm[1], xl[1], x[1][8];
+                    kv_rows_attend<HD, I, E, 1, 4>(a, q1, cu.s, cu.h, i1, (part ? c0 : b0) * kSlice,
+                                                part ? min(c1 * kSlice, cu.q.len) : b1 * kSlice, xm, xl, x);
+                    const float mm = fmaxf(m, xm[0]);
+                    const float f0 = m == -INFINITY ? 0.f : ex2(m - mm), f1 = xm[0] == -INFINITY ? 0.f : ex2(xm[0] - mm);
+                    l = (m == -INFINITY ? l : l * f0) + (xm[0] == -INFINITY ? xl[0] : xl[0] * f1);
+#pragma unroll
+                    for (int d = 0; d < 8; ++d) o[d] = o[d] * f0 + x[0][d] * f1;
+                    m = mm;
                 }
+                if (lane < HD / 8) {
+#pragma unroll
+                    for (int d = 0; d < 8; ++d) merge[r * HD + lane * 8 + d] = o[d];
+                }
+                if (lane == 0) sh.m[0][r] = m, sh.l[0][r] = l;
             }
             __syncthreads();
             if (mr < rows && sh.bad[mr]) {

@@ -183,6 +183,166 @@ __device__ __forceinline__ void tmem_wait_ld(uint32_t *r)
 __device__ __forceinline__ void after_wait(uint32_t *r) { asm volatile("" : TB_W32("+r", r)::"memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// R rows of one kv head again, in fp32, over their visible positions in [j0, j1) only, by the
+// whole warp: for rows whose result is not finite, where a NaN or an infinity may have come
+// from a position that the row does not see.  q: the rows; i: their positions (-1: none).
+// m: the largest exponent of 2 (-inf: nothing seen), l: the sum of the numerators, acc: the
+// weighted sums of dimensions lane % (HD / 8) * 8 ....
+// An infinity in V at the start of a long prompt sends every row here, so: 32 positions at a
+// time, HD / 8 lanes a position (a load takes whole rows), U loads in flight, R rows to a
+// load.  Where a numerator is NaN so is all of its row; once all rows are, the rest need not
+// be looked at.
+template <int HD, class I, class E, int R, int U>
+__device__ __forceinline__ void kv_rows_attend(const AttnArgs &a, const I *const (&q)[R], int s, int h, const int (&i)[R], int j0,
+                                               int j1, float (&m)[R], float (&l)[R], float (&acc)[R][8])
+{
+    constexpr int LR = HD / 8, RW = 32 / LR;   // lanes a row, rows a load
+    const int lane = threadIdx.x & 31, d0 = lane % LR * 8, grp = lane / LR;
+    const E *kp = static_cast<const E *>(a.c.k) + d0, *vp = static_cast<const E *>(a.c.v) + d0;
+    float qq[R][8];
+    KvSpan sp[R];
+    int first = 0, lo = 0x7FFFFFFF, last = -1;   // of all rows
+    unsigned open = 0;                           // rows that are not NaN yet
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        sp[r] = kv_span(max(i[r], 0), a.window, a.sinks);
+        if (i[r] >= 0) first = max(first, sp[r].first), lo = min(lo, sp[r].lo), open |= 1u << r;
+        last = max(last, i[r]);
+        kv_load8(q[r] + d0, qq[r]);
+        m[r] = -INFINITY, l[r] = 0.f;
+#pragma unroll
+        for (int d = 0; d < 8; ++d) acc[r][d] = 0.f;
+    }
+    j1 = min(j1, last + 1);
+    for (int j = j0; j < j1 && open; j += 32) {
+        if (j >= first && j < lo) j = min(lo, j1);   // the stretch that is hidden from all
+        const int p = j + lane;
+        const long long at = p < j1 && (p < first || p >= lo) ? kv_at(a.b, a.c, s, p, h, a.err) : -1;
+        float x[R], w[R];
+        unsigned see[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const bool on = at >= 0 && p <= i[r] && (p < sp[r].first || p >= sp[r].lo);
+            x[r] = -INFINITY;
+            see[r] = __ballot_sync(0xFFFFFFFFu, on);
+        }
+#pragma unroll 1
+        for (int k0 = 0; k0 < 32; k0 += U * RW) {
+            float kk[U][8];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {   // (a position that is none: any row that there is)
+                const long long ka = __shfl_sync(0xFFFFFFFFu, at, k0 + u * RW + grp);
+                kv_load8(kp + (ka < 0 ? 0 : ka), kk[u]);
+            }
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                float sc[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    float2 t = make_float2(0.f, 0.f);
+#pragma unroll
+                    for (int d = 0; d < 8; d += 2)
+                        t = __ffma2_rn(make_float2(qq[r][d], qq[r][d + 1]), make_float2(kk[u][d], kk[u][d + 1]), t);
+                    sc[u] = t.x + t.y;
+                }
+                // the U sums over a row's lanes together: at each step a lane keeps half of them, so
+                // that lane u * (LR / U) of a row's has the u-th in the end
+                int o = LR / 2;
+#pragma unroll
+                for (int n = U / 2; n > 0; n >>= 1, o >>= 1)
+#pragma unroll
+                    for (int u = 0; u < n; ++u) {
+                        const bool up = lane & o;
+                        const float keep = up ? sc[u + n] : sc[u], send = up ? sc[u] : sc[u + n];
+                        sc[u] = keep + __shfl_xor_sync(0xFFFFFFFFu, send, o);
+                    }
+                for (; o > 0; o >>= 1) sc[0] += __shfl_xor_sync(0xFFFFFFFFu, sc[0], o);
+                const float mine = __shfl_sync(0xFFFFFFFFu, sc[0], lane % RW * LR + lane / RW % U * (LR / U));
+                if (lane / (U * RW) == k0 / (U * RW) && (see[r] >> lane & 1u)) x[r] = mine * a.scale2;
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            float top = x[r];   // fmaxf passes NaN over
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+            top = fmaxf(top, m[r]);
+            const float corr = m[r] == -INFINITY ? 0.f : exp2f(m[r] - top);
+            w[r] = x[r] == -INFINITY ? 0.f : exp2f(x[r] - top);
+            m[r] = top;
+            l[r] = l[r] * corr + w[r];
+#pragma unroll
+            for (int d = 0; d < 8; ++d) acc[r][d] *= corr;
+            if (__any_sync(0xFFFFFFFFu, isnan(w[r]))) open &= ~(1u << r);
+        }
+#pragma unroll 1
+        for (int k0 = 0; k0 < 32; k0 += U * RW) {
+            float v[U][8];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const long long va = __shfl_sync(0xFFFFFFFFu, at, k0 + u * RW + grp);
+                kv_load8(vp + (va < 0 ? 0 : va), v[u]);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    const int k = k0 + u * RW + grp;
+                    const float wk = __shfl_sync(0xFFFFFFFFu, w[r], k);
+                    if (see[r] >> k & 1u) {
+#pragma unroll
+                        for (int d = 0; d < 8; d += 2) {
+                            const float2 t = __ffma2_rn(make_float2(wk, wk), make_float2(v[u][d], v[u][d + 1]),
+                                                        make_float2(acc[r][d], acc[r][d + 1]));
+                            acc[r][d] = t.x, acc[r][d + 1] = t.y;
+                        }
+                    }
+                }
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) l[r] += __shfl_xor_sync(0xFFFFFFFFu, l[r], o);
+#pragma unroll
+        for (int d = 0; d < 8; ++d) {
+#pragma unroll
+            for (int o = LR; o < 32; o <<= 1) acc[r][d] += __shfl_xor_sync(0xFFFFFFFFu, acc[r][d], o);
+            if (i[r] >= 0 && !(open >> r & 1u)) acc[r][d] = NAN;
+        }
+    }
+}
+// Whole rows and their output, those of the lanes of todo (row, head and position: the lane's).
+template <int HD, class I, class E>
+__device__ __forceinline__ void kv_rows_again(const AttnArgs &a, unsigned todo, int row, int head, int pos, int s, int h)
+{
+    constexpr int R = 3, U = 4;   // (4 rows are done in 0.8 of the time, and cost the kernel's usual loop 1.5 % by its registers)
+    while (todo) {
+        const I *qp[R];
+        long long to[R];
+        int i[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int src = todo ? __ffs(todo) - 1 : 0;
+            const long long t = __shfl_sync(0xFFFFFFFFu, row, src), n = __shfl_sync(0xFFFFFFFFu, head, src);
+            i[r] = __shfl_sync(0xFFFFFFFFu, pos, src);
+            if (!todo) i[r] = -1;
+            qp[r] = static_cast<const I *>(a.q.p) + (todo ? t * a.q.row + n * a.q.head : 0);
+            to[r] = t * a.o.row + n * a.o.head;
+            todo &= todo - 1;   // (0 stays 0)
+        }
+        float m[R], l[R], x[R][8];
+        kv_rows_attend<HD, I, E, R, U>(a, qp, s, h, i, 0, 0x7FFFFFFF, m, l, x);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+#pragma unroll
+            for (int d = 0; d < 8; ++d) x[r][d] = l[r] == 0.f ? 0.f : x[r][d] / l[r];
+            if (i[r] >= 0 && (threadIdx.x & 31) < HD / 8)
+                kv_store8(static_cast<I *>(const_cast<void *>(a.o.p)) + to[r] + (threadIdx.x & 31) * 8, x[r]);
+        }
+    }
+}
+
 // ---- joining the parts of an item ----
 // Each part's warps add one to the counter of the CTA that has the item's beginning,
 // which waits for all of them and takes that number off again.  Every CTA does its share
@@ -443,6 +603,54 @@ __device__ __noinline__ void kv_leave(const AttnArgs &a, int tpi, int few_rows, 
     }
     if (!owed.joined && j0 == 0 && u1 - u < static_cast<unsigned>(it.n))
         atomicSub(a.arrived + cta, WARPS * static_cast<int>(share.of(u + it.n - 1) - cta));
+}
+
+// The chunk kernels' rows that have to be done again, a warp's: they wait until its last item
+// is out.  In the loop over the items the call cost a long prompt 3 % without being made, and
+// while a warp was at it the CTA's others would sit in bounded waits.  3000 bf16 tokens of 8
+// heads whose first V is NaN: 5.0 ms, against 0.06 without and 66 a row and a position at a
+// time.
+struct KvAgain {   // shared, n zero at first
+    static constexpr int CAP = 4;
+    int n;   // past CAP: all rows of the CTA's items
+    struct {
+        unsigned rows;
+        int row0, t0, p0, s, h;   // the sequence's first row, the row group's first token, the position of token 0
+    } rec[CAP];
+    __device__ __forceinline__ void add(unsigned rows, int row0, int t0, int p0, int s, int h)   // one thread
+    {
+        if (n < CAP) rec[n] = {rows, row0, t0, p0, s, h};
+        ++n;
+    }
+};
+// lists: of the warps from warp0 on, four to a row group of tpt tokens.
+template <int HD, class I, class E, int TILE>
+__device__ __noinline__ void kv_again(const AttnArgs &a, const KvAgain *lists, int warp0, int tpt, int tpi, int few_rows, const KvScan &sh)
+{
+    const int w = (threadIdx.x >> 5) - warp0, tok0 = (w >> 2) * tpt;
+    const int r = (w & 3) * 32 + (threadIdx.x & 31), tok_in = r / a.group, hh = r - tok_in * a.group;
+    const KvAgain &todo = lists[w];
+    if (todo.n <= KvAgain::CAP) {
+        for (int k = 0; k < todo.n; ++k) {
+            const auto &x = todo.rec[k];
+            kv_rows_again<HD, I, E>(a, x.rows, x.row0 + x.t0 + tok_in, x.h * a.group + hh, x.p0 + x.t0 + tok_in, x.s, x.h);
+        }
+        return;
+    }
+    const KvShare share(sh.total, sh.parts);
+    const unsigned cta = sh.parts - 1 - blockIdx.x;
+    const unsigned long long u1 = share.start(cta + 1);
+    KvItem it = kv_item_first<TILE>(a, tpi, few_rows, sh);
+    int j0 = sh.off;
+    for (unsigned long long u = share.start(cta);;) {
+        const int tok = it.t0 + tok0 + tok_in;
+        const unsigned rows = __ballot_sync(0xFFFFFFFFu, j0 == 0 && tok_in < tpt && tok < it.t1);
+        kv_rows_again<HD, I, E>(a, rows, it.q.row0 + tok, it.h * a.group + hh, it.q.len - it.q.n + tok, it.s, it.h);
+        u += it.n - j0;
+        if (u >= u1) break;
+        j0 = 0;
+        kv_item_next<TILE>(a, tpi, few_rows, it);
+    }
 }
 
 // The layer's K and V as 4-D tensors: dimension, then position in the page, head

@@ -61,7 +61,7 @@ struct ManyCfg {
     static constexpr int QG = 128 * HD * 2;              // one row group's Q
     static constexpr int NS = HD == 128 ? 4 : 8;         // ring slots
     static constexpr int STAGE = 4096;                   // a softmax warp's staging for its output rows
-    static constexpr int SMEM = 1024 + 2 * QG + NS * SLOT + 8 * STAGE + 1024;
+    static constexpr int SMEM = 1024 + 2 * QG + NS * SLOT + 8 * STAGE + 2048;
     static constexpr int PART = 256 * HD + 512;          // floats of a partial result: O, m, l
 };
 
@@ -79,10 +79,12 @@ struct ManyShared {
     uint64_t sfull[2], pready[2][2], ofull[2], qfull, qempty, done, join, kvfull[8], kvempty[4], vready[8];
     KvScan scan;
     uint32_t tmem;
-    int fail, bad;
+    int fail, bad[8];       // bad: i + 1 at place i % 8 for an item i of the CTA with a page outside the pool (K and V
+                            // run at most 5 items ahead of the epilogue)
     KvOwed owed;
+    KvAgain again[8];
 };
-static_assert(sizeof(ManyShared) <= 1024, "ManyShared");
+static_assert(sizeof(ManyShared) <= 2048, "ManyShared");
 
 // D[tmem] (+)= A[tmem] * B[smem desc], one thread
 __device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
@@ -114,25 +116,6 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *map
                  "[%5];" ::"r"(dst),
                  "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
                  : "memory");
-}
-
-// One row again, over its visible positions only, by the whole warp: res = the sum
-// of the numerators and the weighted sums of dimensions lane * HD / 32 ....
-template <int HD, class I>
-__device__ __noinline__ void many_row_again(const ManyArgs &a, const ManyPart it, int tok, int hh, float *res)
-{
-    constexpr int D = HD / 32;
-    const int lane = threadIdx.x & 31;
-    const I *qp = static_cast<const I *>(a.a.q.p) + (it.row0 + tok) * a.a.q.row + (it.h * a.a.group + hh) * a.a.q.head +
-                  lane * D;
-    float q[D], m, l, acc[D];
-#pragma unroll
-    for (int d = 0; d < D; ++d) q[d] = kv_f(qp[d]) * a.a.scale2;
-    kv_row_attend<HD, I>(a.a.b, a.a.c, it.s, it.h, it.len - it.n + tok, 0, it.len, a.a.window, a.a.sinks, q, m, l,
-                         acc, a.a.err);
-    res[0] = l;
-#pragma unroll
-    for (int d = 0; d < D; ++d) res[1 + d] = acc[d];
 }
 
 template <int HD, class I>
@@ -173,8 +156,9 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         }
         fence_mbar_init();
         sh.fail = 0;
-        sh.bad = 0;
+        for (int i = 0; i < 8; ++i) sh.bad[i] = 0;
         sh.owed = KvOwed{};
+        for (int i = 0; i < 8; ++i) sh.again[i].n = 0;
     }
     if (warp == 9 && lane < 2) prefetch_map(lane ? &vmap : &kmap);
     if (warp == 10 && lane == 0) prefetch_map(&qmap);
@@ -237,7 +221,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         if (warp == 9) {
             // ---- K and V ----
             bool ok = true;
-            while (ok && u < my.u1) {
+            for (int item = 0; ok && u < my.u1; ++item) {
                 const int j1 = part_end();
                 for (int j = j0; ok && j < j1; ++j) {
                     const int p0 = kv_item_pos<kTileN>(it, j), boxes = kTileN / a.box;
@@ -250,7 +234,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                         pos = p - static_cast<int>(pi) * a.a.c.page_size;
                         if (page < 0 || page >= a.a.c.n_pages) {
                             atomicExch(err, ERR_RUNTIME);
-                            *reinterpret_cast<volatile int *>(&sh.bad) = 1;
+                            *reinterpret_cast<volatile int *>(&sh.bad[item & 7]) = item + 1;
                             page = a.a.c.n_pages;
                         }
                     }
@@ -538,7 +522,9 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                 if (tell >= 0) told();
             }
             if (!ok || !wait(&sh.ofull[g], items)) break;
+            const int at_bad = items & 7;
             ++items;
+            const bool bad = *reinterpret_cast<volatile int *>(&sh.bad[at_bad]) == static_cast<int>(items);
             tc_fence_after();
             const int row = g * 128 + lr;
             if (j0 > 0) {
@@ -558,7 +544,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                 part += 256 * HD - row * 3;
                 if (on) {   // rows that there are not stay out of the traffic
                     __stcg(part, m);
-                    __stcg(part + 256, *reinterpret_cast<volatile int *>(&sh.bad) ? NAN : l);
+                    __stcg(part + 256, bad ? -1.f : l);   // a page outside the pool: a sum that no part has
                 }
                 // the stores are under way; that they have arrived is told later
                 tell = static_cast<int>(it.peer);
@@ -569,7 +555,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                 const unsigned others = it.peer;
                 const float *part = a.a.part + static_cast<size_t>(my.cta + 1) * Cfg::PART;
                 float M = m, L = l;
-                bool odd = *reinterpret_cast<volatile int *>(&sh.bad);
+                bool odd = bad;
                 if (others > 0) {
                     // 8 softmax warps of each of the others
                     if (tid == 0) {
@@ -589,6 +575,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                     for (unsigned c = 0; c < mine_others; ++c) {
                         const float *pp = part + c * Cfg::PART + 256 * HD + row;
                         const float pm = __ldcg(pp), pl = __ldcg(pp + 256);
+                        odd = odd | (pl < 0.f);
                         L += pm == -INFINITY ? pl : ex2(pm - M) * pl;
                     }
                     // O in TMEM becomes the item's sum
@@ -626,7 +613,6 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                 I *out = static_cast<I *>(const_cast<void *>(a.a.o.p));
                 const long long off = on ? (it.row0 + tok) * a.a.o.row + (it.h * a.a.group + hh) * a.a.o.head : -1;
                 I *mine = reinterpret_cast<I *>(stage + warp * Cfg::STAGE);   // [32 rows][64], 16-byte pieces swizzled
-                odd = odd | !isfinite(L) | (M == INFINITY);
                 const float inv = L == 0.f ? 0.f : 1.0f / L;
                 // Rolled, since this code comes by once an item: unrolled, it would come from
                 // beyond the instruction cache every time.
@@ -639,7 +625,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                     float2 nil = make_float2(0.f, 0.f);   // stays zero where everything is finite
 #pragma unroll
                     for (int i = 0; i < 32; i += 2) nil = __ffma2_rn(make_float2(x[i], x[i + 1]), make_float2(0.f, 0.f), nil);
-                    odd = odd | !(nil.x + nil.y == 0.f);
+                    // (a sum of numerators that is NaN: a score that the row sees is, and so is the row)
+                    odd = odd | (!(nil.x + nil.y == 0.f) && !isnan(L));
 #pragma unroll
                     for (int i = 0; i < 32; i += 8) {
                         float y[8];
@@ -660,20 +647,14 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                     }
                 }
                 // rows that are not finite: V of a position that a row does not see may have been
-                // (0 * NaN), or a page lies outside the pool.  Once more, over their own positions only.
-                for (unsigned todo = __ballot_sync(0xFFFFFFFFu, odd && on); todo; todo &= todo - 1) {
-                    const int src = __ffs(todo) - 1;
-                    const int rtok = __shfl_sync(0xFFFFFFFFu, tok, src), rhh = __shfl_sync(0xFFFFFFFFu, hh, src);
-                    const long long ro = __shfl_sync(0xFFFFFFFFu, off, src);
-                    float res[1 + HD / 32];
-                    many_row_again<HD, I>(a, it, rtok, rhh, res);
-                    for (int d = 0; d < HD / 32; ++d)
-                        kv_store1(out + ro + lane * (HD / 32) + d, res[0] == 0.f ? 0.f : res[1 + d] / res[0]);
-                    __syncwarp();
-                }
+                // (0 * NaN), or a page lies outside the pool.  Once more at the end, over their own positions only.
+                const unsigned rows = __ballot_sync(0xFFFFFFFFu, odd && on);
+                if (rows && lane == 0) sh.again[warp].add(rows, it.row0, it.t0 + g * a.tpt, p0, it.s, it.h);
             }
         }
         if (tell >= 0) told();
+        __syncwarp();
+        if (sh.again[warp].n > 0) kv_again<HD, I, I, kTileN>(a.a, sh.again, 0, a.tpt, a.tpi, a.few_rows, sh.scan);
     }
     // ---- the end: nothing in flight, TMEM given back ----
     tc_fence_before();

@@ -51,8 +51,10 @@ struct TfShared {
     uint64_t kfull, kfree, vfull, vfree, kready, vready, qready, sfull, pready[2], ofull, oempty, done, join;
     KvScan scan;
     uint32_t tmem;
-    int fail, bad;
+    int fail, bad[8];        // bad: i + 1 at place i % 8 for an item i of the CTA with a page outside the pool (K and V
+                             // run at most 3 items ahead of the epilogue)
     KvOwed owed;
+    KvAgain again[4];
     float corr[2][128];      // a tile's factor of the rows' sums so far
     float fin[2][2][128];    // an item's m and l
 };
@@ -132,22 +134,6 @@ __device__ __forceinline__ void tf_add(uint32_t *a, const uint32_t *b)   // 32 s
     }
 }
 
-// One row again, over its visible positions only, by the whole warp: res = the sum
-// of the numerators and the weighted sums of dimensions lane * HD / 32 ....
-template <int HD, class I, class E>
-__device__ __noinline__ void tf_row_again(const AttnArgs &a, long long row, int head, int s, int h, int pos, int len, float *res)
-{
-    constexpr int D = HD / 32;
-    const I *qp = static_cast<const I *>(a.q.p) + row * a.q.row + head * a.q.head + (threadIdx.x & 31) * D;
-    float q[D], m, l, acc[D];
-#pragma unroll
-    for (int d = 0; d < D; ++d) q[d] = kv_f(qp[d]) * a.scale2;
-    kv_row_attend<HD, E>(a.b, a.c, s, h, pos, 0, len, a.window, a.sinks, q, m, l, acc, a.err);
-    res[0] = l;
-#pragma unroll
-    for (int d = 0; d < D; ++d) res[1 + d] = acc[d];
-}
-
 template <int HD, int TI, int TC>
 __global__ void __launch_bounds__(kTfThreads, 1)
     k_kv_tf32(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
@@ -190,8 +176,9 @@ __global__ void __launch_bounds__(kTfThreads, 1)
         mbar_init(smem_u32(&sh.join), 128);
         fence_mbar_init();
         sh.fail = 0;
-        sh.bad = 0;
+        for (int i = 0; i < 8; ++i) sh.bad[i] = 0;
         sh.owed = KvOwed{};
+        for (int i = 0; i < 4; ++i) sh.again[i].n = 0;
     }
     if (warp >= 14 && lane == 0) prefetch_map(warp == 15 ? &vmap : &kmap);
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -241,7 +228,7 @@ __global__ void __launch_bounds__(kTfThreads, 1)
             // ---- K (warp 14) and V tiles (15) as they are ----
             const bool kv = warp == 15;
             const uint32_t bar = smem_u32(kv ? &sh.vfull : &sh.kfull), raw = kv ? vraw : kraw;
-            while (ok && u < my.u1) {
+            for (int item = 0; ok && u < my.u1; ++item) {
                 const int j1 = part_end();
                 for (int j = j0; ok && j < j1; ++j) {
                     const int p0 = kv_item_pos<kTfTile>(it, j), boxes = kTfTile / a.box;
@@ -254,7 +241,7 @@ __global__ void __launch_bounds__(kTfThreads, 1)
                         pos = p - static_cast<int>(pi) * aa.c.page_size;
                         if (page < 0 || page >= aa.c.n_pages) {
                             atomicExch(err, ERR_RUNTIME);
-                            *reinterpret_cast<volatile int *>(&sh.bad) = 1;
+                            *reinterpret_cast<volatile int *>(&sh.bad[item & 7]) = item + 1;
                             page = aa.c.n_pages;
                         }
                     }
@@ -640,6 +627,7 @@ __global__ void __launch_bounds__(kTfThreads, 1)
                 if (tell >= 0) told();
             }
             if (!ok) break;
+            const bool bad = *reinterpret_cast<volatile int *>(&sh.bad[items & 7]) == static_cast<int>(items) + 1;
             if (j0 > 0) {
                 // ---- not the item's beginning: the part goes to the CTA that has it
                 // (a page outside the pool: as NaN, so that the rows are done again there) ----
@@ -648,13 +636,13 @@ __global__ void __launch_bounds__(kTfThreads, 1)
 #pragma unroll
                     for (int c = 0; c < HD; c += 4) __stcg(part + c / 4 * 128, make_float4(O[c], O[c + 1], O[c + 2], O[c + 3]));
                     float2 *ml = reinterpret_cast<float2 *>(aa.part + static_cast<size_t>(my.cta) * Cfg::PART + 128 * HD) + row;
-                    __stcg(ml, make_float2(m, *reinterpret_cast<volatile int *>(&sh.bad) ? NAN : l));
+                    __stcg(ml, make_float2(m, bad ? NAN : l));
                 }
                 tell = static_cast<int>(my.share.of(u - j0));
             } else {
                 // ---- the beginning: the other parts, of the CTAs after this one, in order (waited
                 // for, as every wait, within a limit: those CTAs were started before this one) ----
-                bool odd = *reinterpret_cast<volatile int *>(&sh.bad);
+                bool odd = bad;
                 if (j1 < it.n) {
                     const unsigned others = my.share.of(u + it.n - 1) - my.cta;
                     if (row == 0) {
@@ -715,23 +703,17 @@ __global__ void __launch_bounds__(kTfThreads, 1)
                     }
                 }
                 // rows that are not finite: V of a position that a row does not see may have been
-                // (0 * NaN), or a page lies outside the pool.  Once more, over their own positions only.
+                // (0 * NaN), or a page lies outside the pool.  Once more at the end, over their own positions only.
                 __syncwarp();
-                for (unsigned todo = __ballot_sync(0xFFFFFFFFu, odd && on); todo; todo &= todo - 1) {
-                    const int src = __ffs(todo) - 1;
-                    const int rtok = __shfl_sync(0xFFFFFFFFu, tok, src), rhead = __shfl_sync(0xFFFFFFFFu, ghead, src);
-                    const long long rrow = static_cast<long long>(it.q.row0) + rtok;
-                    float res[1 + HD / 32];
-                    tf_row_again<HD, I, E>(aa, rrow, rhead, it.s, it.h, it.q.len - it.q.n + rtok, it.q.len, res);
-                    I *op = out + rrow * aa.o.row + rhead * aa.o.head + lane * (HD / 32);
-                    for (int d = 0; d < HD / 32; ++d) kv_store1(op + d, res[0] == 0.f ? 0.f : res[1 + d] / res[0]);
-                    __syncwarp();
-                }
+                const unsigned rows = __ballot_sync(0xFFFFFFFFu, odd && on);
+                if (rows && lane == 0) sh.again[warp - 4].add(rows, it.q.row0, it.t0, it.q.len - it.q.n, it.s, it.h);
             }
             ++items;
             next_item(j1);
         }
         if (tell >= 0) told();
+        __syncwarp();
+        if (sh.again[warp - 4].n > 0) kv_again<HD, I, E, kTfTile>(aa, sh.again, 4, a.tpi, a.tpi, a.few_rows, sh.scan);
     }
     // ---- the end: nothing in flight, TMEM given back ----
     tc_fence_before();

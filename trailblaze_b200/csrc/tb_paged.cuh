@@ -1,6 +1,6 @@
 // tb_paged.cuh — what the paged cache's kernels share (include/tb_gguf_dequant.h
-// part 4): the device view of one layer's pages and of a step's ragged batch,
-// element conversion, and attention of one row by one warp.
+// part 4): the device view of one layer's pages and of a step's ragged batch, and
+// element conversion.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -167,46 +167,6 @@ __host__ __device__ __forceinline__ KvSpan kv_span(int i, int window, int sinks)
         s.first = sinks < s.lo ? sinks : s.lo;
     }
     return s;
-}
-
-// Attention of one row over its visible positions in [j0, j1), by one warp in
-// fp32: lane l holds dimensions l * HD / 32 ...; q premultiplied by the scale
-// and log2(e), so that scores are exponents of 2.  m: the running maximum (-inf:
-// nothing seen), l the sum of 2^(score - m), acc the weighted sum of V.
-template <int HD, class E>
-__device__ void kv_row_attend(const KvBatch &b, const KvView &c, int s, int h, int i, int j0, int j1, int window,
-                              int sinks, const float (&q)[HD / 32], float &m, float &l, float (&acc)[HD / 32],
-                              int *err)
-{
-    constexpr int D = HD / 32;
-    const int lane = threadIdx.x & 31;
-    const KvSpan sp = kv_span(i, window, sinks);
-    m = -INFINITY;
-    l = 0.f;
-#pragma unroll
-    for (int d = 0; d < D; ++d) acc[d] = 0.f;
-    if (j1 > i + 1) j1 = i + 1;
-    for (int j = j0; j < j1; ++j) {
-        if (j >= sp.first && j < sp.lo) {
-            j = sp.lo - 1;   // the hidden stretch between the first tokens and the window
-            continue;
-        }
-        const long long at = kv_at(b, c, s, j, h, err);
-        if (at < 0) continue;
-        const E *k = static_cast<const E *>(c.k) + at + lane * D, *v = static_cast<const E *>(c.v) + at + lane * D;
-        float sc = 0.f;
-#pragma unroll
-        for (int d = 0; d < D; ++d) sc = fmaf(q[d], kv_f(k[d]), sc);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sc += __shfl_xor_sync(0xFFFFFFFFu, sc, o);
-        const float mn = fmaxf(m, sc);   // a NaN score keeps m here and poisons p below
-        const float corr = m == -INFINITY ? 0.f : exp2f(m - mn);
-        const float p = sc == -INFINITY ? 0.f : exp2f(sc - mn);
-        l = l * corr + p;
-#pragma unroll
-        for (int d = 0; d < D; ++d) acc[d] = fmaf(p, kv_f(v[d]), acc[d] * corr);
-        m = mn;
-    }
 }
 
 }  // namespace tb
