@@ -478,7 +478,8 @@ int    tb_cuda_kv_append_dev(const tb_kv_cache *cache, int layer, const tb_kv_ba
  * window > 0 only those with i - j < window or j < sinks;
  *   out[t][h] = sum_j softmax_j(scale * q[t][h] . k[j]) v[j]
  * with kv head h / (n_heads / n_kv_heads).  A row that sees nothing is zero.
- * Hidden positions have no influence, whatever bits they hold.  Scores,
+ * Hidden positions have no influence, whatever bits they hold, and the table's
+ * entries for pages that no row of the call sees are not looked at.  Scores,
  * softmax and sums are fp32; fp32 activations keep fp32 accuracy over any
  * cache type; 16-bit activations over a cache of the same type may round the
  * softmax numerators to that type before the second product.  d_ws: workspace

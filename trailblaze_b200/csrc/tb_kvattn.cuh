@@ -422,6 +422,12 @@ __device__ __forceinline__ int kv_item_pos(const KvItem &it, int j)
 {
     return (j < it.ns ? j : j - it.ns + it.lo) * TILE;
 }
+// True when a row of the item sees any of the positions [p, p + n).  The page of others is not
+// looked at: it may have been given away since the window left it.
+__device__ __forceinline__ bool kv_item_sees(const AttnArgs &a, const KvItem &it, int p, int n)
+{
+    return p < it.q.len && (p < a.sinks || p + n > kv_span(it.q.len - it.q.n + it.t0, a.window, a.sinks).lo);
+}
 // True for a sequence of this launch: one of more rows than few_rows.
 __device__ __forceinline__ bool kv_item_seq(const AttnArgs &a, int few_rows, int s, KvSeq &q)
 {

@@ -225,10 +225,10 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                 const int j1 = part_end();
                 for (int j = j0; ok && j < j1; ++j) {
                     const int p0 = kv_item_pos<kTileN>(it, j), boxes = kTileN / a.box;
-                    // lane l: box l of the tile, its page (past the end: a page that reads as zeros)
+                    // lane l: box l of the tile, its page (past the end, or seen by no row: one that reads as zeros)
                     int page = a.a.c.n_pages, pos = 0;
                     const int p = p0 + lane * a.box;
-                    if (lane < boxes && p < it.q.len) {
+                    if (lane < boxes && kv_item_sees(a.a, it, p, a.box)) {
                         const uint32_t pi = fdiv(static_cast<uint32_t>(p), a.a.c.page_div);
                         page = __ldg(a.a.b.pages + static_cast<long long>(it.s) * a.a.b.pages_stride + pi);
                         pos = p - static_cast<int>(pi) * a.a.c.page_size;

@@ -232,10 +232,10 @@ __global__ void __launch_bounds__(kTfThreads, 1)
                 const int j1 = part_end();
                 for (int j = j0; ok && j < j1; ++j) {
                     const int p0 = kv_item_pos<kTfTile>(it, j), boxes = kTfTile / a.box;
-                    // lane l: box l of the tile, its page (past the end: a page that reads as zeros)
+                    // lane l: box l of the tile, its page (past the end, or seen by no row: one that reads as zeros)
                     int page = aa.c.n_pages, pos = 0;
                     const int p = p0 + lane * a.box;
-                    if (lane < boxes && p < it.q.len) {
+                    if (lane < boxes && kv_item_sees(aa, it, p, a.box)) {
                         const uint32_t pi = fdiv(static_cast<uint32_t>(p), aa.c.page_div);
                         page = __ldg(aa.b.pages + static_cast<long long>(it.s) * aa.b.pages_stride + pi);
                         pos = p - static_cast<int>(pi) * aa.c.page_size;
