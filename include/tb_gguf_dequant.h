@@ -411,14 +411,16 @@ typedef struct {
  * are device memory, read by the kernels.  n_tokens: rows in the step's
  * buffers (rows outside every sequence are left alone); max_new and max_len:
  * the most new tokens and positions of any sequence; they only choose between
- * kernels, and the results are right for any value.
+ * kernels, and the results are right for any value.  pages_width: the entries
+ * that a row of the table has (0: pages_stride); none past them is read, and
+ * rows may overlap.
  * A sequence whose range leaves [0, n_tokens], whose new tokens outnumber its
  * positions or whose positions outnumber its table's (or 2^31 - 256) sets the error word (2)
  * and is skipped, its rows of the output zero; so does a page outside the
  * pool, whose positions then count as hidden and are not stored to. */
 typedef struct {
     const int *d_start, *d_len, *d_pages;
-    int        n_seqs, n_tokens, max_new, max_len, pages_stride;
+    int        n_seqs, n_tokens, max_new, max_len, pages_stride, pages_width;
 } tb_kv_batch;
 
 /* Rows of heads: element (token t, head h, d) is p[t * row + h * head + d]

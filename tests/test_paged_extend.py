@@ -108,3 +108,19 @@ def test_extend_all_of_the_c_entry():
     assert call([f, s, g], [1, 1, 1]) == 2                  # the last holder of the shared page keeps it
     assert out[0, :2].tolist() == [1, 1] and out[1, :2].tolist() == [2, 3]
     L.tb_cuda_kv_pool_destroy(p)
+
+
+def test_the_width_of_a_table_is_checked():
+    import ctypes
+    from trailblaze_b200._lib import KvBatch, KvCache, KvRows
+    L = lib()
+    c = KvCache(0x10000, 0x20000, 30, 2, 8, 16, 4, 128, 65536, 8192, 2048, 128)
+    r = KvRows(0x40000, 4096, 128)
+
+    def attend(*tail):
+        b = KvBatch(0x1000, 0x2000, *tail)
+        return L.tb_cuda_kv_attend_dev(ctypes.byref(c), 0, ctypes.byref(b), 30, 16, ctypes.byref(r), ctypes.byref(r), 0.1, 0, 0,
+                                       0x50000, 1 << 30, None)
+    assert attend(0x3000, 2, 0, 1, 16, 4) == 1 and attend(0x3000, 2, 0, 1, 16, 4, 3) == 1
+    assert attend(0x3000, 2, 0, 1, 16, 0, 3) == 1 and attend(None, 2, 0, 1, 16, 0, 0) == 1
+    assert attend(0x3000, 2, 0, 1, 16, 4, -1) == 0 and attend(None, 2, 0, 1, 16, 0, 3) == 0

@@ -42,7 +42,7 @@ class KvCache(ctypes.Structure):
 class KvBatch(ctypes.Structure):
     """tb_kv_batch (include/tb_gguf_dequant.h, part 4)."""
     _fields_ = [(n, ctypes.c_void_p) for n in ("d_start", "d_len", "d_pages")] + \
-               [(n, ctypes.c_int) for n in ("n_seqs", "n_tokens", "max_new", "max_len", "pages_stride")]
+               [(n, ctypes.c_int) for n in ("n_seqs", "n_tokens", "max_new", "max_len", "pages_stride", "pages_width")]
 
 
 class KvRows(ctypes.Structure):

@@ -194,10 +194,12 @@ bool kv_cache_ok(const tb_kv_cache *c, int layer)
     return kv_disjoint(c->head_dim, 4, d);
 }
 
+int kv_table_width(const tb_kv_batch *b) { return b->pages_width > 0 ? b->pages_width : b->pages_stride; }
+
 bool kv_batch_ok(const tb_kv_batch *b)
 {
     return b && b->n_seqs >= 0 && b->n_tokens >= 0 && b->max_new >= 0 && b->max_len >= 0 && b->pages_stride >= 0 &&
-           (b->n_seqs == 0 || (b->d_start && b->d_len && (b->d_pages || b->pages_stride == 0)));
+           b->pages_width >= 0 && (b->n_seqs == 0 || (b->d_start && b->d_len && (b->d_pages || kv_table_width(b) == 0)));
 }
 
 bool kv_rows_ok(const tb_kv_rows *r, int type, int n_tokens, int heads, int hd, bool written)
@@ -222,7 +224,7 @@ tb::KvView kv_view(const tb_kv_cache *c, int layer)
 
 tb::KvBatch kv_batch(const tb_kv_batch *b)
 {
-    return tb::KvBatch{b->d_start, b->d_len, b->d_pages, b->n_seqs, b->n_tokens, b->pages_stride};
+    return tb::KvBatch{b->d_start, b->d_len, b->d_pages, b->n_seqs, b->n_tokens, b->pages_stride, kv_table_width(b)};
 }
 
 tb::KvRows kv_rows(const tb_kv_rows *r) { return tb::KvRows{r->p, r->row, r->head}; }

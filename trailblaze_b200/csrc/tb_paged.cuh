@@ -21,7 +21,7 @@ struct KvView {
 
 struct KvBatch {
     const int *start, *len, *pages;
-    int n_seqs, n_tokens, pages_stride;
+    int n_seqs, n_tokens, pages_stride, pages_width;
 };
 
 struct KvRows {
@@ -137,7 +137,7 @@ __device__ __forceinline__ bool kv_seq(const KvBatch &b, const KvView &c, int s,
     q.len = b.len[s];
     // (lengths near 2^31 would overflow where they are rounded up to tiles)
     const bool ok = a >= 0 && e >= a && e <= b.n_tokens && q.len >= 0 && q.len <= 0x7FFFFF00 && q.n <= q.len &&
-                    q.len <= static_cast<long long>(b.pages_stride) * c.page_size;
+                    q.len <= static_cast<long long>(b.pages_width) * c.page_size;
     if (!ok && err) atomicExch(err, ERR_RUNTIME);
     return ok;
 }

@@ -106,8 +106,11 @@ class Batch:
             raise ValueError("start and lens contiguous, rows of pages contiguous")
         self.start, self.lens, self.pages, self.device = start, lens, pages, start.device
         self.n_tokens = n_tokens
-        self.struct = KvBatch(start.data_ptr(), lens.data_ptr(), pages.data_ptr(), n, n_tokens, max_new, max_len,
-                              pages.stride(0) if n > 1 else pages.shape[1])
+        width = pages.shape[1]
+        stride = pages.stride(0) if n > 1 and width else width   # a dimension of one element has no stride of its own
+        if stride >= 2 ** 31:
+            raise ValueError(f"rows of pages {stride} entries apart")
+        self.struct = KvBatch(start.data_ptr(), lens.data_ptr(), pages.data_ptr(), n, n_tokens, max_new, max_len, stride, width)
         self._ref = ctypes.byref(self.struct)
 
 
