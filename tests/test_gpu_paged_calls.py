@@ -177,3 +177,15 @@ def test_a_captured_step_follows_its_tables(paged, kq):  # noqa: F811
         torch.cuda.synchronize()
         c.check(out)
     assert kq.tb_cuda_last_error() == 0
+
+
+def test_a_rotary_table_of_no_positions(paged, kq):  # noqa: F811
+    """Every position is past it: the error word, and nothing is stored."""
+    c = Case(paged, [1, 3], [1, 20], 4, 2, 64, F32, F32, 16, seed=38)
+    k0 = c.k.clone()
+    out = c.cache.append(1, c.batch, c.q, c.nk, c.nv, rope=paged.Rope.make(0, 64))
+    torch.cuda.synchronize()
+    assert kq.tb_cuda_last_error() == 2
+    assert not bool(out.any()) and torch.equal(c.k.nan_to_num(nan=5.0), k0.nan_to_num(nan=5.0))
+    with pytest.raises(ValueError):   # pairs there must be
+        c.cache.append(1, c.batch, c.q, c.nk, c.nv, rope=paged.Rope(torch.empty(4, 0, 2, device="cuda")))

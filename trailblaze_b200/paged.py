@@ -69,10 +69,12 @@ class Rope:
                 or not table.is_cuda:
             raise ValueError("a contiguous float32 CUDA table [positions, pairs, 2] expected")
         self.table, self.interleaved, self.device = table, bool(interleaved), table.device
+        # a table of no positions has no memory, and no table means no rotation: one row that no position is in
+        self._memory = table if table.numel() else torch.empty(1, max(1, table.shape[1]), 2, device=table.device)
         self._plain = self.struct(None, None, 0.0)
 
     def struct(self, q_norm, k_norm, eps) -> KvRope:
-        return KvRope(self.table.data_ptr(), q_norm, k_norm, self.table.shape[0], 2 * self.table.shape[1],
+        return KvRope(self._memory.data_ptr(), q_norm, k_norm, self.table.shape[0], 2 * self.table.shape[1],
                       self.interleaved, eps)
 
     @classmethod
