@@ -189,3 +189,17 @@ def test_a_rotary_table_of_no_positions(paged, kq):  # noqa: F811
     assert not bool(out.any()) and torch.equal(c.k.nan_to_num(nan=5.0), k0.nan_to_num(nan=5.0))
     with pytest.raises(ValueError):   # pairs there must be
         c.cache.append(1, c.batch, c.q, c.nk, c.nv, rope=paged.Rope(torch.empty(4, 0, 2, device="cuda")))
+
+
+def test_rows_that_want_a_gradient_are_refused(paged, kq):  # noqa: F811
+    """There is no backward pass, and outputs without a graph would lose the gradient without a word."""
+    c = Case(paged, [2], [20], 4, 2, 64, F32, F32, 16, seed=39)
+    q, w = c.q.clone().requires_grad_(), torch.ones(64, device="cuda", requires_grad=True)
+    for call in (lambda: c.cache.attend(1, c.batch, q), lambda: c.cache.append(1, c.batch, q, c.nk, c.nv),
+                 lambda: c.cache.append(1, c.batch, c.q, c.nk, c.nv.clone().requires_grad_()),
+                 lambda: c.cache.append(1, c.batch, c.q, c.nk, c.nv, k_norm=w)):
+        with pytest.raises(ValueError, match="backward"):
+            call()
+        with torch.no_grad():
+            call()
+    assert torch.equal(c.cache.attend(1, c.batch, q.detach()), c.cache.attend(1, c.batch, c.q))

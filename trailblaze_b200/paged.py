@@ -52,9 +52,15 @@ def _rows(t: torch.Tensor, heads: int, dim: int, device) -> KvRows:
     return KvRows(t.data_ptr(), stride[0] if shape[0] > 1 else 0, stride[1] if heads > 1 else 0)
 
 
+def _no_grad(t: torch.Tensor) -> None:
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError("the paged cache has no backward pass: detached rows and weights, or torch.no_grad(), expected")
+
+
 def _vector(t: torch.Tensor | None, n: int, what: str, device) -> int | None:
     if t is None:
         return None
+    _no_grad(t)
     if t.dtype != torch.float32 or t.shape != (n,) or not t.is_contiguous() or t.device != device:
         raise ValueError(f"{what}: a contiguous float32 vector of {n} on {device} expected")
     return t.data_ptr()
@@ -350,3 +356,5 @@ class PagedKV:
                 raise ValueError(f"rows of shape {tuple(t.shape)}: the batch has {n} rows")
             if t.dtype != dtype:
                 raise ValueError("q, k and v of one type expected")
+            if t.requires_grad:
+                _no_grad(t)
