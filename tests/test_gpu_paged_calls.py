@@ -203,3 +203,24 @@ def test_rows_that_want_a_gradient_are_refused(paged, kq):  # noqa: F811
         with torch.no_grad():
             call()
     assert torch.equal(c.cache.attend(1, c.batch, q.detach()), c.cache.attend(1, c.batch, c.q))
+
+
+def test_numbers_that_do_not_fit_are_refused(paged, kq):  # noqa: F811
+    """ctypes drops the upper bits of a number that is too large for a C int."""
+    c = Case(paged, [2], [20], 4, 2, 64, F32, F32, 16, seed=41)
+    far = 2 ** 32
+    for kw in (dict(window=far + 3), dict(window=-far + 3), dict(window=4, sinks=far + 1), dict(window=4, sinks=-1)):
+        with pytest.raises(ValueError):
+            c.cache.attend(1, c.batch, c.q, **kw)
+    for layer in (far + 1, far, -1, 2):
+        with pytest.raises(ValueError):
+            c.cache.attend(layer, c.batch, c.q)
+        with pytest.raises(ValueError):
+            c.cache.append(layer, c.batch, c.q, c.nk, c.nv)
+    for tail in ((far + 2, 2, 20), (2, far + 2, 20), (2, 2, far + 20)):
+        with pytest.raises(ValueError):
+            paged.Batch(c.batch.start, c.batch.lens, c.batch.pages, *tail)
+    for args in ((far + 8, 64), (8, far + 64)):
+        with pytest.raises(ValueError):
+            paged.Rope.make(*args)
+    assert torch.equal(c.cache.attend(1, c.batch, c.q, window=2 ** 31 - 1), c.cache.attend(1, c.batch, c.q))

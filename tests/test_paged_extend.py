@@ -124,3 +124,20 @@ def test_the_width_of_a_table_is_checked():
     assert attend(0x3000, 2, 0, 1, 16, 4) == 1 and attend(0x3000, 2, 0, 1, 16, 4, 3) == 1
     assert attend(0x3000, 2, 0, 1, 16, 0, 3) == 1 and attend(None, 2, 0, 1, 16, 0, 0) == 1
     assert attend(0x3000, 2, 0, 1, 16, 4, -1) == 0 and attend(None, 2, 0, 1, 16, 0, 3) == 0
+
+
+def test_numbers_that_do_not_fit_are_refused():
+    """ctypes and numpy drop the upper bits of a number that is too large for a C int."""
+    c = Host(4, 16)
+    s = c.pool.new()
+    c.extend({s: 20})
+    far = 2 ** 32
+    for call in (lambda: c.pool.extend(s, far + 1), lambda: c.pool.extend(s + far, 1), lambda: c.extend({s: far + 1}),
+                 lambda: c.extend({s + far: 1}), lambda: c.extend({s: np.int64(far + 1)}), lambda: c.pool.truncate(s, far + 5),
+                 lambda: c.pool.free(s + far), lambda: c.pool.fork(s + far), lambda: c.pool.length(s + far),
+                 lambda: c.pool.pages(s + far), lambda: PagePool(far + 4, 16), lambda: PagePool(4, far + 16),
+                 lambda: PagedKV.copy_pages(c, [far], [1]), lambda: PagedKV.copy_pages(c, np.asarray([0]), np.asarray([far + 1])),
+                 lambda: PagedKV.copy_pages(c, [0.5], [1])):
+        with pytest.raises(ValueError):
+            call()
+    assert c.pool.length(s) == 20 and c.pool.free_pages == 2

@@ -18,6 +18,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import operator
 
 import numpy as np
 import torch
@@ -29,6 +30,9 @@ from ._lib import KvBatch, KvCache, KvRope, KvRows, RopeScale, lib
 # call that a decode step makes for every layer)
 _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else \
     lambda index: torch.cuda.current_stream(index).cuda_stream
+# likewise without the checks that torch is initialised, which a cache's tensors answer
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", torch.cuda.is_current_stream_capturing)
 
 _WS_ZEROED = 2048   # TB_KV_WS_ZEROED
 
@@ -50,6 +54,24 @@ def _rows(t: torch.Tensor, heads: int, dim: int, device) -> KvRows:
         raise ValueError(f"rows on {t.device}: the cache is on {device}")
     # a dimension of one element has no stride of its own
     return KvRows(t.data_ptr(), stride[0] if shape[0] > 1 else 0, stride[1] if heads > 1 else 0)
+
+
+def _int(n, what: str) -> int:
+    """A C int: ctypes and numpy would drop the upper bits of a larger one."""
+    n = operator.index(n)
+    if not -2 ** 31 <= n < 2 ** 31:
+        raise ValueError(f"{what}: {n} does not fit 32 bits")
+    return n
+
+
+def _ints(a, what: str) -> np.ndarray:
+    a = np.asarray(a)
+    if a.dtype != np.int32:
+        b = a.astype(np.int32)
+        if a.size and (a.dtype.kind not in "iu" or a.tobytes() != b.astype(a.dtype).tobytes()):
+            raise ValueError(f"{what}: whole numbers of 32 bits expected")
+        a = b
+    return np.ascontiguousarray(a)
 
 
 def _no_grad(t: torch.Tensor) -> None:
@@ -89,10 +111,10 @@ class Rope:
              attn_factor: float = 0.0, device="cuda") -> "Rope":
         """scaling: None, "linear", "ntk" or "yarn" (tb_rope_scale in the header has the formulas)."""
         mode = {None: 0, "linear": 1, "ntk": 2, "yarn": 3}.get(scaling, -1)
-        if n_pos < 0 or rot_dim <= 0 or rot_dim % 2:
+        if _int(n_pos, "n_pos") < 0 or _int(rot_dim, "rot_dim") <= 0 or rot_dim % 2:
             raise ValueError(f"a table of {n_pos} positions and {rot_dim} rotary dimensions")
         t = torch.empty(n_pos, rot_dim // 2, 2, dtype=torch.float32, device=device)
-        s = RopeScale(base, factor, beta_fast, beta_slow, attn_factor, mode, orig_len)
+        s = RopeScale(base, factor, beta_fast, beta_slow, attn_factor, mode, _int(orig_len, "orig_len"))
         with torch.cuda.device(t.device):
             if t.numel() and lib().tb_cuda_rope_table_dev(t.data_ptr(), n_pos, rot_dim, ctypes.byref(s),
                                                           torch.cuda.current_stream().cuda_stream) != 1:
@@ -118,7 +140,8 @@ class Batch:
         stride = pages.stride(0) if n > 1 and width else width   # a dimension of one element has no stride of its own
         if stride >= 2 ** 31:
             raise ValueError(f"rows of pages {stride} entries apart")
-        self.struct = KvBatch(start.data_ptr(), lens.data_ptr(), pages.data_ptr(), n, n_tokens, max_new, max_len, stride, width)
+        self.struct = KvBatch(start.data_ptr(), lens.data_ptr(), pages.data_ptr(), n, _int(n_tokens, "n_tokens"),
+                              _int(max_new, "max_new"), _int(max_len, "max_len"), stride, width)
         self._ref = ctypes.byref(self.struct)
 
 
@@ -128,7 +151,7 @@ class PagePool:
     def __init__(self, n_pages: int, page_size: int):
         self.L = lib()
         self.n_pages, self.page_size = n_pages, page_size
-        self.p = self.L.tb_cuda_kv_pool_create(n_pages, page_size)
+        self.p = self.L.tb_cuda_kv_pool_create(_int(n_pages, "n_pages"), _int(page_size, "page_size"))
         if not self.p:
             raise ValueError(f"a pool of {n_pages} pages of {page_size} positions")
 
@@ -146,30 +169,30 @@ class PagePool:
         return self._id(self.L.tb_cuda_kv_pool_new(self.p), "new")
 
     def fork(self, seq: int) -> int:
-        return self._id(self.L.tb_cuda_kv_pool_fork(self.p, seq), f"fork({seq})")
+        return self._id(self.L.tb_cuda_kv_pool_fork(self.p, _int(seq, "seq")), f"fork({seq})")
 
     def extend(self, seq: int, n: int) -> tuple[int, int] | None:
         """Room for n more positions; the (source, destination) of a page to copy first, if any."""
         a, b = ctypes.c_int(-1), ctypes.c_int(-1)
-        r = self._id(self.L.tb_cuda_kv_pool_extend(self.p, seq, n, ctypes.byref(a), ctypes.byref(b)),
+        r = self._id(self.L.tb_cuda_kv_pool_extend(self.p, _int(seq, "seq"), _int(n, "n"), ctypes.byref(a), ctypes.byref(b)),
                      f"extend({seq}, {n})")
         return (a.value, b.value) if r else None
 
     def extend_all(self, new: dict[int, int]) -> tuple[np.ndarray, np.ndarray]:
         """Room for new[seq] more positions of each sequence, or of none where one cannot have it; the (sources,
         destinations) of the pages to copy first."""
-        seqs, n = np.asarray(list(new), np.int32), np.asarray(list(new.values()), np.int32)
+        seqs, n = _ints(list(new), "sequences"), _ints(list(new.values()), "positions")
         src, dst = np.empty(len(new), np.int32), np.empty(len(new), np.int32)
         m = self._id(self.L.tb_cuda_kv_pool_extend_all(self.p, seqs.ctypes.data, n.ctypes.data, len(new), src.ctypes.data,
                                                        dst.ctypes.data), f"extend({new})")
         return src[:m], dst[:m]
 
     def truncate(self, seq: int, length: int) -> None:
-        if self.L.tb_cuda_kv_pool_truncate(self.p, seq, length) != 1:
+        if self.L.tb_cuda_kv_pool_truncate(self.p, _int(seq, "seq"), _int(length, "length")) != 1:
             raise RuntimeError(f"truncate({seq}, {length}) failed")
 
     def free(self, seq: int) -> None:
-        if self.L.tb_cuda_kv_pool_free(self.p, seq) != 1:
+        if self.L.tb_cuda_kv_pool_free(self.p, _int(seq, "seq")) != 1:
             raise RuntimeError(f"free({seq}) failed")
 
     def compact(self) -> tuple[np.ndarray, np.ndarray]:
@@ -179,10 +202,10 @@ class PagePool:
         return src[:n], dst[:n]
 
     def length(self, seq: int) -> int:
-        return self._id(self.L.tb_cuda_kv_pool_len(self.p, seq), f"length({seq})")
+        return self._id(self.L.tb_cuda_kv_pool_len(self.p, _int(seq, "seq")), f"length({seq})")
 
     def pages(self, seq: int) -> np.ndarray:
-        n = self._id(self.L.tb_cuda_kv_pool_pages(self.p, seq, None, 0), f"pages({seq})")
+        n = self._id(self.L.tb_cuda_kv_pool_pages(self.p, _int(seq, "seq"), None, 0), f"pages({seq})")
         a = np.empty(n, np.int32)
         self.L.tb_cuda_kv_pool_pages(self.p, seq, a.ctypes.data, n)
         return a
@@ -253,7 +276,7 @@ class PagedKV:
         lens = [self.pool.length(s) for s in seqs]
         tables = [self.pool.pages(s) for s in seqs]
         width = max([len(t) for t in tables], default=0) or 1
-        start = np.concatenate([[0], np.cumsum(new)]).astype(np.int32)
+        start = _ints(np.concatenate([[0], np.cumsum(np.asarray(new, np.int64))]), "new")
         at = np.full((len(seqs), width), -1, np.int32)
         for i, t in enumerate(tables):
             at[i, :len(t)] = t
@@ -268,6 +291,8 @@ class PagedKV:
         """Norms and rotates q (returned, or in q_out) and k, and stores k and v at the batch's positions."""
         heads, dim, dev = q.shape[1] if q.dim() == 3 else 0, self.head_dim, self.device
         self._tokens(batch, q, k, v)
+        if not 0 <= layer < self.n_layers:
+            raise ValueError(f"layer {layer} of {self.n_layers}")
         if rope is not None and rope.device != dev:
             raise ValueError(f"rotary table on {rope.device}: the cache is on {dev}")
         rq, rk, rv = _rows(q, heads, dim, dev), _rows(k, self.n_kv_heads, dim, dev), _rows(v, self.n_kv_heads, dim, dev)
@@ -294,7 +319,7 @@ class PagedKV:
         return torch.zeros(self.L.tb_cuda_kv_attend_ws(), dtype=torch.uint8, device=self.device)
 
     def _own_workspace(self, stream: int) -> tuple:
-        if torch.cuda.is_current_stream_capturing():
+        if _capturing():
             # from the graph's memory and not kept: what ran on the stream before, another graph captured on
             # it and this graph's replays on any stream have nothing of it in common
             ws = torch.empty(self.L.tb_cuda_kv_attend_ws(), dtype=torch.uint8, device=self.device)
@@ -312,6 +337,8 @@ class PagedKV:
         """Attention of the batch's new tokens over their sequences' positions (tb_cuda_kv_attend_dev)."""
         heads, dim, dev = q.shape[1] if q.dim() == 3 else 0, self.head_dim, self.device
         self._tokens(batch, q)
+        if not (0 <= window < 2 ** 31 and 0 <= sinks < 2 ** 31 and 0 <= layer < self.n_layers):
+            raise ValueError(f"layer {layer} of {self.n_layers}, window {window}, {sinks} first tokens")
         rq = _rows(q, heads, dim, dev)
         if out is None:
             out = torch.empty_like(q)
@@ -333,7 +360,7 @@ class PagedKV:
 
     def copy_pages(self, src, dst) -> None:
         """Pages dst[i] = pages src[i], K and V of every layer; host sequences of page numbers."""
-        src, dst = np.ascontiguousarray(src, dtype=np.int32), np.ascontiguousarray(dst, dtype=np.int32)
+        src, dst = _ints(src, "src"), _ints(dst, "dst")
         if src.ndim != 1 or src.shape != dst.shape:
             raise ValueError("src and dst: page numbers, one for one")
         if self._on_device(self.L.tb_cuda_kv_copy_dev, self._ref, src.ctypes.data, dst.ctypes.data, src.size,
@@ -342,7 +369,7 @@ class PagedKV:
 
     def _on_device(self, call, *args) -> int:
         """The entry points launch on the current device: the cache's, for the length of the call."""
-        if torch.cuda.current_device() == self.device.index:
+        if _current_device() == self.device.index:
             return call(*args)
         with torch.cuda.device(self.device):
             return call(*args)
