@@ -270,8 +270,7 @@ __global__ void __launch_bounds__(FewCfg<HD, TI, TC>::W * 32, FewCfg<HD, TI, TC>
                 pg = -1;
                 if (my < ic.sl.n) {
                     const int j = (my < ic.sl.ns ? my : my - ic.sl.ns + ic.sl.lo) * kSlice;
-                    pg = __ldg(a.b.pages + static_cast<long long>(ic.s) * a.b.pages_stride +
-                               fdiv(static_cast<uint32_t>(j), a.c.page_div));
+                    pg = a.b.pages[static_cast<long long>(ic.s) * a.b.pages_stride + fdiv(static_cast<uint32_t>(j), a.c.page_div)];
                 }
             }
             const int page = __shfl_sync(0xFFFFFFFFu, pg, ic.step - pg_base);

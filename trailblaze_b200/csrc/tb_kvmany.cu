@@ -230,7 +230,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                     const int p = p0 + lane * a.box;
                     if (lane < boxes && kv_item_sees(a.a, it, p, a.box)) {
                         const uint32_t pi = fdiv(static_cast<uint32_t>(p), a.a.c.page_div);
-                        page = __ldg(a.a.b.pages + static_cast<long long>(it.s) * a.a.b.pages_stride + pi);
+                        page = a.a.b.pages[static_cast<long long>(it.s) * a.a.b.pages_stride + pi];
                         pos = p - static_cast<int>(pi) * a.a.c.page_size;
                         if (page < 0 || page >= a.a.c.n_pages) {
                             atomicExch(err, ERR_RUNTIME);

@@ -237,7 +237,7 @@ __global__ void __launch_bounds__(kTfThreads, 1)
                     const int p = p0 + lane * a.box;
                     if (lane < boxes && kv_item_sees(aa, it, p, a.box)) {
                         const uint32_t pi = fdiv(static_cast<uint32_t>(p), aa.c.page_div);
-                        page = __ldg(aa.b.pages + static_cast<long long>(it.s) * aa.b.pages_stride + pi);
+                        page = aa.b.pages[static_cast<long long>(it.s) * aa.b.pages_stride + pi];
                         pos = p - static_cast<int>(pi) * aa.c.page_size;
                         if (page < 0 || page >= aa.c.n_pages) {
                             atomicExch(err, ERR_RUNTIME);

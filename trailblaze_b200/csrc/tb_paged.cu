@@ -175,7 +175,7 @@ __global__ void __launch_bounds__(256, 2) k_kv_append(const __grid_constant__ Ap
         cs[e] = 1.f, sn[e] = 0.f;
         if (e < n_turn) {
             const bool second = a.inter ? (e & 1) : d >= half;
-            const float2 v = __ldg(angles + (a.inter ? d >> 1 : second ? d - half : d));
+            const float2 v = angles[a.inter ? d >> 1 : second ? d - half : d];
             cs[e] = v.x;
             sn[e] = second ? v.y : -v.y;
         }
@@ -189,8 +189,8 @@ __global__ void __launch_bounds__(256, 2) k_kv_append(const __grid_constant__ Ap
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const int d = d0 + e, m = e >= n_turn ? d : MODE == TURN_PAIRS ? d ^ 1 : d >= half ? d - half : d + half;
-                wd[e] = __ldg(nw + d);
-                wm[e] = __ldg(nw + m);
+                wd[e] = nw[d];
+                wm[e] = nw[m];
             }
         }
         for (; h - grp < n; h += U * step, p += U * inc, o += U * o_inc) {

@@ -46,7 +46,9 @@ int kv_attend_launch(const KvView &c, const KvBatch &b, int hd, int ti, int tc, 
 
 // Launch with programmatic stream serialization: the kernels of the paged cache
 // begin with griddepcontrol.wait (after what needs no other kernel's data), so a
-// launch's start-up overlaps the end of the one before it.  1 = launched.
+// launch's start-up overlaps the end of the one before it.  Nothing that a kernel may
+// write is read by __ldg: the grid lives while the one before it still writes, and such a
+// load may be moved ahead of the wait.  1 = launched.
 inline int kv_launch(const void *fn, dim3 grid, unsigned threads, size_t smem, void **args, cudaStream_t st)
 {
     cudaLaunchAttribute attr[1];
