@@ -119,3 +119,15 @@ def test_many_items_with_hidden_values(paged, kq, io, cache, every):  # noqa: F8
     at = [lens[r // 20] - 20 + r % 20 + 1 for r in rows]
     ref, bound = R.attend(c.q[rows], c.k[1], c.v[1], list(range(len(rows) + 1)), at, [c.table[r // 20] for r in rows], 1 / 8)
     assert bool(((got[rows].double() - ref).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("cache", [F32, F16, BF16])
+@pytest.mark.parametrize("new,length", [(1, 40), (40, 64)])
+def test_products_beyond_fp32(paged, kq, cache, new, length):  # noqa: F811
+    """Queries so large that q . k leaves fp32 while scale * q . k does not: rows like any other."""
+    c = Case(paged, [new], [length], 4, 2, 64, F32, cache, 16, seed=53)
+    q, scale = c.q * 2.0 ** 125, 2.0 ** -125 / 8
+    c.k.mul_(2.0)
+    got = c.cache.attend(1, c.batch, q, scale=scale)
+    ref, bound = R.attend(q, c.k[1], c.v[1], c.start, c.lens, c.table, scale)
+    assert bool(((got.double() - ref).abs() <= bound).all())

@@ -209,6 +209,8 @@ __device__ __forceinline__ void kv_rows_attend(const AttnArgs &a, const I *const
         if (i[r] >= 0) first = max(first, sp[r].first), lo = min(lo, sp[r].lo), open |= 1u << r;
         last = max(last, i[r]);
         kv_load8(q[r] + d0, qq[r]);
+#pragma unroll
+        for (int d = 0; d < 8; ++d) qq[r][d] *= a.scale2;   // before the products: they may leave fp32 without
         m[r] = -INFINITY, l[r] = 0.f;
 #pragma unroll
         for (int d = 0; d < 8; ++d) acc[r][d] = 0.f;
@@ -258,7 +260,7 @@ __device__ __forceinline__ void kv_rows_attend(const AttnArgs &a, const I *const
                     }
                 for (; o > 0; o >>= 1) sc[0] += __shfl_xor_sync(0xFFFFFFFFu, sc[0], o);
                 const float mine = __shfl_sync(0xFFFFFFFFu, sc[0], lane % RW * LR + lane / RW % U * (LR / U));
-                if (lane / (U * RW) == k0 / (U * RW) && (see[r] >> lane & 1u)) x[r] = mine * a.scale2;
+                if (lane / (U * RW) == k0 / (U * RW) && (see[r] >> lane & 1u)) x[r] = mine;
             }
         }
 #pragma unroll
