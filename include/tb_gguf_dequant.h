@@ -415,9 +415,10 @@ typedef struct {
  * that a row of the table has (0: pages_stride); none past them is read, and
  * rows may overlap.
  * A sequence whose range leaves [0, n_tokens], whose new tokens outnumber its
- * positions or whose positions outnumber its table's (or 2^31 - 256) sets the error word (2)
- * and is skipped, its rows of the output zero; so does a page outside the
- * pool, whose positions then count as hidden and are not stored to. */
+ * positions or whose positions outnumber its table's (or 2^31 - 256) sets the
+ * error word (2) and is skipped, its rows of the output zero; so does a page
+ * outside the pool, whose positions then count as hidden and are not stored to
+ * (append: their rows of q_out are zero). */
 typedef struct {
     const int *d_start, *d_len, *d_pages;
     int        n_seqs, n_tokens, max_new, max_len, pages_stride, pages_width;
@@ -484,11 +485,11 @@ int    tb_cuda_kv_append_dev(const tb_kv_cache *cache, int layer, const tb_kv_ba
  * entries for pages that no row of the call sees are not looked at.  Scores,
  * softmax and sums are fp32; fp32 activations keep fp32 accuracy over any
  * cache type; 16-bit activations over a cache of the same type may round the
- * softmax numerators to that type before the second product.  d_ws: workspace
- * of tb_cuda_kv_attend_ws() bytes, 16-byte aligned, its first
- * TB_KV_WS_ZEROED bytes zeroed once before its first call; every call leaves it ready for the next, one that ends with an
- * error word too.  Calls that may overlap on the GPU need one each.
- * Stream-ordered.  1 = issued. */
+ * softmax numerators to that type before the second product.  out must not
+ * overlap q.  d_ws: workspace of tb_cuda_kv_attend_ws() bytes, 16-byte aligned,
+ * its first TB_KV_WS_ZEROED bytes zeroed once before its first call; every call
+ * leaves it ready for the next, one that ends with an error word too.  Calls
+ * that may overlap on the GPU need one each.  Stream-ordered.  1 = issued. */
 #define TB_KV_WS_ZEROED 2048
 size_t tb_cuda_kv_attend_ws(void);
 int    tb_cuda_kv_attend_dev(const tb_kv_cache *cache, int layer, const tb_kv_batch *batch, int io_type, int n_heads,

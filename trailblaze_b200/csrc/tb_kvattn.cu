@@ -34,9 +34,10 @@
 // sums are fp32.
 //
 // Measured (8 kv heads of 128, 4 query heads each): 64 sequences of up to 16384 bf16
-// positions, 2.07 GB, in 306 us, 6.76 TB/s, what a copy reaches; one sequence of 4096
-// fp32 positions, 33.6 MB, in 19 us against 5 us of bytes: launch, scan, the first
-// page, Q and the joining of 16 parts stand one behind the other there.
+// positions, 2.07 GB, in 307 to 338 us by the GPU, 6.1 to 6.7 TB/s, where a copy reaches
+// 6.5; one sequence of 4096 fp32 positions, 33.6 MB, in 19 us against 5 us of bytes:
+// launch, scan, the first page, Q and the joining of 16 parts stand one behind the other
+// there.
 #include "../../include/tb_gguf_dequant.h"
 #include "tb_kvattn.cuh"
 

@@ -33,8 +33,9 @@
 // numerators lie 2^7 higher, up to 2^15, so that what it cannot hold lies 2^-32 below
 // the largest.
 //
-// Measured (32 query and 8 kv heads of 128, bf16): 8192 tokens from the start in 504
-// us, 1092 TFLOP/s of the pairs that are seen; 512 tokens at 4096 in 48 us.  A unit
+// Measured (32 query and 8 kv heads of 128, bf16): 8192 tokens from the start in 559
+// us, 983 TFLOP/s of the pairs that are seen (call after call under the power cap; 500
+// to 510 us in a burst of 20); 512 tokens at 4096 in 46 us.  A unit
 // takes some 3000 cycles, 2048 of them tensor pipe: what is left is the way from the
 // last P over P V and the next S back to the softmax warps (1200) and their 128
 // exponentials a row (1024 of the multi-function unit), which the other group's

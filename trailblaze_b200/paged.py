@@ -334,7 +334,8 @@ class PagedKV:
     def attend(self, layer: int, batch: Batch, q: torch.Tensor, out: torch.Tensor | None = None,
                scale: float | None = None, window: int = 0, sinks: int = 0,
                workspace: torch.Tensor | None = None) -> torch.Tensor:
-        """Attention of the batch's new tokens over their sequences' positions (tb_cuda_kv_attend_dev)."""
+        """Attention of the batch's new tokens over their sequences' positions (tb_cuda_kv_attend_dev); out must not
+        overlap q."""
         heads, dim, dev = q.shape[1] if q.dim() == 3 else 0, self.head_dim, self.device
         self._tokens(batch, q)
         if not (0 <= window < 2 ** 31 and 0 <= sinks < 2 ** 31 and 0 <= layer < self.n_layers):
