@@ -613,35 +613,89 @@ __device__ __noinline__ void kv_leave(const AttnArgs &a, int tpi, int few_rows, 
         atomicSub(a.arrived + cta, WARPS * static_cast<int>(share.of(u + it.n - 1) - cta));
 }
 
-// The chunk kernels' rows that have to be done again, a warp's: they wait until its last item
-// is out.  In the loop over the items the call cost a long prompt 3 % without being made, and
-// while a warp was at it the CTA's others would sit in bounded waits.  3000 bf16 tokens of 8
-// heads whose first V is NaN: 5.0 ms, against 0.06 without and 66 a row and a position at a
-// time.
-struct KvAgain {   // shared, n zero at first
+// True when V is finite in the positions [j0, j1) of a head (those of pages that are none
+// count as that), by the whole warp.
+template <int HD, class E>
+__device__ __forceinline__ bool kv_finite(const AttnArgs &a, int s, int h, int j0, int j1)
+{
+    constexpr int LR = HD / 8, RW = 32 / LR, U = 4;
+    const int lane = threadIdx.x & 31, grp = lane / LR;
+    const E *vp = static_cast<const E *>(a.c.v) + lane % LR * 8;
+    float nil = 0.f;
+    for (int j = j0; j < j1; j += 32) {
+        const long long at = j + lane < j1 ? kv_at(a.b, a.c, s, j + lane, h, nullptr) : -1;
+#pragma unroll 1
+        for (int k0 = 0; k0 < 32; k0 += U * RW) {
+            float v[U][8];
+            bool on[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const long long va = __shfl_sync(0xFFFFFFFFu, at, k0 + u * RW + grp);
+                on[u] = va >= 0;
+                kv_load8(vp + (va < 0 ? 0 : va), v[u]);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int d = 0; d < 8; ++d) nil = on[u] ? fmaf(v[u][d], 0.f, nil) : nil;
+        }
+    }
+    return !__any_sync(0xFFFFFFFFu, !(nil == 0.f));
+}
+
+// The chunk kernels' rows that are not finite, a warp's: they wait until its last item is out.
+// In the loop over the items a call from here cost a long prompt 3 % without being made, and
+// while a warp was at it the CTA's others would sit in bounded waits.
+// Two things lead here: what a row sees, and 0 times what its tiles hold besides.  The
+// second needs a V that is not finite where the tiles pass the rows' ends or the window:
+// LOOK looks there, and where there is none the rows stay as they are: 3000 bf16 tokens of 8
+// heads whose first V is NaN take 92 us, 62 without (5.0 ms with every row done again, 66 a
+// position at a time).  Not for operands in parts, to which an infinity is NaN.
+struct KvAgain {   // shared, n and must zero at first
     static constexpr int CAP = 4;
-    int n;   // past CAP: all rows of the CTA's items
+    int n;      // past CAP: all rows of the CTA's items
+    int must;   // an item has a page outside the pool
     struct {
         unsigned rows;
-        int row0, t0, p0, s, h;   // the sequence's first row, the row group's first token, the position of token 0
+        int t0, s, h, must;   // the row group's first token
     } rec[CAP];
-    __device__ __forceinline__ void add(unsigned rows, int row0, int t0, int p0, int s, int h)   // one thread
+    __device__ __forceinline__ void add(unsigned rows, int t0, int s, int h, bool bad)   // one thread
     {
-        if (n < CAP) rec[n] = {rows, row0, t0, p0, s, h};
+        if (n < CAP) rec[n] = {rows, t0, s, h, bad};
         ++n;
+        must |= bad;
     }
 };
 // lists: of the warps from warp0 on, four to a row group of tpt tokens.
-template <int HD, class I, class E, int TILE>
+template <int HD, class I, class E, int TILE, bool LOOK>
 __device__ __noinline__ void kv_again(const AttnArgs &a, const KvAgain *lists, int warp0, int tpt, int tpi, int few_rows, const KvScan &sh)
 {
     const int w = (threadIdx.x >> 5) - warp0, tok0 = (w >> 2) * tpt;
     const int r = (w & 3) * 32 + (threadIdx.x & 31), tok_in = r / a.group, hh = r - tok_in * a.group;
     const KvAgain &todo = lists[w];
+    // rows of row tile rt of sequence s, head h, the lane's at position pos
+    auto again = [&](unsigned rows, int s, int h, const KvSeq &q, int rt, int tok, bool must) {
+        if (!rows) return;
+        const int pos = q.len - q.n + tok;
+        if (LOOK && !must) {
+            KvItem it;
+            kv_item_tiles<TILE>(a, tpi, q, rt, &it);
+            const int low = __shfl_sync(0xFFFFFFFFu, pos, __ffs(rows) - 1), high = __shfl_sync(0xFFFFFFFFu, pos, 31 - __clz(rows));
+            const int end = min(q.len, ((q.len - q.n + it.t1 - 1) / TILE + 1) * TILE);
+            const KvSpan s0 = kv_span(low, a.window, a.sinks), s1 = kv_span(high, a.window, a.sinks);
+            // past the first row's position, and between the first tokens and the last row's window
+            if (kv_finite<HD, E>(a, s, h, low + 1, end) && kv_finite<HD, E>(a, s, h, s0.first, min(s1.lo, it.ns * TILE)) &&
+                kv_finite<HD, E>(a, s, h, max(s0.first, it.lo * TILE), s1.lo))
+                return;
+        }
+        kv_rows_again<HD, I, E>(a, rows, q.row0 + tok, h * a.group + hh, pos, s, h);
+    };
     if (todo.n <= KvAgain::CAP) {
         for (int k = 0; k < todo.n; ++k) {
             const auto &x = todo.rec[k];
-            kv_rows_again<HD, I, E>(a, x.rows, x.row0 + x.t0 + tok_in, x.h * a.group + hh, x.p0 + x.t0 + tok_in, x.s, x.h);
+            KvSeq q;
+            kv_seq(a.b, a.c, x.s, q, nullptr);
+            again(x.rows, x.s, x.h, q, x.t0 / tpi, x.t0 + tok_in, x.must);
         }
         return;
     }
@@ -653,7 +707,7 @@ __device__ __noinline__ void kv_again(const AttnArgs &a, const KvAgain *lists, i
     for (unsigned long long u = share.start(cta);;) {
         const int tok = it.t0 + tok0 + tok_in;
         const unsigned rows = __ballot_sync(0xFFFFFFFFu, j0 == 0 && tok_in < tpt && tok < it.t1);
-        kv_rows_again<HD, I, E>(a, rows, it.q.row0 + tok, it.h * a.group + hh, it.q.len - it.q.n + tok, it.s, it.h);
+        again(rows, it.s, it.h, it.q, it.rt, tok, todo.must);
         u += it.n - j0;
         if (u >= u1) break;
         j0 = 0;

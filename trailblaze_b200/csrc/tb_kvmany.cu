@@ -159,7 +159,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         sh.fail = 0;
         for (int i = 0; i < 8; ++i) sh.bad[i] = 0;
         sh.owed = KvOwed{};
-        for (int i = 0; i < 8; ++i) sh.again[i].n = 0;
+        for (int i = 0; i < 8; ++i) sh.again[i].n = sh.again[i].must = 0;
     }
     if (warp == 9 && lane < 2) prefetch_map(lane ? &vmap : &kmap);
     if (warp == 10 && lane == 0) prefetch_map(&qmap);
@@ -614,6 +614,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                 I *out = static_cast<I *>(const_cast<void *>(a.a.o.p));
                 const long long off = on ? (it.row0 + tok) * a.a.o.row + (it.h * a.a.group + hh) * a.a.o.head : -1;
                 I *mine = reinterpret_cast<I *>(stage + warp * Cfg::STAGE);   // [32 rows][64], 16-byte pieces swizzled
+                const bool bad_page = odd;
                 const float inv = L == 0.f ? 0.f : 1.0f / L;
                 // Rolled, since this code comes by once an item: unrolled, it would come from
                 // beyond the instruction cache every time.
@@ -650,12 +651,15 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                 // rows that are not finite: V of a position that a row does not see may have been
                 // (0 * NaN), or a page lies outside the pool.  Once more at the end, over their own positions only.
                 const unsigned rows = __ballot_sync(0xFFFFFFFFu, odd && on);
-                if (rows && lane == 0) sh.again[warp].add(rows, it.row0, it.t0 + g * a.tpt, p0, it.s, it.h);
+                if (rows) {
+                    const bool must = __any_sync(0xFFFFFFFFu, bad_page && on);
+                    if (lane == 0) sh.again[warp].add(rows, it.t0 + g * a.tpt, it.s, it.h, must);
+                }
             }
         }
         if (tell >= 0) told();
         __syncwarp();
-        if (sh.again[warp].n > 0) kv_again<HD, I, I, kTileN>(a.a, sh.again, 0, a.tpt, a.tpi, a.few_rows, sh.scan);
+        if (sh.again[warp].n > 0) kv_again<HD, I, I, kTileN, true>(a.a, sh.again, 0, a.tpt, a.tpi, a.few_rows, sh.scan);
     }
     // ---- the end: nothing in flight, TMEM given back ----
     tc_fence_before();

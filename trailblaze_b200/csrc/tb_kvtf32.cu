@@ -178,7 +178,7 @@ __global__ void __launch_bounds__(kTfThreads, 1)
         sh.fail = 0;
         for (int i = 0; i < 8; ++i) sh.bad[i] = 0;
         sh.owed = KvOwed{};
-        for (int i = 0; i < 4; ++i) sh.again[i].n = 0;
+        for (int i = 0; i < 4; ++i) sh.again[i].n = sh.again[i].must = 0;
     }
     if (warp >= 14 && lane == 0) prefetch_map(warp == 15 ? &vmap : &kmap);
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -706,14 +706,14 @@ __global__ void __launch_bounds__(kTfThreads, 1)
                 // (0 * NaN), or a page lies outside the pool.  Once more at the end, over their own positions only.
                 __syncwarp();
                 const unsigned rows = __ballot_sync(0xFFFFFFFFu, odd && on);
-                if (rows && lane == 0) sh.again[warp - 4].add(rows, it.q.row0, it.t0, it.q.len - it.q.n, it.s, it.h);
+                if (rows && lane == 0) sh.again[warp - 4].add(rows, it.t0, it.s, it.h, true);
             }
             ++items;
             next_item(j1);
         }
         if (tell >= 0) told();
         __syncwarp();
-        if (sh.again[warp - 4].n > 0) kv_again<HD, I, E, kTfTile>(aa, sh.again, 4, a.tpi, a.tpi, a.few_rows, sh.scan);
+        if (sh.again[warp - 4].n > 0) kv_again<HD, I, E, kTfTile, false>(aa, sh.again, 4, a.tpi, a.tpi, a.few_rows, sh.scan);
     }
     // ---- the end: nothing in flight, TMEM given back ----
     tc_fence_before();
